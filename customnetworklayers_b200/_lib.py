@@ -5,7 +5,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_int, c_longlong, c_ulonglong, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_ulonglong, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libcnl_b200.so")
@@ -46,6 +46,17 @@ SIGNATURES = {
     "cnl_wmedian_forward": (c_int, [c_void_p] * 5 + [c_int] * 5 + [c_void_p]),
     "cnl_wmedian_backward": (c_int, [c_void_p] * 8 + [c_int] * 5 + [c_void_p]),
     "cnl_wmedian_scratch_bytes": (c_longlong, [c_int]),
+    "cnl_ckpt8_store": (c_int, [c_void_p] * 3 + [c_longlong, c_int, c_int, c_void_p]),
+    "cnl_ckpt8_restore": (c_int, [c_void_p] * 3 + [c_longlong, c_int, c_int, c_void_p]),
+    "cnl_act8_forward": (c_int, [c_void_p] * 4 + [c_longlong] + [c_int] * 3 + [c_void_p]),
+    "cnl_act8_backward": (c_int, [c_void_p] * 4 + [c_longlong] + [c_int] * 3 + [c_void_p]),
+    "cnl_blocknorm_scratch_bytes": (c_longlong, [c_longlong, c_int, c_longlong]),
+    "cnl_blocknorm_forward": (c_int, [c_void_p] * 13 + [c_longlong, c_int, c_longlong] + [c_int] * 3 + [c_float] + [c_int] * 3 + [c_void_p]),
+    "cnl_blocknorm_backward": (c_int, [c_void_p] * 22 + [c_longlong, c_int, c_longlong] + [c_int] * 6 + [c_void_p]),
+    "cnl_linattn_segments": (c_int, [c_int] * 3),
+    "cnl_linattn_forward": (c_int, [c_void_p] * 10 + [c_int] * 5 + [c_float, c_int, c_void_p]),
+    "cnl_linattn_backward": (c_int, [c_void_p] * 15 + [c_int] * 5 + [c_float, c_int, c_void_p]),
+    "cnl_linattn_step": (c_int, [c_void_p] * 7 + [c_int] * 4 + [c_float, c_int, c_void_p]),
     "cnl_last_error": (c_char_p, []),
     "cnl_version": (c_char_p, []),
 }
@@ -55,6 +66,11 @@ OPT_FUSE = 2
 OPT_TIMING = 3
 OPT_RECOMPUTE = 4
 OPT_FLOW = 5
+
+# element types, checkpoint formats and activations of the network operators (include/cnl_b200.h)
+F32, F16, BF16 = 0, 1, 2
+CKPT_NONE, CKPT_INT8, CKPT_E4M3 = 0, 1, 2
+ACT_GELU, ACT_SILU = 1, 2
 
 _lib = None
 

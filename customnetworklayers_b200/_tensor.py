@@ -1,0 +1,43 @@
+"""Argument checks and launch plumbing shared by the network operators (`ckpt8`, `blocknorm`, `linattn`)."""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+DTYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+
+
+def check_tensor(t, name: str, dtype=None, device=None, shape=None, contiguous: bool = True) -> None:
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if contiguous and not t.is_contiguous():
+        raise RuntimeError(f"{name} must be contiguous")
+    if dtype is None:
+        if t.dtype not in DTYPES:
+            raise RuntimeError(f"{name} must be float32, float16 or bfloat16, not {t.dtype}")
+    elif t.dtype != dtype:
+        raise RuntimeError(f"{name} must be {dtype}, not {t.dtype}")
+    if device is not None and t.device != device:
+        raise RuntimeError(f"{name} must be on {device}, not on {t.device}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise RuntimeError(f"{name} must have shape {list(shape)}, not {list(t.shape)}")
+
+
+def ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def launch(what: str, fn, device, *args) -> None:
+    """fn(*args, stream) on the current stream of `device`, with that device current."""
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc != 0:
+        _lib.check(rc, what)
+
+
+def wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)

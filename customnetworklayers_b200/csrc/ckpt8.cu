@@ -1,0 +1,284 @@
+// Activations kept in 8 bits: store, restore, and activations whose forward pass leaves the codes of its input and whose
+// backward pass reads them (format: ckpt8.cuh).
+//
+// Every kernel is one pass over memory and HBM bound: b + 1 + 1/32 bytes an element for store and restore, 2 b + 1 + 1/32
+// for the activations (b = 2 or 4).  A lane holds one 16-byte vector, so a block of 32 elements lies in 4 (16-bit types) or
+// 8 (fp32) neighbouring lanes and its maximum costs two or three shuffles; four vectors a thread are loaded before the first
+// is used.  Addresses that are not 16-byte aligned take the same code with one element a lane.
+#include "ckpt8.cuh"
+
+#include <type_traits>
+
+namespace cnl {
+namespace ckpt8 {
+
+constexpr int kThreads = 256;
+constexpr int kUnroll = 4;
+
+// Phi(x) = exp(-x^2/2) t P(t) for x <= 0, t = 1 / (1 + 0.3 |x|), and 1 - that for x > 0.  P was fitted here to the scaled
+// complementary error function by least squares with weights moved towards an even relative error over |x| <= 14:
+// 8.2e-6 with degree 5 (a 64th of fp16's half step), 1.6e-7 with degree 7.
+template <typename T>
+__device__ __forceinline__ float cdf_tail(float x) {                     // t P(t)
+    const float t = __fdividef(1.0f, fmaf(0.3f, fabsf(x), 1.0f));
+    float p;
+    if constexpr (sizeof(T) == 4) {
+        p = fmaf(t, 0.03567475825548172f, -0.15720295906066895f);
+        p = fmaf(t, p, 0.20635318756103516f);
+        p = fmaf(t, p, -0.053683266043663025f);
+        p = fmaf(t, p, 0.12856139242649078f);
+        p = fmaf(t, p, 0.0999135747551918f);
+        p = fmaf(t, p, 0.1207539439201355f);
+        p = fmaf(t, p, 0.11962930113077164f);
+    } else {
+        p = fmaf(t, -0.0770978331565857f, 0.21603818237781525f);
+        p = fmaf(t, p, -0.0169492457062006f);
+        p = fmaf(t, p, 0.14419695734977722f);
+        p = fmaf(t, p, 0.11374179273843765f);
+        p = fmaf(t, p, 0.12007424235343933f);
+    }
+    return t * p;
+}
+
+template <int ACT, typename T>
+__device__ __forceinline__ float act(float x) {
+    if constexpr (ACT == CNL_ACT_GELU) {
+        const float e = __expf(-0.5f * x * x);
+        const float q = cdf_tail<T>(x) * e;
+        return x * (x > 0.0f ? 1.0f - q : q);
+    } else {
+        return __fdividef(x, 1.0f + __expf(-x));
+    }
+}
+
+template <int ACT, typename T>
+__device__ __forceinline__ float act_slope(float x) {
+    if constexpr (ACT == CNL_ACT_GELU) {
+        const float e = __expf(-0.5f * x * x);
+        const float q = cdf_tail<T>(x) * e;
+        return fmaf(x * 0.3989422804014327f, e, x > 0.0f ? 1.0f - q : q);
+    } else {
+        const float e = __expf(-fabsf(x));                       // never overflows; e / (1 + e)^2 is even in x
+        const float r = __fdividef(1.0f, 1.0f + e);
+        return fmaf(x * e, r * r, x >= 0.0f ? r : e * r);
+    }
+}
+
+// V consecutive elements from `at` (0 beyond count); V > 1 reads 16 bytes where they all exist.
+template <typename T, int V>
+__device__ __forceinline__ void read(const T* __restrict__ x, long long at, long long count, float (&v)[V]) {
+    if (V > 1 && at + V <= count) {
+        if constexpr (V > 1) load_vec<T, V>(x + at, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = at + i < count ? to_f32(x[at + i]) : 0.0f;
+    }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void write(T* __restrict__ x, long long at, long long count, const float (&v)[V]) {
+    if (V > 1 && at + V <= count) {
+        if constexpr (V > 1) store_vec<T, V>(x + at, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (at + i < count) x[at + i] = from_f32<T>(v[i]);
+    }
+}
+
+template <int V>
+__device__ __forceinline__ void write_codes(unsigned char* __restrict__ codes, long long at, long long count, const unsigned char (&c)[V]) {
+    if (V > 1 && at + V <= count) {
+        unsigned w[(V + 3) / 4] = {};
+#pragma unroll
+        for (int i = 0; i < V; ++i) w[i / 4] |= (unsigned)c[i] << (8 * (i % 4));
+        if constexpr (V == 8) *reinterpret_cast<uint2*>(codes + at) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<unsigned*>(codes + at) = w[0];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (at + i < count) codes[at + i] = c[i];
+    }
+}
+
+template <int V>
+__device__ __forceinline__ void read_codes(const unsigned char* __restrict__ codes, long long at, long long count, unsigned (&w)[(V + 3) / 4]) {
+    if (V > 1 && at + V <= count) {
+        if constexpr (V == 8) {
+            const uint2 q = __ldg(reinterpret_cast<const uint2*>(codes + at));
+            w[0] = q.x; w[(V + 3) / 4 - 1] = q.y;
+        } else w[0] = __ldg(reinterpret_cast<const unsigned*>(codes + at));
+    } else {
+#pragma unroll
+        for (int i = 0; i < (V + 3) / 4; ++i) w[i] = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (at + i < count) w[i / 4] |= (unsigned)codes[at + i] << (8 * (i % 4));
+    }
+}
+
+// x -> codes, scales (if not null) and, with ACT, y = act(x)
+template <typename T, int V, int FMT, int ACT>
+__global__ void __launch_bounds__(kThreads) store_kernel(const T* __restrict__ x, T* __restrict__ y, unsigned char* __restrict__ codes,
+                                                         unsigned char* __restrict__ scales, long long count) {
+    constexpr int kLanes = kBlock / V;
+    const long long first = ((long long)blockIdx.x * kUnroll * kThreads + threadIdx.x) * V;
+    float v[kUnroll][V];
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) read<T, V>(x, first + (long long)j * kThreads * V, count, v[j]);
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+        const long long at = first + (long long)j * kThreads * V;
+        if (codes) {                                              // the same for the whole grid
+            unsigned char c[V];
+            const int s = encode<FMT, kLanes, V>(v[j], c);
+            write_codes<V>(codes, at, count, c);
+            if (at < count && (threadIdx.x & (kLanes - 1)) == 0) scales[at / kBlock] = scale_byte(s);
+        }
+        if constexpr (ACT != 0) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[j][i] = act<ACT, T>(v[j][i]);
+            write<T, V>(y, at, count, v[j]);
+        }
+    }
+}
+
+// codes, scales -> x, or with ACT g_x = g_y * act'(x)
+template <typename T, int V, int FMT, int ACT>
+__global__ void __launch_bounds__(kThreads) restore_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
+                                                           const T* __restrict__ g, T* __restrict__ out, long long count) {
+    const long long first = ((long long)blockIdx.x * kUnroll * kThreads + threadIdx.x) * V;
+    unsigned w[kUnroll][(V + 3) / 4];
+    int s[kUnroll];
+    float gv[kUnroll][V];
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+        const long long at = first + (long long)j * kThreads * V;
+        read_codes<V>(codes, at, count, w[j]);
+        s[j] = at < count ? scale_exponent(__ldg(scales + at / kBlock)) : 0;
+        if constexpr (ACT != 0) read<T, V>(g, at, count, gv[j]);
+    }
+    constexpr int kSafe = std::is_same<T, __half>::value ? 7 : 118;                   // no code can leave the type's range up to here
+    constexpr float kTop = std::is_same<T, float>::value ? 3.402823466e38f : std::is_same<T, __half>::value ? 65504.0f : 3.38953139e38f;
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+        const long long at = first + (long long)j * kThreads * V;
+        float v[V];
+        decode<FMT, V>(w[j], s[j], v);
+        if constexpr (ACT != 0) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = gv[j][i] * act_slope<ACT, T>(v[i]);
+        } else if (s[j] > kSafe) {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (fabsf(v[i]) > kTop) v[i] = copysignf(kTop, v[i]);
+        }
+        write<T, V>(out, at, count, v);
+    }
+}
+
+template <int V>
+inline int grid_for(long long count, unsigned* grid) {
+    const long long per = (long long)kThreads * kUnroll * V, blocks = (count + per - 1) / per;
+    if (blocks > 0x7fffffffLL) return fail(CNL_ERR_BAD_SHAPE, "count %lld is too large", count);
+    *grid = (unsigned)blocks;
+    return CNL_OK;
+}
+
+template <typename T, int FMT, int ACT>
+int run_store(const void* x, void* y, unsigned char* codes, unsigned char* scales, long long count, cudaStream_t st) {
+    constexpr int V = 16 / (int)sizeof(T);
+    unsigned grid = 0;
+    // one element a lane where a pointer is not aligned (a view that starts at an odd element)
+    if (aligned16(x) && aligned16(y) && aligned16(codes)) {
+        CNL_TRY(grid_for<V>(count, &grid));
+        store_kernel<T, V, FMT, ACT><<<grid, kThreads, 0, st>>>((const T*)x, (T*)y, codes, scales, count);
+    } else {
+        CNL_TRY(grid_for<1>(count, &grid));
+        store_kernel<T, 1, FMT, ACT><<<grid, kThreads, 0, st>>>((const T*)x, (T*)y, codes, scales, count);
+    }
+    return after_launch("ckpt8 store");
+}
+
+template <typename T, int FMT, int ACT>
+int run_restore(const unsigned char* codes, const unsigned char* scales, const void* g, void* out, long long count, cudaStream_t st) {
+    constexpr int V = 16 / (int)sizeof(T);
+    unsigned grid = 0;
+    if (aligned16(g) && aligned16(out) && aligned16(codes)) {
+        CNL_TRY(grid_for<V>(count, &grid));
+        restore_kernel<T, V, FMT, ACT><<<grid, kThreads, 0, st>>>(codes, scales, (const T*)g, (T*)out, count);
+    } else {
+        CNL_TRY(grid_for<1>(count, &grid));
+        restore_kernel<T, 1, FMT, ACT><<<grid, kThreads, 0, st>>>(codes, scales, (const T*)g, (T*)out, count);
+    }
+    return after_launch("ckpt8 restore");
+}
+
+int check(long long count, int dtype, int fmt) {
+    if (count < 0) return fail(CNL_ERR_BAD_SHAPE, "count %lld is negative", count);
+    CNL_TRY(check_dtype(dtype));
+    if (fmt != CNL_CKPT_INT8 && fmt != CNL_CKPT_E4M3) return fail(CNL_ERR_BAD_OPTION, "fmt %d is not CNL_CKPT_INT8 or CNL_CKPT_E4M3", fmt);
+    return CNL_OK;
+}
+
+int check_act(int act) {
+    if (act != CNL_ACT_GELU && act != CNL_ACT_SILU) return fail(CNL_ERR_BAD_OPTION, "act %d is not CNL_ACT_GELU or CNL_ACT_SILU", act);
+    return CNL_OK;
+}
+
+// F<T, FMT, ACT> for the run-time values
+#define CNL_CKPT8_DISPATCH(F, ...)                                                                                      \
+    do {                                                                                                                \
+        const bool i8 = fmt == CNL_CKPT_INT8;                                                                           \
+        if (dtype == CNL_F32) return i8 ? F<float, CNL_CKPT_INT8, ACT>(__VA_ARGS__) : F<float, CNL_CKPT_E4M3, ACT>(__VA_ARGS__);      \
+        if (dtype == CNL_F16) return i8 ? F<__half, CNL_CKPT_INT8, ACT>(__VA_ARGS__) : F<__half, CNL_CKPT_E4M3, ACT>(__VA_ARGS__);    \
+        return i8 ? F<__nv_bfloat16, CNL_CKPT_INT8, ACT>(__VA_ARGS__) : F<__nv_bfloat16, CNL_CKPT_E4M3, ACT>(__VA_ARGS__);            \
+    } while (0)
+
+template <int ACT>
+int store_any(const void* x, void* y, unsigned char* codes, unsigned char* scales, long long count, int dtype, int fmt, cudaStream_t st) {
+    CNL_CKPT8_DISPATCH(run_store, x, y, codes, scales, count, st);
+}
+template <int ACT>
+int restore_any(const unsigned char* codes, const unsigned char* scales, const void* g, void* out, long long count, int dtype, int fmt, cudaStream_t st) {
+    CNL_CKPT8_DISPATCH(run_restore, codes, scales, g, out, count, st);
+}
+
+}  // namespace ckpt8
+}  // namespace cnl
+
+using namespace cnl;
+
+extern "C" int cnl_ckpt8_store(const void* x, unsigned char* codes, unsigned char* scales, long long count, int dtype, int fmt, void* stream) {
+    CNL_TRY(ckpt8::check(count, dtype, fmt));
+    if (count == 0) return CNL_OK;
+    if (!x || !codes || !scales) return fail(CNL_ERR_NULL, "null pointer argument");
+    return ckpt8::store_any<0>(x, nullptr, codes, scales, count, dtype, fmt, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int cnl_ckpt8_restore(const unsigned char* codes, const unsigned char* scales, void* x, long long count, int dtype, int fmt, void* stream) {
+    CNL_TRY(ckpt8::check(count, dtype, fmt));
+    if (count == 0) return CNL_OK;
+    if (!x || !codes || !scales) return fail(CNL_ERR_NULL, "null pointer argument");
+    return ckpt8::restore_any<0>(codes, scales, nullptr, x, count, dtype, fmt, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int cnl_act8_forward(const void* x, void* y, unsigned char* codes, unsigned char* scales, long long count, int dtype, int fmt, int act, void* stream) {
+    CNL_TRY(ckpt8::check(count, dtype, fmt));
+    CNL_TRY(ckpt8::check_act(act));
+    if (count == 0) return CNL_OK;
+    if (!x || !y || !codes != !scales) return fail(CNL_ERR_NULL, "null pointer argument");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (act == CNL_ACT_GELU) return ckpt8::store_any<CNL_ACT_GELU>(x, y, codes, scales, count, dtype, fmt, st);
+    return ckpt8::store_any<CNL_ACT_SILU>(x, y, codes, scales, count, dtype, fmt, st);
+}
+
+extern "C" int cnl_act8_backward(const unsigned char* codes, const unsigned char* scales, const void* g_y, void* g_x, long long count, int dtype, int fmt, int act, void* stream) {
+    CNL_TRY(ckpt8::check(count, dtype, fmt));
+    CNL_TRY(ckpt8::check_act(act));
+    if (count == 0) return CNL_OK;
+    if (!codes || !scales || !g_y || !g_x) return fail(CNL_ERR_NULL, "null pointer argument");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (act == CNL_ACT_GELU) return ckpt8::restore_any<CNL_ACT_GELU>(codes, scales, g_y, g_x, count, dtype, fmt, st);
+    return ckpt8::restore_any<CNL_ACT_SILU>(codes, scales, g_y, g_x, count, dtype, fmt, st);
+}

@@ -37,6 +37,22 @@ int ensure_dynamic_smem(const void* kernel, int bytes) {
     return CNL_OK;
 }
 
+int sm_count(int* out) {
+    static std::mutex mu;
+    static std::map<int, int> known;                             // device -> multiprocessors
+    int dev = 0;
+    CNL_TRY(check_cuda(cudaGetDevice(&dev), "cudaGetDevice"));
+    std::lock_guard<std::mutex> lock(mu);
+    auto it = known.find(dev);
+    if (it == known.end()) {
+        int n = 0;
+        CNL_TRY(check_cuda(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute"));
+        it = known.emplace(dev, n).first;
+    }
+    *out = it->second;
+    return CNL_OK;
+}
+
 }  // namespace cnl
 
 extern "C" const char* cnl_last_error(void) { return cnl::last_error_ref().c_str(); }

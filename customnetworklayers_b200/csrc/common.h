@@ -26,6 +26,9 @@ int ensure_dynamic_smem(const void* kernel, int bytes);
 template <typename K>
 inline int ensure_dynamic_smem(K* kernel, int bytes) { return ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), bytes); }
 
+// Multiprocessors of the current device (queried once per device).
+int sm_count(int* out);
+
 // Counts a launch and turns a launch-configuration error into an error code.
 inline int after_launch(const char* kernel) {
     g_launches.fetch_add(1, std::memory_order_relaxed);

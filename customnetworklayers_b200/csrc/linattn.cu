@@ -1,0 +1,383 @@
+// Linear attention with a decay for each head: drivers, the kernel in fp32 arithmetic, the scan over segments and the
+// single-token step (formulas: linattn.cuh).
+#include "linattn.cuh"
+
+namespace cnl {
+namespace lin {
+
+constexpr int kMaxD = 128;
+constexpr int kC = 32;                       // positions of a chunk
+constexpr int kThreads = 256;
+
+// ---- sweep in fp32 arithmetic -----------------------------------------------------------------------------------
+// A block walks one segment of one head chunk by chunk.  Operands, the C x C product and W lie in shared memory in fp32;
+// every product is plain multiply-adds on 4 x 4 register tiles.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) sweep_kernel(const Sweep s) {
+    extern __shared__ float4 smem4[];
+    const int da = s.da, dc = s.dc, pa = (da + 3) / 4 * 4, pc = (dc + 3) / 4 * 4;
+    const int ra = pa + 4, rc = pc + 4;                          // row strides: 16-byte rows on different banks
+    float* A = reinterpret_cast<float*>(smem4);
+    float* B = A + kC * ra;
+    float* Cc = B + kC * ra;
+    float* W = Cc + kC * rc;
+    float* P = W + pa * rc;
+    const int tid = threadIdx.x;
+    const int seg = blockIdx.x % s.segments, bh = blockIdx.x / s.segments, head = bh % s.h, bat = bh / s.h;
+    const float ld = clamp_log(s.log_decay[head]);
+    const int n = s.lengths ? min(max(s.lengths[bat], 0), s.t) : s.t;
+    const long long first = (long long)seg * s.seg;
+    const int lo = (int)(first < n ? first : n), hi = (int)(first + s.seg < n ? first + s.seg : n);
+    const long long size = (long long)da * dc;
+
+    const float* w0 = s.start ? s.start + ((long long)bh * s.segments + seg) * size : nullptr;
+    for (int e = tid; e < pa * pc; e += kThreads) {
+        const int i = e / pc, j = e - i * pc;
+        W[i * rc + j] = w0 && i < da && j < dc ? (s.transposed ? w0[(long long)j * da + i] : w0[(long long)i * dc + j]) : 0.0f;
+    }
+    for (int c0 = lo; c0 < hi; c0 += kC) {
+        const int m = min(kC, hi - c0);
+        __syncthreads();
+        auto fetch = [&](const Rows& r, float* dst, int d, int stride) {
+            const int p = stride - 4;
+            const T* src = (const T*)r.p + bat * r.sb + head * r.sh;
+            for (int e = tid; e < kC * p; e += kThreads) {
+                const int j = e / p, x = e - j * p;
+                const long long tok = s.reversed ? n - 1 - (c0 + j) : c0 + j;
+                dst[j * stride + x] = j < m && x < d ? to_f32(src[tok * r.st + x]) : 0.0f;
+            }
+        };
+        if (s.out) fetch(s.a, A, da, ra);
+        fetch(s.b, B, da, ra);
+        fetch(s.c, Cc, dc, rc);
+        __syncthreads();
+        if (s.out) {
+            for (int e = tid; e < kC * kC; e += kThreads) {
+                const int i = e / kC, j = e % kC;
+                float v = 0.0f;
+                if (j <= i && i < m) {
+                    for (int x = 0; x < pa; x += 4) {
+                        const float4 p = *reinterpret_cast<const float4*>(A + i * ra + x), q = *reinterpret_cast<const float4*>(B + j * ra + x);
+                        v = fmaf(p.x, q.x, v); v = fmaf(p.y, q.y, v); v = fmaf(p.z, q.z, v); v = fmaf(p.w, q.w, v);
+                    }
+                    v *= power(ld, i - j) * s.in_scale;
+                }
+                P[i * (kC + 1) + j] = v;
+            }
+            __syncthreads();
+            const int cols = pc / 4;
+            for (int e = tid; e < kC / 4 * cols; e += kThreads) {
+                const int i0 = e / cols * 4, x = e % cols * 4;
+                float in[4][4] = {}, far[4][4] = {};
+                for (int j = 0; j < min(m, i0 + 4); ++j) {
+                    const float4 q = *reinterpret_cast<const float4*>(Cc + j * rc + x);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float p = P[(i0 + r) * (kC + 1) + j];
+                        in[r][0] = fmaf(p, q.x, in[r][0]); in[r][1] = fmaf(p, q.y, in[r][1]);
+                        in[r][2] = fmaf(p, q.z, in[r][2]); in[r][3] = fmaf(p, q.w, in[r][3]);
+                    }
+                }
+                for (int y = 0; y < pa; ++y) {
+                    const float4 q = *reinterpret_cast<const float4*>(W + y * rc + x);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float p = A[(i0 + r) * ra + y];
+                        far[r][0] = fmaf(p, q.x, far[r][0]); far[r][1] = fmaf(p, q.y, far[r][1]);
+                        far[r][2] = fmaf(p, q.z, far[r][2]); far[r][3] = fmaf(p, q.w, far[r][3]);
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (i0 + r >= m) break;
+                    const long long tok = s.reversed ? n - 1 - (c0 + i0 + r) : c0 + i0 + r;
+                    T* out = (T*)s.out + (((long long)bat * s.t + tok) * s.h + head) * dc;
+                    const float f = power(ld, i0 + r + s.off);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (x + k < dc) out[x + k] = from_f32<T>(s.out_scale * fmaf(f, far[r][k], in[r][k]));
+                }
+            }
+            __syncthreads();
+        }
+        for (int e = tid; e < m * pa; e += kThreads) {
+            const int j = e / pa, x = e - j * pa;
+            B[j * ra + x] *= power(ld, m - s.off - j) * s.in_scale;
+        }
+        __syncthreads();
+        const float keep = power(ld, m);
+        const int cols = pc / 4;
+        for (int e = tid; e < pa / 4 * cols; e += kThreads) {
+            const int y = e / cols * 4, x = e % cols * 4;
+            float acc[4][4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float4 q = *reinterpret_cast<const float4*>(W + (y + r) * rc + x);
+                acc[r][0] = keep * q.x; acc[r][1] = keep * q.y; acc[r][2] = keep * q.z; acc[r][3] = keep * q.w;
+            }
+            for (int j = 0; j < m; ++j) {
+                const float4 p = *reinterpret_cast<const float4*>(B + j * ra + y), q = *reinterpret_cast<const float4*>(Cc + j * rc + x);
+                const float pv[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    acc[r][0] = fmaf(pv[r], q.x, acc[r][0]); acc[r][1] = fmaf(pv[r], q.y, acc[r][1]);
+                    acc[r][2] = fmaf(pv[r], q.z, acc[r][2]); acc[r][3] = fmaf(pv[r], q.w, acc[r][3]);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) *reinterpret_cast<float4*>(W + (y + r) * rc + x) = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
+        }
+    }
+    __syncthreads();
+    if (s.end) {
+        float* w1 = s.end + ((long long)bh * s.segments + seg) * size;
+        for (int e = tid; e < da * dc; e += kThreads) {
+            const int i = e / dc, j = e - i * dc;
+            w1[e] = W[i * rc + j];
+        }
+    }
+    if (s.out) {                                                 // rows behind the sequence's end
+        const long long zlo = first > n ? first : n, zhi = first + s.seg < s.t ? first + s.seg : s.t;
+        for (long long e = zlo * dc + tid; e < zhi * dc; e += kThreads) {
+            const long long tok = e / dc;
+            ((T*)s.out)[(((long long)bat * s.t + tok) * s.h + head) * dc + (e - tok * dc)] = from_f32<T>(0.0f);
+        }
+    }
+}
+
+template <typename T>
+int launch_sweep(const Sweep& s, cudaStream_t st) {
+    const int pa = (s.da + 3) / 4 * 4, pc = (s.dc + 3) / 4 * 4;
+    const int bytes = (2 * kC * (pa + 4) + kC * (pc + 4) + pa * (pc + 4) + kC * (kC + 1)) * 4;
+    CNL_TRY(ensure_dynamic_smem(sweep_kernel<T>, bytes));
+    sweep_kernel<T><<<(unsigned)((long long)s.batch * s.h * s.segments), kThreads, bytes, st>>>(s);
+    return after_launch("linear attention sweep");
+}
+
+int run_sweep_f32(const Sweep& s, int dtype, cudaStream_t st) {
+    if (dtype == CNL_F32) return launch_sweep<float>(s, st);
+    if (dtype == CNL_F16) return launch_sweep<__half>(s, st);
+    return launch_sweep<__nv_bfloat16>(s, st);
+}
+
+int run_sweep(const Sweep& s, int dtype, cudaStream_t st) { return run_sweep_f32(s, dtype, st); }
+
+// ---- scan over the segments -------------------------------------------------------------------------------------
+// local[seg] (W of every segment from 0) becomes W at the segment's start; `last` receives W at the sequence's end.
+__global__ void __launch_bounds__(256) scan_kernel(float* __restrict__ local, const float* __restrict__ init, float* __restrict__ last,
+                                                   const float* __restrict__ log_decay, const int* __restrict__ lengths, int t, int h,
+                                                   int size, int segments, int seg) {
+    const int parts = (size + 255) >> 8;
+    const long long bh = blockIdx.x / parts;
+    const int e = (int)(blockIdx.x - bh * parts) * 256 + threadIdx.x;
+    if (e >= size) return;
+    const float ld = clamp_log(log_decay[bh % h]);
+    const int n = lengths ? min(max(lengths[bh / h], 0), t) : t;
+    float* p = local + bh * segments * size + e;
+    float w = init ? init[bh * size + e] : 0.0f;
+    constexpr int kAhead = 8;
+    for (int s0 = 0; s0 < segments; s0 += kAhead) {
+        float v[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) v[i] = s0 + i < segments ? p[(long long)(s0 + i) * size] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (s0 + i >= segments) break;
+            p[(long long)(s0 + i) * size] = w;
+            const long long left = n - (long long)(s0 + i) * seg;
+            const int len = (int)(left < 0 ? 0 : left < seg ? left : seg);
+            w = fmaf(power(ld, len), w, v[i]);
+        }
+    }
+    if (last) last[bh * size + e] = w;
+}
+
+int run_scan(float* local, const float* init, float* last, const float* log_decay, const int* lengths, int b, int t, int h, int size,
+             int segments, int seg, cudaStream_t st) {
+    scan_kernel<<<(unsigned)((long long)((size + 255) / 256) * b * h), 256, 0, st>>>(local, init, last, log_decay, lengths, t, h, size, segments, seg);
+    return after_launch("linear attention scan");
+}
+
+// ---- one token --------------------------------------------------------------------------------------------------
+// S <- l S + k v^T in place, o = scale q^T S.  One block a head; reads and writes the state once: HBM bound, 8 dk dv bytes.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) step_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
+                                                   const float* __restrict__ log_decay, float* __restrict__ state, T* __restrict__ out,
+                                                   int h, int dk, int dv, int cols, float scale, long long qb, long long qh, long long kb,
+                                                   long long kh, long long vb, long long vh) {
+    __shared__ float sq[kMaxD], sk[kMaxD], red[256 * V];
+    const long long bh = blockIdx.x;
+    const int head = (int)(bh % h);
+    const long long bat = bh / h;
+    for (int i = threadIdx.x; i < dk; i += 256) {
+        sq[i] = to_f32(q[bat * qb + head * qh + i]);
+        sk[i] = to_f32(k[bat * kb + head * kh + i]);
+    }
+    const int tx = threadIdx.x % cols, ty = threadIdx.x / cols, rows = 256 / cols, x = tx * V;
+    const bool live = x < dv;
+    const float l = expf(clamp_log(log_decay[head]));
+    float vv[V], acc[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        vv[i] = live ? to_f32(v[bat * vb + head * vh + x + i]) : 0.0f;
+        acc[i] = 0.0f;
+    }
+    __syncthreads();
+    float* s = state + bh * dk * dv + x;
+    if (live) {
+#pragma unroll 8
+        for (int y = ty; y < dk; y += rows) {
+            float w[V];
+            if constexpr (V == 4) {
+                const float4 f = *reinterpret_cast<const float4*>(s + (long long)y * dv);
+                w[0] = f.x; w[1] = f.y; w[2] = f.z; w[3] = f.w;
+            } else w[0] = s[(long long)y * dv];
+            const float kk = sk[y], qq = sq[y];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                w[i] = fmaf(l, w[i], kk * vv[i]);
+                acc[i] = fmaf(qq, w[i], acc[i]);
+            }
+            if constexpr (V == 4) *reinterpret_cast<float4*>(s + (long long)y * dv) = make_float4(w[0], w[1], w[2], w[3]);
+            else s[(long long)y * dv] = w[0];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) red[i * 256 + threadIdx.x] = acc[i];
+    __syncthreads();
+    if (ty == 0 && live) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float o = 0.0f;
+            for (int r = 0; r < rows; ++r) o += red[i * 256 + r * cols + tx];
+            out[bh * dv + x + i] = from_f32<T>(scale * o);
+        }
+    }
+}
+
+template <typename T>
+int launch_step(const void* q, const void* k, const void* v, const long long* st6, const float* log_decay, float* state, void* out, int b,
+                int h, int dk, int dv, float scale, cudaStream_t st) {
+    const bool vec = dv % 4 == 0 && aligned16(state);
+    const int need = vec ? dv / 4 : dv;
+    int cols = 1;
+    while (cols < need) cols <<= 1;
+    const unsigned grid = (unsigned)((long long)b * h);
+    if (vec)
+        step_kernel<T, 4><<<grid, 256, 0, st>>>((const T*)q, (const T*)k, (const T*)v, log_decay, state, (T*)out, h, dk, dv, cols, scale, st6[0], st6[1], st6[2], st6[3], st6[4], st6[5]);
+    else
+        step_kernel<T, 1><<<grid, 256, 0, st>>>((const T*)q, (const T*)k, (const T*)v, log_decay, state, (T*)out, h, dk, dv, cols, scale, st6[0], st6[1], st6[2], st6[3], st6[4], st6[5]);
+    return after_launch("linear attention step");
+}
+
+int check(int b, int t, int h, int dk, int dv, int dtype) {
+    if (b < 0 || t < 0 || h < 1 || dk < 1 || dv < 1 || dk > kMaxD || dv > kMaxD)
+        return fail(CNL_ERR_BAD_SHAPE, "b %d, t %d, h %d, dk %d, dv %d: head sizes must be within 1..%d", b, t, h, dk, dv, kMaxD);
+    if ((long long)b * h > (1 << 24)) return fail(CNL_ERR_BAD_SHAPE, "b * h = %lld is above 2^24", (long long)b * h);
+    return check_dtype(dtype);
+}
+
+// Segments of a sequence: enough blocks for two an SM, but none shorter than 256 positions (a segment costs a round trip of
+// its state, dk x dv floats, through memory).
+int segment_plan(int b, int t, int h, int* segments, int* seg) {
+    int sms = 0;
+    CNL_TRY(sm_count(&sms));
+    const long long heads = (long long)b * h > 0 ? (long long)b * h : 1;
+    long long want = (2LL * sms + heads - 1) / heads, most = (t + 255) / 256;
+    if (want > most) want = most;
+    if (want < 1) want = 1;
+    long long len = ((long long)t + want - 1) / want;
+    len = (len + 127) / 128 * 128;
+    if (len < 128) len = 128;
+    *seg = (int)len;
+    *segments = (int)(t > 0 ? (t + len - 1) / len : 1);
+    return CNL_OK;
+}
+
+}  // namespace lin
+}  // namespace cnl
+
+using namespace cnl;
+using namespace cnl::lin;
+
+extern "C" int cnl_linattn_segments(int b, int t, int h) {
+    int segments = 0, seg = 0;
+    if (b < 0 || t < 0 || h < 1) return 1;
+    if (segment_plan(b, t, h, &segments, &seg) != CNL_OK) return -1;
+    return segments;
+}
+
+extern "C" int cnl_linattn_forward(const void* q, const void* k, const void* v, const long long* strides_host, const float* log_decay,
+                                   const int* lengths, const float* state, void* out, float* state_out, float* starts, int b, int t, int h,
+                                   int dk, int dv, float scale, int dtype, void* stream) {
+    CNL_TRY(lin::check(b, t, h, dk, dv, dtype));
+    if (b == 0) return CNL_OK;
+    if ((t > 0 && (!q || !k || !v || !out)) || !strides_host || !log_decay) return fail(CNL_ERR_NULL, "null pointer argument");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int segments = 0, seg = 0;
+    CNL_TRY(segment_plan(b, t, h, &segments, &seg));
+    if (segments > 1 && !starts) return fail(CNL_ERR_NULL, "%d segments need the starts buffer", segments);
+    const long long* s = strides_host;
+    const Rows Q = {q, s[0], s[1], s[2]}, Kk = {k, s[3], s[4], s[5]}, V = {v, s[6], s[7], s[8]};
+    Sweep w = {};
+    w.log_decay = log_decay; w.lengths = lengths; w.batch = b; w.t = t; w.h = h; w.segments = segments; w.seg = seg;
+    w.b = Kk; w.c = V; w.da = dk; w.dc = dv; w.off = 1; w.in_scale = 1.0f; w.out_scale = scale;
+    if (segments > 1) {
+        w.end = starts;
+        CNL_TRY(run_sweep(w, dtype, st));
+        CNL_TRY(run_scan(starts, state, state_out, log_decay, lengths, b, t, h, dk * dv, segments, seg, st));
+        w.start = starts; w.end = nullptr;
+    } else {
+        w.start = state; w.end = state_out;
+    }
+    w.a = Q; w.out = out;
+    return run_sweep(w, dtype, st);
+}
+
+extern "C" int cnl_linattn_backward(const void* q, const void* k, const void* v, const void* g_out, const long long* strides_host,
+                                    const float* log_decay, const int* lengths, const float* state, const float* starts,
+                                    const float* g_state_out, void* g_q, void* g_k, void* g_v, float* g_state, float* scratch, int b, int t,
+                                    int h, int dk, int dv, float scale, int dtype, void* stream) {
+    CNL_TRY(lin::check(b, t, h, dk, dv, dtype));
+    if (b == 0) return CNL_OK;
+    if ((t > 0 && (!q || !k || !v || !g_out || !g_q || !g_k || !g_v)) || !strides_host || !log_decay) return fail(CNL_ERR_NULL, "null pointer argument");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int segments = 0, seg = 0;
+    CNL_TRY(segment_plan(b, t, h, &segments, &seg));
+    if (segments > 1 && (!starts || !scratch)) return fail(CNL_ERR_NULL, "%d segments need starts and scratch", segments);
+    const long long* s = strides_host;
+    const Rows Q = {q, s[0], s[1], s[2]}, Kk = {k, s[3], s[4], s[5]}, V = {v, s[6], s[7], s[8]}, G = {g_out, s[9], s[10], s[11]};
+    Sweep w = {};
+    w.log_decay = log_decay; w.lengths = lengths; w.batch = b; w.t = t; w.h = h; w.segments = segments; w.seg = seg;
+    // dq
+    w.a = G; w.b = V; w.c = Kk; w.da = dv; w.dc = dk; w.off = 1; w.in_scale = 1.0f; w.out_scale = scale;
+    w.start = segments > 1 ? starts : state; w.transposed = 1; w.out = g_q;
+    CNL_TRY(run_sweep(w, dtype, st));
+    // the reversed sweeps: W = sum of scale l^.. q do^T
+    w.off = 0; w.reversed = 1; w.in_scale = scale; w.out_scale = 1.0f;
+    w.b = Q; w.c = G; w.da = dk; w.dc = dv; w.transposed = 0; w.start = nullptr; w.out = nullptr;
+    if (segments > 1) {
+        w.end = scratch;
+        CNL_TRY(run_sweep(w, dtype, st));
+        CNL_TRY(run_scan(scratch, g_state_out, g_state, log_decay, lengths, b, t, h, dk * dv, segments, seg, st));
+        w.start = scratch; w.end = nullptr;
+    } else {
+        w.start = g_state_out; w.end = g_state;
+    }
+    w.a = Kk; w.out = g_v;
+    CNL_TRY(run_sweep(w, dtype, st));
+    w.end = nullptr;
+    w.a = V; w.b = G; w.c = Q; w.da = dv; w.dc = dk; w.transposed = 1; w.out = g_k;
+    return run_sweep(w, dtype, st);
+}
+
+extern "C" int cnl_linattn_step(const void* q, const void* k, const void* v, const long long* strides_host, const float* log_decay, float* state,
+                                void* out, int b, int h, int dk, int dv, float scale, int dtype, void* stream) {
+    CNL_TRY(lin::check(b, 1, h, dk, dv, dtype));
+    if (b == 0) return CNL_OK;
+    if (!q || !k || !v || !strides_host || !log_decay || !state || !out) return fail(CNL_ERR_NULL, "null pointer argument");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == CNL_F32) return launch_step<float>(q, k, v, strides_host, log_decay, state, out, b, h, dk, dv, scale, st);
+    if (dtype == CNL_F16) return launch_step<__half>(q, k, v, strides_host, log_decay, state, out, b, h, dk, dv, scale, st);
+    return launch_step<__nv_bfloat16>(q, k, v, strides_host, log_decay, state, out, b, h, dk, dv, scale, st);
+}

@@ -30,6 +30,20 @@ extern "C" {
 
 #define CNL_NUM_IDS 10        /* __uniqueIds__, cudaTV/cudaCode/TVInpaintFista.h:5 */
 
+/* element types of the network operators (cnl_ckpt8_*, cnl_act8_*, cnl_blocknorm_*, cnl_linattn_*) */
+#define CNL_F32 0
+#define CNL_F16 1
+#define CNL_BF16 2
+
+/* formats of an 8-bit activation checkpoint */
+#define CNL_CKPT_NONE 0
+#define CNL_CKPT_INT8 1
+#define CNL_CKPT_E4M3 2
+
+/* activations of cnl_act8_* */
+#define CNL_ACT_GELU 1        /* x Phi(x), the exact form */
+#define CNL_ACT_SILU 2        /* x sigmoid(x) */
+
 /* options for cnl_tv_set_option */
 #define CNL_OPT_CONDITIONER 1   /* 1 (default): stateful spike kill / rescale of returned gradients after 10 runs
                                    (cudaTV/cudaCode/TVInpaintFista.cu:128-155, :1760-1792); 0: off */
@@ -253,6 +267,81 @@ int cnl_wmedian_forward(const float* flow, const float* weights, float* out, int
 int cnl_wmedian_backward(const float* flow, const float* weights, const int* tap, const float* alpha, const float* grad,
                          float* g_flow, float* g_weights, void* scratch, int n, int c, int h, int w, int k, void* stream);
 long long cnl_wmedian_scratch_bytes(int k);
+
+/*
+ * Activations kept in 8 bits for the backward pass.  No reference counterpart.
+ * An 8-bit checkpoint of count elements is codes [count] (one byte each) and scales [ceil(count / 32)]: thirty-two
+ * neighbouring elements share the power of two 2^(scale - 127).  fmt CNL_CKPT_INT8: a whole number -127..127 (error at most
+ * half of the unit, i.e. max|block| / 128); CNL_CKPT_E4M3: a float of 4 exponent and 3 mantissa bits (error at most 1/16 of
+ * the element, down to the format's subnormals).  Elements that are not finite come back as NaN.
+ *   cnl_ckpt8_store   : x [count] of `dtype` -> codes, scales
+ *   cnl_ckpt8_restore : codes, scales -> x [count] of `dtype`, saturated to the type's finite range
+ *   cnl_act8_forward  : y = act(x), and codes, scales of x in the same pass (both null: y alone)
+ *   cnl_act8_backward : g_x = g_y * act'(x restored from codes, scales)
+ */
+int cnl_ckpt8_store(const void* x, unsigned char* codes, unsigned char* scales, long long count, int dtype, int fmt,
+                    void* stream);
+int cnl_ckpt8_restore(const unsigned char* codes, const unsigned char* scales, void* x, long long count, int dtype, int fmt,
+                      void* stream);
+int cnl_act8_forward(const void* x, void* y, unsigned char* codes, unsigned char* scales, long long count, int dtype, int fmt,
+                     int act, void* stream);
+int cnl_act8_backward(const unsigned char* codes, const unsigned char* scales, const void* g_y, void* g_x, long long count,
+                      int dtype, int fmt, int act, void* stream);
+
+/*
+ * Norms before and after a block, fused with the block's gate, residual scale and residual sum.  No reference counterpart.
+ *   N(v; w, b) = (v - mu) r w + b over the d channels of a row; layer = 0: mu = 0, r = (mean v^2 + eps)^-1/2;
+ *                layer = 1: mu = mean v, r = (mean (v - mu)^2 + eps)^-1/2
+ *   y = x + scale * a(gate) * N(u; w_post, b_post)      u may be null: y = x and y is not written
+ *   h = N(y; w_pre, b_pre)                              w_pre may be null: no h.  h is taken of y before it is rounded
+ * x, u, y, h [rows][d] of `dtype`; the parameters scale, w_post, b_post, w_pre, b_pre [d] of `wdtype` (dtype or CNL_F32);
+ * scale, b_post, b_pre may be null (1, 0, 0).  gate_mode 0: no gate; 1: gate [rows][d]; 2: gate [groups][d], one row for
+ * rows / groups consecutive rows; sigmoid_gate 1: a = sigmoid, 0: a = identity.  groups matters with gate_mode 2 only.
+ * 1 <= d <= 8192.  Rows are contiguous; 16-byte aligned tensors with d a multiple of 8 run as vectors.
+ * stats [rows][4] floats (16-byte aligned; may be null in a forward call that no backward call follows).
+ * fmt other than CNL_CKPT_NONE: the forward call also leaves x, u and a gate of mode 1 as 8-bit checkpoints whose blocks run
+ * along a row, codes [3][rows][d] and scales [3][rows][ceil(d / 32)] (a plane whose tensor is absent, and x's without w_pre,
+ * is not touched and, at the end, need not exist), and the backward call reads those instead of x, u and gate.
+ * cnl_blocknorm_backward: g_y, g_h may be null (zero); each of g_x, g_u, g_gate, g_scale, g_w_post, g_b_post, g_w_pre, g_b_pre may be
+ * null (not wanted).  Column sums are joined in a fixed order.  scratch: cnl_blocknorm_scratch_bytes(rows, d, groups) bytes
+ * (groups 1 unless gate_mode is 2).
+ */
+long long cnl_blocknorm_scratch_bytes(long long rows, int d, long long groups);
+int cnl_blocknorm_forward(const void* x, const void* u, const void* gate, const void* scale, const void* w_post,
+                          const void* b_post, const void* w_pre, const void* b_pre, void* y, void* h, float* stats,
+                          unsigned char* codes, unsigned char* scales, long long rows, int d, long long groups, int gate_mode,
+                          int sigmoid_gate, int layer, float eps, int dtype, int wdtype, int fmt, void* stream);
+int cnl_blocknorm_backward(const void* x, const void* u, const void* gate, const unsigned char* codes,
+                           const unsigned char* scales, const float* stats, const void* scale, const void* w_post,
+                           const void* b_post, const void* w_pre, const void* b_pre, const void* g_y, const void* g_h, void* g_x,
+                           void* g_u, void* g_gate, void* g_scale, void* g_w_post, void* g_b_post, void* g_w_pre, void* g_b_pre,
+                           void* scratch, long long rows, int d, long long groups, int gate_mode, int sigmoid_gate, int layer,
+                           int dtype, int wdtype, int fmt, void* stream);
+
+/*
+ * Linear attention with a decay for each head.  No reference counterpart.
+ *   S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,   o_t = scale q_t^T S_t,   S_{-1} = state (null: 0)
+ * q, k [b][t][h][dk], v [b][t][h][dv] of `dtype`, the last dimension contiguous; strides_host: HOST array of the batch, token
+ * and head strides, in elements, of q, k, v (and of g_out in the backward call).  out, g_q, g_k, g_v are contiguous.
+ * log_decay [h] fp32, at most 0 (-inf: no memory; not checked).  lengths [b] int (null: t): tokens at or behind lengths[b]
+ * are not read, give zero rows and zero gradients; values are held to 0..t.  state, state_out, g_state_out, g_state
+ * [b][h][dk][dv] fp32, each may be null.  dk, dv within 1..128.
+ * starts: cnl_linattn_segments(b, t, h) * b * h * dk * dv floats, filled by the forward call (states at the start of the
+ * segments that run in parallel) and read by the backward call; scratch: as many floats.  Both may be null where
+ * cnl_linattn_segments is 1; the backward call then reads `state`.
+ * cnl_linattn_step: one token, q, k [b][h][dk], v [b][h][dv], strides_host the batch and head strides of q, k, v; state is
+ * updated in place.
+ */
+int cnl_linattn_segments(int b, int t, int h);
+int cnl_linattn_forward(const void* q, const void* k, const void* v, const long long* strides_host, const float* log_decay,
+                        const int* lengths, const float* state, void* out, float* state_out, float* starts, int b, int t, int h,
+                        int dk, int dv, float scale, int dtype, void* stream);
+int cnl_linattn_backward(const void* q, const void* k, const void* v, const void* g_out, const long long* strides_host,
+                         const float* log_decay, const int* lengths, const float* state, const float* starts,
+                         const float* g_state_out, void* g_q, void* g_k, void* g_v, float* g_state, float* scratch, int b, int t,
+                         int h, int dk, int dv, float scale, int dtype, void* stream);
+int cnl_linattn_step(const void* q, const void* k, const void* v, const long long* strides_host, const float* log_decay,
+                     float* state, void* out, int b, int h, int dk, int dv, float scale, int dtype, void* stream);
 
 /* Message for the last error on the calling thread ("" if none). */
 const char* cnl_last_error(void);

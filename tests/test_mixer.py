@@ -1,0 +1,167 @@
+"""The network operators together, as a network in front of the optimisation layers runs them."""
+import copy
+
+import pytest
+import torch
+
+from customnetworklayers_b200.mixer import PixelMixer
+from tests.operators_ref import act, act_slope, attention, block_norm, put_away
+
+
+class _Act(torch.autograd.Function):
+    """GELU whose slope is taken at the 8-bit value of its input."""
+
+    @staticmethod
+    def forward(ctx, x, fmt):
+        ctx.save_for_backward(x)
+        ctx.fmt = fmt
+        return act(x, "gelu")
+
+    @staticmethod
+    def backward(ctx, g):
+        (x,) = ctx.saved_tensors
+        at = x if ctx.fmt is None else put_away(x.reshape(-1).cpu(), ctx.fmt).view(x.shape).to(x.device)
+        return g * act_slope(at, "gelu"), None
+
+
+def reference(m, x, states=None, lengths=None):
+    """The mixer's forward pass in 64 bits from the modules' own parameters (norms keep full precision)."""
+    m = copy.deepcopy(m).double()
+    x = x.detach().double().clone().requires_grad_(True)
+    n, c = x.shape[0], x.shape[-1]
+    y, ends = x, []
+    h = block_norm(y, None, None, None, None, None, m.pre.weight, m.pre.bias, m.pre.kind == "layer", True)[1]
+    for i in range(len(m.gate)):
+        a, r = m.attention[i], m.after_attention[i]
+        q, k, v = a.qkv(h).view(n, -1, 3, a.heads, c // a.heads).unbind(2)
+        o, end = attention(q, k, v, a.log_decay, None if states is None else states[i].double(), lengths, (c // a.heads) ** -0.5)
+        ends.append(end)
+        layer = r.kind == "layer"
+        y, h = block_norm(y, a.out(o.reshape(x.shape)), m.gate[i](h), r.scale, r.weight, r.bias, r.next_weight, r.next_bias, layer, True)
+        r = m.after_mlp[i]
+        u = m.down[i](_Act.apply(m.up[i](h), getattr(m.act, "fmt", None)))
+        y, h = block_norm(y, u, None, r.scale, r.weight, r.bias, r.next_weight, r.next_bias, layer, True)
+    return m, x, y, ends
+
+
+def rel(a, b):
+    a, b = a.detach().double().cpu(), b.detach().double().cpu()
+    return float((a - b).norm() / b.norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+def test_image_forward_and_backward(kind):
+    torch.manual_seed(0)
+    m = PixelMixer(48, 3, depth=2, kind=kind).cuda()
+    x = torch.randn(2, 9, 13, 48, device="cuda", requires_grad=True)
+    y, ends = m(x)
+    up = torch.randn_like(y)
+    m2, x2, y2, ends2 = reference(m, x)
+    y.backward(up)
+    y2.backward(up.double())
+    # some hundred 32-bit roundings of 2^-24 in sequence through five sublayers, each relative to its rows
+    assert rel(y, y2) <= 2.0 ** -16
+    assert all(rel(a, b) <= 2.0 ** -16 for a, b in zip(ends, ends2))
+    assert rel(x.grad, x2.grad) <= 2.0 ** -15
+    for (name, p), q in zip(m.named_parameters(), m2.parameters()):
+        assert rel(p.grad, q.grad) <= 2.0 ** -14, name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,allowed", [("int8", 2.0 ** -5), ("e4m3", 2.0 ** -3)])
+def test_with_checkpoints_in_8_bits(fmt, allowed):
+    torch.manual_seed(1)
+    m = PixelMixer(64, 2, depth=2, checkpoint=fmt).cuda()
+    plain = PixelMixer(64, 2, depth=2).cuda()
+    plain.load_state_dict(m.state_dict())
+    x = torch.randn(2, 300, 64, device="cuda", requires_grad=True)
+    y, _ = m(x)
+    z, _ = plain(x)
+    # the same forward pass but for the two forms of GELU (2^-21 of a value)
+    assert rel(y, z) <= 2.0 ** -16
+    up = torch.randn_like(y)
+    (a,) = torch.autograd.grad(y, x, up)
+    (b,) = torch.autograd.grad(z, x, up)
+    # an element is off by at most 1/64 of its block's largest (int8) or 1/16 of itself (e4m3); norms and slopes pass that
+    # on with a factor around one, and errors of different elements are independent
+    assert 0 < rel(a, b) <= allowed
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_prompt_at_once_and_its_tokens_one_by_one(dtype):
+    torch.manual_seed(2)
+    m = PixelMixer(32, 4, depth=2).cuda().to(dtype)
+    x = torch.randn(3, 40, 32, device="cuda").to(dtype)
+    with torch.no_grad():
+        whole, ends = m(x)
+        _, states = m(x[:, :30])
+        tail = [m.step(x[:, t], states) for t in range(30, 40)]
+    allowed = 2.0 ** -16 if dtype == torch.float32 else 2.0 ** -4       # bf16: projections and norms round 2^-8 some 20 times
+    assert rel(torch.stack(tail, 1), whole[:, 30:]) <= allowed
+    assert all(rel(a, b) <= allowed for a, b in zip(states, ends))
+
+
+@pytest.mark.gpu
+def test_padded_batch_and_fresh_states():
+    torch.manual_seed(3)
+    m = PixelMixer(32, 2, depth=1).cuda()
+    x = torch.randn(2, 50, 32, device="cuda")
+    lengths = torch.tensor([50, 20], dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        y, ends = m(x, m.new_states(2), lengths)
+        short, end = m(x[1:, :20])
+    assert rel(y[1:, :20], short) <= 2.0 ** -18 and rel(ends[0][1:], end[0]) <= 2.0 ** -18
+
+
+@pytest.mark.gpu
+def test_in_front_of_the_inpainting_layer():
+    """Mixer -> confidence and data term -> TV layer: one backward pass through both."""
+    from customnetworklayers_b200 import tvInpaint_cuda_ext
+    from customnetworklayers_b200.TVInpainting import TVInpaint
+    torch.manual_seed(4)
+    h, w = 24, 32
+    m = PixelMixer(32, 2, depth=1, checkpoint="int8").cuda()
+    head = torch.nn.Linear(32, 5).cuda()
+    layer = TVInpaint("cuda", its=10, pid=9)
+    feat = torch.randn(1, h, w, 32, device="cuda")
+    z = head(m(feat)[0])
+    wx, wy, c = (torch.sigmoid(z[..., i:i + 1]) for i in range(3))
+    b = z[..., 3:5]
+    sol = layer(wx, wy, c, b, torch.zeros_like(b))
+    sol.square().mean().backward()
+    tvInpaint_cuda_ext.release(9)
+    for name, p in list(m.named_parameters()) + list(head.named_parameters()):
+        assert p.grad is not None and torch.isfinite(p.grad).all() and p.grad.abs().max() > 0, name
+
+
+@pytest.mark.gpu
+def test_training_step_in_a_graph():
+    torch.manual_seed(5)
+    m = PixelMixer(64, 2, depth=1, checkpoint="int8").cuda()
+    x = torch.randn(1, 700, 64, device="cuda")
+    params = list(m.parameters())
+
+    def once():
+        y, _ = m(x)
+        return torch.autograd.grad(y.square().sum(), params)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            once()
+    torch.cuda.current_stream().wait_stream(side)
+    want = [g.clone() for g in once()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = once()
+    keep = x.clone()
+    x.zero_()
+    graph.replay()
+    x.copy_(keep)
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert rel(a, b) <= 2.0 ** -16                    # the library's products may split their sums differently
