@@ -154,13 +154,9 @@ int launch_sweep(const Sweep& s, cudaStream_t st) {
     return after_launch("linear attention sweep");
 }
 
-int run_sweep_f32(const Sweep& s, int dtype, cudaStream_t st) {
-    if (dtype == CNL_F32) return launch_sweep<float>(s, st);
-    if (dtype == CNL_F16) return launch_sweep<__half>(s, st);
-    return launch_sweep<__nv_bfloat16>(s, st);
+int run_sweep(const Sweep& s, int dtype, cudaStream_t st) {
+    return dtype == CNL_F32 ? launch_sweep<float>(s, st) : run_sweep_mma(s, dtype, st);
 }
-
-int run_sweep(const Sweep& s, int dtype, cudaStream_t st) { return run_sweep_f32(s, dtype, st); }
 
 // ---- scan over the segments -------------------------------------------------------------------------------------
 // local[seg] (W of every segment from 0) becomes W at the segment's start; `last` receives W at the sequence's end.

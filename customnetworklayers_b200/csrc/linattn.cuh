@@ -41,7 +41,7 @@ __device__ __forceinline__ float clamp_log(float a) { return a < -1e30f ? -1e30f
 __device__ __forceinline__ float power(float a, int n) { return expf(a * (float)n); }
 
 int run_sweep(const Sweep& s, int dtype, cudaStream_t st);          // dispatches to the kernel that serves the type and sizes
-int run_sweep_f32(const Sweep& s, int dtype, cudaStream_t st);
+int run_sweep_mma(const Sweep& s, int dtype, cudaStream_t st);      // fp16, bf16: tensor cores
 
 }  // namespace lin
 }  // namespace cnl

@@ -144,6 +144,29 @@ def test_decays_from_none_to_all(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("size", [2.0 ** -9, 2.0 ** 5])
+def test_fp16_near_the_ends_of_its_range(size):
+    """Small: products near and under fp16's smallest normal number.  Large: a carried state above its largest number (65504)
+    whose outputs are in range, because q is small."""
+    x, decay, do, ds = make(1, 300, 2, 32, 32, torch.float16, seed=13)
+    decay = torch.tensor([-2.0 ** -9, -0.1])
+    big = size > 1
+    x = {"q": (x["q"].double() * (2.0 ** -9 if big else size)).half(), "k": (x["k"].double().abs() * (size * 16 if big else size)).half(),
+         "v": (x["v"].double().abs() * (size * 8 if big else size)).half(), "state": x["state"] * 0}
+    d = {k: v.cuda() for k, v in x.items()}
+    o, end = linattn.linear_attention(d["q"], d["k"], d["v"], decay.cuda(), state=d["state"], scale=2.0 ** -4)
+    f = {k: v.double() for k, v in x.items()}
+    ro, rend = attention(f["q"], f["k"], f["v"], decay.double(), f["state"], None, 2.0 ** -4)
+    a = {k: v.abs() for k, v in f.items()}
+    mo, mend = attention(a["q"], a["k"], a["v"], decay.double(), a["state"], None, 2.0 ** -4)
+    assert not big or rend.abs().max() > 65504 > 2 * ro.abs().max()
+    # a weight under 2^-14 is off by up to 2^-25 (half of fp16's smallest step) for each of the chunk's 64 rows of v
+    low = 64 * 2.0 ** -25 * float(a["v"].max())
+    assert_within(o, ro, HALF[torch.float16] * (ro.abs() + 2 * mo) + 512 * 2.0 ** -24 * mo + low + TINY[torch.float16], "out")
+    assert_within(end, rend, 512 * 2.0 ** -24 * mend, "end state")
+
+
+@pytest.mark.gpu
 def test_lengths_out_of_range_are_held_to_the_batch():
     x, decay, _, _ = make(3, 40, 2, 8, 8, torch.float32)
     d = {k: v.cuda() for k, v in x.items()}
