@@ -15,10 +15,9 @@ from typing import Optional
 import torch
 from torch import nn
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._tensor import DTYPES, check_tensor, launch, ptr, wants_grad
+from ._tensor import DTYPES, check_tensor, first_order, launch, on_device, ptr, wants_grad
 from .ckpt8 import BLOCK, format_code
 from .dist import allreduce_scalar_grads
 
@@ -51,16 +50,17 @@ def _check(x, u, gate, scale, weight, bias, next_weight, next_bias):
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_CHANNELS:
         raise RuntimeError(f"x must have 1 to {MAX_CHANNELS} channels in its last dimension")
     d = x.shape[-1]
+    device = x.device
     if u is not None:
-        check_tensor(u, "u", x.dtype, x.device, x.shape)
+        check_tensor(u, "u", x.dtype, device, x.shape)
     if gate is not None:
-        check_tensor(gate, "gate", x.dtype, x.device)
+        check_tensor(gate, "gate", x.dtype, device)
     wdtype = (weight if weight is not None else next_weight).dtype
     if wdtype not in (x.dtype, torch.float32):
         raise RuntimeError(f"parameters must be {x.dtype} or float32, not {wdtype}")
     for t, name in ((scale, "scale"), (weight, "weight"), (bias, "bias"), (next_weight, "next_weight"), (next_bias, "next_bias")):
         if t is not None:
-            check_tensor(t, name, wdtype, x.device, (d,))
+            check_tensor(t, name, wdtype, device, (d,))
     if next_bias is not None and next_weight is None:
         raise RuntimeError("next_bias needs next_weight")
     return wdtype
@@ -114,7 +114,7 @@ class BlockNormFunction(Function):
         return y if h is None else (y, h)
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, *grads):
         x, u, gate, codes, scales, stats, scale, weight, bias, next_weight, next_bias = ctx.saved_tensors
         shape, dtype, device, mode, groups, gate_shape, sigmoid, layer, code = ctx.meta
@@ -131,15 +131,18 @@ class BlockNormFunction(Function):
         need = ctx.needs_input_grad
         d = shape[-1]
         rows = shape.numel() // d
-        new = lambda wanted, like_shape, like_dtype: torch.empty(like_shape, dtype=like_dtype, device=device) if wanted else None  # noqa: E731
         wdtype = (weight if weight is not None else next_weight).dtype
-        g_x = new(need[0], shape, dtype)
-        g_u = new(need[1], shape, dtype)
-        g_gate = new(need[2], gate_shape, dtype)
-        g_params = [new(need[i], (d,), wdtype) for i in range(3, 8)]
+        like = g_y if g_y is not None else g_h
+        g_x = torch.empty_like(like) if need[0] else None
+        g_u = torch.empty_like(like) if need[1] else None
+        g_gate = torch.empty(gate_shape, dtype=dtype, device=device) if need[2] else None
+        g_params = [None] * 5
+        wanted = [i for i in range(5) if need[3 + i]]
+        if wanted:
+            for i, g in zip(wanted, torch.empty((len(wanted), d), dtype=wdtype, device=device).unbind(0)):
+                g_params[i] = g
         lib = _lib.load()
-        with torch.cuda.device(device):
-            scratch = torch.empty(lib.cnl_blocknorm_scratch_bytes(rows, d, groups) // 4, dtype=torch.float32, device=device)
+        scratch = torch.empty(on_device(device, lib.cnl_blocknorm_scratch_bytes, rows, d, groups), dtype=torch.uint8, device=device)
         launch("block norm backward", lib.cnl_blocknorm_backward, device, ptr(x), ptr(u), ptr(gate), ptr(codes), ptr(scales),
                stats.data_ptr(), ptr(scale), ptr(weight), ptr(bias), ptr(next_weight), ptr(next_bias), ptr(g_y), ptr(g_h), ptr(g_x),
                ptr(g_u), ptr(g_gate), *(ptr(g) for g in g_params), scratch.data_ptr(), rows, d, groups, mode, sigmoid, layer,

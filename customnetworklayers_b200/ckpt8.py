@@ -16,10 +16,9 @@ from typing import Optional
 import torch
 from torch import nn
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._tensor import DTYPES, check_tensor, launch, wants_grad
+from ._tensor import DTYPES, check_tensor, first_order, launch, wants_grad
 
 FORMATS = {"int8": _lib.CKPT_INT8, "e4m3": _lib.CKPT_E4M3}
 KINDS = {"gelu": _lib.ACT_GELU, "silu": _lib.ACT_SILU}
@@ -110,17 +109,28 @@ def backward(stored: Stored8, grad: torch.Tensor, kind: str) -> torch.Tensor:
 class Activation8Function(Function):
     @staticmethod
     def forward(ctx, x, kind, fmt):
-        y, stored = forward(x.contiguous(), kind, fmt)
-        ctx.save_for_backward(stored.codes, stored.scales)
-        ctx.meta = (stored.shape, stored.dtype, fmt, kind)
+        x = x.contiguous()
+        check_tensor(x, "x")
+        n = x.numel()
+        y = torch.empty_like(x)
+        # codes and scales in one allocation, the scales behind the codes
+        packed = torch.empty(n + -(-n // BLOCK), dtype=torch.uint8, device=x.device)
+        ctx.save_for_backward(packed)
+        ctx.meta = meta = (DTYPES[x.dtype], format_code(fmt), _kind_code(kind))
+        at = packed.data_ptr()
+        launch("activation forward", _lib.load().cnl_act8_forward, x.device, x.data_ptr(), y.data_ptr(), at, at + n, n, *meta)
         return y
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, grad):
-        codes, scales = ctx.saved_tensors
-        shape, dtype, fmt, kind = ctx.meta
-        return backward(Stored8(codes, scales, shape, dtype, fmt), grad.contiguous(), kind), None, None
+        (packed,) = ctx.saved_tensors
+        grad = grad.contiguous()
+        n = grad.numel()
+        g = torch.empty_like(grad)
+        at = packed.data_ptr()
+        launch("activation backward", _lib.load().cnl_act8_backward, grad.device, at, at + n, grad.data_ptr(), g.data_ptr(), n, *ctx.meta)
+        return g, None, None
 
 
 def activation(x: torch.Tensor, kind: str = "gelu", fmt: str = "int8") -> torch.Tensor:

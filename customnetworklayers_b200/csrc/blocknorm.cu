@@ -150,8 +150,73 @@ __device__ __forceinline__ void get_codes(const unsigned char* __restrict__ code
     }
 }
 
+// ---- rows on their way --------------------------------------------------------------------------------------------
+// VEC rows arrive by cp.async in slots of shared memory that belong to one thread each: a thread waits for its own copies and
+// needs no barrier, and STAGES - 1 rows are under way while one is worked on without costing registers.  An SM needs some
+// 45 KB in flight to keep HBM busy; 512 threads with five 16-byte tensors a row are 40 KB a stage.
+template <typename T, bool VEC, int TENSORS, int STAGES>
+struct Slots {
+    static constexpr int kParts = VEC ? (int)sizeof(T) * K / 16 : 0;       // 16-byte parts of a thread's channels
+    static constexpr int bytes = TENSORS * kParts * STAGES * 16;           // for one thread
+    unsigned char* base;
+
+    __device__ __forceinline__ unsigned char* at(int stage, int tensor, int part) const {
+        return base + (((stage * TENSORS + tensor) * kParts + part) * blockDim.x + threadIdx.x) * 16;
+    }
+    __device__ __forceinline__ void ask(int stage, int tensor, const T* __restrict__ row, const Args& a, int t) const {
+        if (t * K < a.d) {
+#pragma unroll
+            for (int i = 0; i < kParts; ++i)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(at(stage, tensor, i))),
+                             "l"(reinterpret_cast<const unsigned char*>(row + t * K) + 16 * i) : "memory");
+        }
+    }
+    __device__ __forceinline__ void ask_codes(int stage, int tensor, const unsigned char* __restrict__ codes, const Args& a, int t) const {
+        if (t * K < a.d)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((unsigned)__cvta_generic_to_shared(at(stage, tensor, 0))), "l"(codes + t * K) : "memory");
+    }
+    __device__ __forceinline__ void close() const { asm volatile("cp.async.commit_group;" ::: "memory"); }
+    __device__ __forceinline__ void wait() const { asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory"); }
+
+    __device__ __forceinline__ void take(int stage, int tensor, const Args& a, int t, float (&v)[K]) const {
+        if (t * K < a.d) {
+            if constexpr (kParts == 2) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float4 q = *reinterpret_cast<const float4*>(at(stage, tensor, i));
+                    v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
+                }
+            } else if constexpr (kParts == 1) {
+                const uint4 q = *reinterpret_cast<const uint4*>(at(stage, tensor, 0));
+                const unsigned w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 f = unpack2(w[j], T());
+                    v[2 * j] = f.x; v[2 * j + 1] = f.y;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; ++k) v[k] = 0.0f;
+        }
+    }
+    __device__ __forceinline__ void take_codes(int stage, int tensor, int s, const Args& a, int t, float (&v)[K]) const {
+        if (t * K < a.d) {
+            const uint2 q = *reinterpret_cast<const uint2*>(at(stage, tensor, 0));
+            const unsigned w[2] = {q.x, q.y};
+            if (a.fmt == CNL_CKPT_INT8) ckpt8::decode<CNL_CKPT_INT8, K>(w, s, v);
+            else ckpt8::decode<CNL_CKPT_E4M3, K>(w, s, v);
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; ++k) v[k] = 0.0f;
+        }
+    }
+};
+template <typename T> constexpr int kStagesOf = sizeof(T) == 4 ? 2 : 3;
+
 // ---- sums over a row --------------------------------------------------------------------------------------------
 // WIDE: a row spans several warps, whose sums meet in shared memory (two buffers in turn, so one barrier a sum).
+// The barrier is one of its own for every row slot of the block: rows do not wait for one another.
 template <bool WIDE, int N>
 __device__ __forceinline__ void row_sum(float (&v)[N], int tpr, float* __restrict__ sm, int& turn) {
     if constexpr (!WIDE) {
@@ -170,7 +235,7 @@ __device__ __forceinline__ void row_sum(float (&v)[N], int tpr, float* __restric
             for (int o = 1; o < 32; o <<= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
             if (lane == 0) buf[warp * 2 + i] = v[i];
         }
-        __syncthreads();
+        asm volatile("bar.sync %0, %1;" ::"r"((int)threadIdx.x / tpr + 1), "r"(tpr) : "memory");
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float p = lane < wpr ? buf[(first + lane) * 2 + i] : 0.0f;
@@ -206,32 +271,57 @@ __device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f
 
 // ---- forward ----------------------------------------------------------------------------------------------------
 template <typename T, bool VEC, bool WIDE, int BLOCK>
-__global__ void __launch_bounds__(BLOCK) forward_kernel(const Args a) {
+__global__ void __launch_bounds__(BLOCK, BLOCK <= 256 ? 3 : 1) forward_kernel(const Args a) {
+    constexpr int kStages = kStagesOf<T>;
+    extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ float sm[2 * 32 * 2];
+    const Slots<T, VEC, 3, kStages> slots = {dynamic};
     const int rpb = blockDim.x / a.tpr, slot = threadIdx.x / a.tpr, t = threadIdx.x - slot * a.tpr;
     const long long group = blockIdx.x / a.nb;
     const int j = blockIdx.x - (int)(group * a.nb);
-    const long long end = (group + 1) * a.per;
+    const long long begin = group * a.per + (long long)j * rpb, end = (group + 1) * a.per, step = (long long)a.nb * rpb;
     const int blocks = (a.d + 31) >> 5;
-    int turn = 0;
-    for (long long base = group * a.per + (long long)j * rpb; base < end; base += (long long)a.nb * rpb) {
-        const long long row = base + slot;
-        const bool live = slot < rpb && row < end;
-        const long long off = (live ? row : base) * a.d;
-        float y[K];
-        get<T, VEC>((const T*)a.x + off, a, t, y);
-        float mu_u = 0.0f, r_u = 0.0f, mu_y = 0.0f, r_y = 0.0f;
-        if (a.codes && a.w1) put_codes<VEC>(a.codes + off, a.scales + (live ? row : base) * blocks, a, t, live, y);
-        if (a.u) {
-            float u[K], z[K];
-            get<T, VEC>((const T*)a.u + off, a, t, u);
-            if (a.gate_full) get<T, VEC>((const T*)a.gate + off, a, t, z);
-            else if (a.gate_group) get<T, VEC>((const T*)a.gate + group * a.d, a, t, z);
-            if (a.codes) {
-                const long long n = a.rows * a.d, nb = a.rows * blocks, so = (live ? row : base) * blocks;
-                put_codes<VEC>(a.codes + n + off, a.scales + nb + so, a, t, live, u);
-                if (a.gate_full) put_codes<VEC>(a.codes + 2 * n + off, a.scales + 2 * nb + so, a, t, live, z);
+    auto ask = [&](int stage, long long base) {
+        if constexpr (VEC) {
+            const long long row = base + slot;
+            if (row < end) {
+                const long long off = row * a.d;
+                slots.ask(stage, 0, (const T*)a.x + off, a, t);
+                if (a.u) slots.ask(stage, 1, (const T*)a.u + off, a, t);
+                if (a.gate_full) slots.ask(stage, 2, (const T*)a.gate + off, a, t);
             }
+            slots.close();
+        }
+    };
+    int turn = 0, stage = 0;
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) ask(i, begin + i * step);
+    for (long long base = begin; base < end; base += step) {
+        const long long row = base + slot;
+        const bool live = row < end;
+        const long long off = (live ? row : base) * a.d;
+        float y[K], u[K], z[K];
+        if constexpr (VEC) {
+            slots.wait();
+            slots.take(stage, 0, a, t, y);
+            if (a.u) slots.take(stage, 1, a, t, u);
+            if (a.gate_full) slots.take(stage, 2, a, t, z);
+            ask(stage == 0 ? kStages - 1 : stage - 1, base + (kStages - 1) * step);
+            stage = stage == kStages - 1 ? 0 : stage + 1;
+        } else {
+            get<T, VEC>((const T*)a.x + off, a, t, y);
+            if (a.u) get<T, VEC>((const T*)a.u + off, a, t, u);
+            if (a.gate_full) get<T, VEC>((const T*)a.gate + off, a, t, z);
+        }
+        if (a.gate_group) get<T, VEC>((const T*)a.gate + group * a.d, a, t, z);
+        float mu_u = 0.0f, r_u = 0.0f, mu_y = 0.0f, r_y = 0.0f;
+        if (a.codes) {
+            const long long n = a.rows * a.d, nb = a.rows * blocks, so = (live ? row : base) * blocks;
+            if (a.w1) put_codes<VEC>(a.codes + off, a.scales + so, a, t, live, y);
+            if (a.u) put_codes<VEC>(a.codes + n + off, a.scales + nb + so, a, t, live, u);
+            if (a.gate_full) put_codes<VEC>(a.codes + 2 * n + off, a.scales + 2 * nb + so, a, t, live, z);
+        }
+        if (a.u) {
             center<VEC, WIDE>(u, a, t, sm, turn, mu_u, r_u);
             float w[K], b[K], s[K];
             param<T, VEC>(a.w2, a, t, 0.0f, w);
@@ -264,13 +354,18 @@ __global__ void __launch_bounds__(BLOCK) forward_kernel(const Args a) {
 template <typename T, bool VEC, bool WIDE, int BLOCK>
 __global__ void __launch_bounds__(BLOCK, BLOCK <= 256 ? 2 : 1) backward_kernel(const Args a) {
     constexpr bool kSharedSums = BLOCK > 256;                              // rows of up to 1024 threads: 64 registers each, sums in shared memory
-    extern __shared__ float dyn[];
+    constexpr bool kAsync = VEC && !kSharedSums;
+    constexpr int kStages = kStagesOf<T>;
+    extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ float sm[2 * 32 * 2];
+    const Slots<T, kAsync, 5, kStages> slots = {dynamic};
+    float* dyn = reinterpret_cast<float*>(dynamic);                        // the sums, once the rows are done
     const int rpb = blockDim.x / a.tpr, slot = threadIdx.x / a.tpr, t = threadIdx.x - slot * a.tpr;
     const long long group = blockIdx.x / a.nb;
     const int j = blockIdx.x - (int)(group * a.nb);
-    const long long end = (group + 1) * a.per;
+    const long long begin = group * a.per + (long long)j * rpb, end = (group + 1) * a.per, step = (long long)a.nb * rpb;
     const int blocks = (a.d + 31) >> 5;
+    const long long n = a.rows * a.d, nb = a.rows * blocks;
     float acc[kSharedSums ? 1 : kSums][K];
     if constexpr (kSharedSums) {
         for (int i = 0; i < kSums * K; ++i) dyn[i * blockDim.x + threadIdx.x] = 0.0f;
@@ -284,31 +379,81 @@ __global__ void __launch_bounds__(BLOCK, BLOCK <= 256 ? 2 : 1) backward_kernel(c
         if constexpr (kSharedSums) dyn[(i * K + k) * blockDim.x + threadIdx.x] += v;
         else acc[i][k] += v;
     };
-    int turn = 0;
-    for (long long base = group * a.per + (long long)j * rpb; base < end; base += (long long)a.nb * rpb) {
+    // statistics and scale bytes of a row; asked for one row ahead
+    float4 st_next = {};
+    unsigned sc_next = 0;
+    auto small = [&](long long base) {
         const long long row = base + slot;
-        const bool live = slot < rpb && row < end;
-        const long long at = live ? row : base, off = at * a.d, so = at * blocks, n = a.rows * a.d, nb = a.rows * blocks;
-        const float4 st = __ldg(a.stats + at);
-        float g[K], y[K], u[K], z[K];
-        // everything the row needs is asked for before its first use
-        if (a.fmt) {
-            if (a.dh) get_codes<VEC>(a.codes + off, a.scales + so, a, t, y);
-            if (a.u) {
-                get_codes<VEC>(a.codes + n + off, a.scales + nb + so, a, t, u);
-                if (a.gate_full) get_codes<VEC>(a.codes + 2 * n + off, a.scales + 2 * nb + so, a, t, z);
+        if (row >= end) return;
+        st_next = __ldg(a.stats + row);
+        if (kAsync && a.fmt && t * K < a.d) {
+            const unsigned char* sc = a.scales + row * blocks + (t >> 2);
+            sc_next = (a.dh ? __ldg(sc) : 0u) | (a.u ? __ldg(sc + nb) : 0u) << 8 | (a.gate_full ? __ldg(sc + 2 * nb) : 0u) << 16;
+        }
+    };
+    auto ask = [&](int stage, long long base) {
+        if constexpr (kAsync) {
+            const long long row = base + slot;
+            if (row < end) {
+                const long long off = row * a.d;
+                if (a.dy) slots.ask(stage, 0, (const T*)a.dy + off, a, t);
+                if (a.dh) slots.ask(stage, 1, (const T*)a.dh + off, a, t);
+                if (a.fmt) {
+                    if (a.dh) slots.ask_codes(stage, 2, a.codes + off, a, t);
+                    if (a.u) slots.ask_codes(stage, 3, a.codes + n + off, a, t);
+                    if (a.gate_full) slots.ask_codes(stage, 4, a.codes + 2 * n + off, a, t);
+                } else {
+                    if (a.dh) slots.ask(stage, 2, (const T*)a.x + off, a, t);
+                    if (a.u) slots.ask(stage, 3, (const T*)a.u + off, a, t);
+                    if (a.gate_full) slots.ask(stage, 4, (const T*)a.gate + off, a, t);
+                }
             }
+            slots.close();
+        }
+    };
+    int turn = 0, stage = 0;
+    small(begin);
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) ask(i, begin + i * step);
+    for (long long base = begin; base < end; base += step) {
+        const long long row = base + slot;
+        const bool live = row < end;
+        const long long off = (live ? row : base) * a.d;
+        const float4 st = st_next;
+        const unsigned sc = sc_next;
+        float g[K], y[K], u[K], z[K], dh[K];
+        if constexpr (kAsync) {
+            slots.wait();
+            if (a.dy) slots.take(stage, 0, a, t, g);
+            if (a.dh) slots.take(stage, 1, a, t, dh);
+            if (a.fmt) {
+                if (a.dh) slots.take_codes(stage, 2, ckpt8::scale_exponent((unsigned char)sc), a, t, y);
+                if (a.u) slots.take_codes(stage, 3, ckpt8::scale_exponent((unsigned char)(sc >> 8)), a, t, u);
+                if (a.gate_full) slots.take_codes(stage, 4, ckpt8::scale_exponent((unsigned char)(sc >> 16)), a, t, z);
+            } else {
+                if (a.dh) slots.take(stage, 2, a, t, y);
+                if (a.u) slots.take(stage, 3, a, t, u);
+                if (a.gate_full) slots.take(stage, 4, a, t, z);
+            }
+            ask(stage == 0 ? kStages - 1 : stage - 1, base + (kStages - 1) * step);
+            stage = stage == kStages - 1 ? 0 : stage + 1;
         } else {
-            if (a.dh) get<T, VEC>((const T*)a.x + off, a, t, y);
-            if (a.u) {
-                get<T, VEC>((const T*)a.u + off, a, t, u);
+            const long long so = (live ? row : base) * blocks;
+            if (a.fmt) {
+                if (a.dh) get_codes<VEC>(a.codes + off, a.scales + so, a, t, y);
+                if (a.u) get_codes<VEC>(a.codes + n + off, a.scales + nb + so, a, t, u);
+                if (a.gate_full) get_codes<VEC>(a.codes + 2 * n + off, a.scales + 2 * nb + so, a, t, z);
+            } else {
+                if (a.dh) get<T, VEC>((const T*)a.x + off, a, t, y);
+                if (a.u) get<T, VEC>((const T*)a.u + off, a, t, u);
                 if (a.gate_full) get<T, VEC>((const T*)a.gate + off, a, t, z);
             }
+            if (a.dy) get<T, VEC>((const T*)a.dy + off, a, t, g);
+            if (a.dh) get<T, VEC>((const T*)a.dh + off, a, t, dh);
         }
+        small(base + step);
         if (a.gate_group) get<T, VEC>((const T*)a.gate + group * a.d, a, t, z);
-        if (a.dy) {
-            get<T, VEC>((const T*)a.dy + off, a, t, g);
-        } else {
+        if (!a.dy) {
 #pragma unroll
             for (int k = 0; k < K; ++k) g[k] = 0.0f;
         }
@@ -331,8 +476,7 @@ __global__ void __launch_bounds__(BLOCK, BLOCK <= 256 ? 2 : 1) backward_kernel(c
             }
         }
         if (a.dh) {
-            float dh[K], w1[K], sum[2] = {0.0f, 0.0f};
-            get<T, VEC>((const T*)a.dh + off, a, t, dh);
+            float w1[K], sum[2] = {0.0f, 0.0f};
             param<T, VEC>(a.w1, a, t, 0.0f, w1);
 #pragma unroll
             for (int k = 0; k < K; ++k) {
@@ -378,6 +522,8 @@ __global__ void __launch_bounds__(BLOCK, BLOCK <= 256 ? 2 : 1) backward_kernel(c
                 if (slot == 0 && c < a.d) out[i * a.d + c] = dyn[(i * K + k) * blockDim.x + threadIdx.x];
             }
     } else {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncthreads();                                                   // the slots become the sums' room
         const int unit = WIDE ? a.tpr : 32, units = WIDE ? rpb : blockDim.x >> 5;
 #pragma unroll
         for (int i = 0; i < kSums; ++i) {
@@ -535,22 +681,22 @@ inline bool aligned_all(const void* const* p, int n) {
 template <typename T, bool VEC>
 int launch_forward(const Args& a, const Plan& p, cudaStream_t st) {
     const unsigned grid = (unsigned)(p.groups * p.nb);
-    if (p.tpr <= 32) forward_kernel<T, VEC, false, 256><<<grid, p.block, 0, st>>>(a);
-    else if (p.tpr <= 256) forward_kernel<T, VEC, true, 256><<<grid, p.block, 0, st>>>(a);
-    else forward_kernel<T, VEC, true, 1024><<<grid, p.block, 0, st>>>(a);
+    const int bytes = Slots<T, VEC, 3, kStagesOf<T>>::bytes * p.block;
+    auto* kernel = p.tpr <= 32 ? forward_kernel<T, VEC, false, 256> : p.tpr <= 256 ? forward_kernel<T, VEC, true, 256> : forward_kernel<T, VEC, true, 1024>;
+    CNL_TRY(ensure_dynamic_smem(kernel, bytes));
+    kernel<<<grid, p.block, bytes, st>>>(a);
     return after_launch("blocknorm forward");
 }
 
 template <typename T, bool VEC>
 int launch_backward(const Args& a, const Plan& p, cudaStream_t st) {
     const unsigned grid = (unsigned)(p.groups * p.nb);
-    const int narrow = K * p.block * (int)sizeof(float);
-    if (p.tpr <= 32) backward_kernel<T, VEC, false, 256><<<grid, p.block, narrow, st>>>(a);
-    else if (p.tpr <= 256) backward_kernel<T, VEC, true, 256><<<grid, p.block, narrow, st>>>(a);
-    else {
-        CNL_TRY(ensure_dynamic_smem(backward_kernel<T, VEC, true, 1024>, kSums * narrow));
-        backward_kernel<T, VEC, true, 1024><<<grid, p.block, kSums * narrow, st>>>(a);
-    }
+    const int join = K * p.block * (int)sizeof(float);                   // the block's join of one of the four sums
+    const int slots = p.tpr <= 256 ? Slots<T, VEC, 5, kStagesOf<T>>::bytes * p.block : kSums * join;
+    const int bytes = slots > join ? slots : join;
+    auto* kernel = p.tpr <= 32 ? backward_kernel<T, VEC, false, 256> : p.tpr <= 256 ? backward_kernel<T, VEC, true, 256> : backward_kernel<T, VEC, true, 1024>;
+    CNL_TRY(ensure_dynamic_smem(kernel, bytes));
+    kernel<<<grid, p.block, bytes, st>>>(a);
     return after_launch("blocknorm backward");
 }
 
@@ -622,7 +768,7 @@ extern "C" int cnl_blocknorm_forward(const void* x, const void* u, const void* g
     int sms = 0;
     CNL_TRY(sm_count(&sms));
     Plan p;
-    CNL_TRY(plan(rows, d, gate_mode == 2 ? groups : 1, vec, d > 256 * K ? 2 * sms : 8 * sms, &p));
+    CNL_TRY(plan(rows, d, gate_mode == 2 ? groups : 1, vec, d > 256 * K ? sms : 3 * sms, &p));      // as many blocks as are resident
     a.rows = rows; a.per = rows / p.groups; a.d = d; a.tpr = p.tpr; a.nb = p.nb; a.eps = eps; a.inv_d = 1.0f / (float)d;
     a.layer = layer; a.gate_full = gate_mode == 1; a.gate_group = gate_mode == 2; a.sigmoid = sigmoid_gate;
     a.w_f32 = wdtype == CNL_F32; a.fmt = fmt;

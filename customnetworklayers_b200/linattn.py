@@ -13,18 +13,18 @@ from typing import Optional
 import torch
 from torch import nn
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._tensor import DTYPES, check_tensor, launch, ptr, wants_grad
+from ._tensor import DTYPES, check_tensor, first_order, launch, on_device, ptr, wants_grad
 
 MAX_HEAD = 128
+_ARRAYS = {n: ctypes.c_longlong * n for n in (6, 9, 12)}
 
 
 def _strides(*tensors):
     """HOST array of the strides, in elements, of every dimension but the last."""
     flat = [s for t in tensors for s in t.stride()[:-1]]
-    return (ctypes.c_longlong * len(flat))(*flat)
+    return _ARRAYS[len(flat)](*flat)
 
 
 def _check(q, k, v, log_decay, state, lengths, dims: int):
@@ -57,8 +57,7 @@ def forward(q, k, v, log_decay, state=None, lengths=None, scale: Optional[float]
     lib = _lib.load()
     out = torch.empty((b, t, h, dv), dtype=q.dtype, device=q.device)
     end = torch.empty((b, h, dk, dv), dtype=torch.float32, device=q.device)
-    with torch.cuda.device(q.device):
-        segments = lib.cnl_linattn_segments(b, t, h)
+    segments = on_device(q.device, lib.cnl_linattn_segments, b, t, h)
     if segments < 1:
         raise RuntimeError("linear attention: " + _lib.last_error())
     starts = torch.empty((b, h, segments, dk, dv), dtype=torch.float32, device=q.device) if segments > 1 else None
@@ -107,7 +106,7 @@ class LinearAttentionFunction(Function):
         return out, end
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, grad_out, grad_state):
         q, k, v, log_decay, state, lengths, starts = ctx.saved_tensors
         if grad_out is None and grad_state is None:
