@@ -17,29 +17,10 @@
 // joined in a fixed order across the block and then, by a second small kernel, over the blocks: same bits every call.
 #include <type_traits>
 
-#include "ckpt8.cuh"
+#include "blocknorm.cuh"
 
 namespace cnl {
 namespace bnorm {
-
-constexpr int K = 8;                 // channels a thread holds
-constexpr int kMaxD = 8192;
-constexpr int kSums = 4;             // A, B, dw1, db1
-
-struct Args {
-    const void *x, *u, *gate;                     // [rows][d]; gate [rows][d], [groups][d] or null
-    const void *scale, *w2, *b2, *w1, *b1;        // [d] each, scale / b2 / b1 may be null; w1 null: no h
-    void *y, *h;
-    float4* stats;                                // per row: mu_u, r_u, mu_y, r_y
-    unsigned char *codes, *scales;                // 8-bit forms of x, u and a full gate, [3][rows][d] and [3][rows][blocks]
-    const void *dy, *dh;
-    void *dx, *du, *dgate;
-    float* partial;                               // [groups * nb][4][d]
-    long long rows, per;                          // rows in all, rows of a group
-    int d, tpr, nb;                               // channels, threads of a row, blocks of a group
-    float eps, inv_d;
-    int layer, gate_full, gate_group, sigmoid, w_f32, fmt;
-};
 
 // ---- eight channels of a row ------------------------------------------------------------------------------------
 // VEC: channels 8 t .. 8 t + 7 as 16-byte vectors (d a multiple of 8, aligned rows); otherwise channels t, t + tpr, ...
@@ -150,70 +131,6 @@ __device__ __forceinline__ void get_codes(const unsigned char* __restrict__ code
     }
 }
 
-// ---- rows on their way --------------------------------------------------------------------------------------------
-// VEC rows arrive by cp.async in slots of shared memory that belong to one thread each: a thread waits for its own copies and
-// needs no barrier, and STAGES - 1 rows are under way while one is worked on without costing registers.  An SM needs some
-// 45 KB in flight to keep HBM busy; 512 threads with five 16-byte tensors a row are 40 KB a stage.
-template <typename T, bool VEC, int TENSORS, int STAGES>
-struct Slots {
-    static constexpr int kParts = VEC ? (int)sizeof(T) * K / 16 : 0;       // 16-byte parts of a thread's channels
-    static constexpr int bytes = TENSORS * kParts * STAGES * 16;           // for one thread
-    unsigned char* base;
-
-    __device__ __forceinline__ unsigned char* at(int stage, int tensor, int part) const {
-        return base + (((stage * TENSORS + tensor) * kParts + part) * blockDim.x + threadIdx.x) * 16;
-    }
-    __device__ __forceinline__ void ask(int stage, int tensor, const T* __restrict__ row, const Args& a, int t) const {
-        if (t * K < a.d) {
-#pragma unroll
-            for (int i = 0; i < kParts; ++i)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(at(stage, tensor, i))),
-                             "l"(reinterpret_cast<const unsigned char*>(row + t * K) + 16 * i) : "memory");
-        }
-    }
-    __device__ __forceinline__ void ask_codes(int stage, int tensor, const unsigned char* __restrict__ codes, const Args& a, int t) const {
-        if (t * K < a.d)
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((unsigned)__cvta_generic_to_shared(at(stage, tensor, 0))), "l"(codes + t * K) : "memory");
-    }
-    __device__ __forceinline__ void close() const { asm volatile("cp.async.commit_group;" ::: "memory"); }
-    __device__ __forceinline__ void wait() const { asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory"); }
-
-    __device__ __forceinline__ void take(int stage, int tensor, const Args& a, int t, float (&v)[K]) const {
-        if (t * K < a.d) {
-            if constexpr (kParts == 2) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float4 q = *reinterpret_cast<const float4*>(at(stage, tensor, i));
-                    v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
-                }
-            } else if constexpr (kParts == 1) {
-                const uint4 q = *reinterpret_cast<const uint4*>(at(stage, tensor, 0));
-                const unsigned w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 f = unpack2(w[j], T());
-                    v[2 * j] = f.x; v[2 * j + 1] = f.y;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < K; ++k) v[k] = 0.0f;
-        }
-    }
-    __device__ __forceinline__ void take_codes(int stage, int tensor, int s, const Args& a, int t, float (&v)[K]) const {
-        if (t * K < a.d) {
-            const uint2 q = *reinterpret_cast<const uint2*>(at(stage, tensor, 0));
-            const unsigned w[2] = {q.x, q.y};
-            if (a.fmt == CNL_CKPT_INT8) ckpt8::decode<CNL_CKPT_INT8, K>(w, s, v);
-            else ckpt8::decode<CNL_CKPT_E4M3, K>(w, s, v);
-        } else {
-#pragma unroll
-            for (int k = 0; k < K; ++k) v[k] = 0.0f;
-        }
-    }
-};
-template <typename T> constexpr int kStagesOf = sizeof(T) == 4 ? 2 : 3;
-
 // ---- sums over a row --------------------------------------------------------------------------------------------
 // WIDE: a row spans several warps, whose sums meet in shared memory (two buffers in turn, so one barrier a sum).
 // The barrier is one of its own for every row slot of the block: rows do not wait for one another.
@@ -267,52 +184,24 @@ __device__ __forceinline__ void center(float (&v)[K], const Args& a, int t, floa
     r = rsqrtf(fmaf(s[0], a.inv_d, a.eps));
 }
 
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
-
 // ---- forward ----------------------------------------------------------------------------------------------------
 template <typename T, bool VEC, bool WIDE, int BLOCK>
 __global__ void __launch_bounds__(BLOCK, BLOCK <= 256 ? 3 : 1) forward_kernel(const Args a) {
-    constexpr int kStages = kStagesOf<T>;
-    extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ float sm[2 * 32 * 2];
-    const Slots<T, VEC, 3, kStages> slots = {dynamic};
     const int rpb = blockDim.x / a.tpr, slot = threadIdx.x / a.tpr, t = threadIdx.x - slot * a.tpr;
     const long long group = blockIdx.x / a.nb;
     const int j = blockIdx.x - (int)(group * a.nb);
     const long long begin = group * a.per + (long long)j * rpb, end = (group + 1) * a.per, step = (long long)a.nb * rpb;
     const int blocks = (a.d + 31) >> 5;
-    auto ask = [&](int stage, long long base) {
-        if constexpr (VEC) {
-            const long long row = base + slot;
-            if (row < end) {
-                const long long off = row * a.d;
-                slots.ask(stage, 0, (const T*)a.x + off, a, t);
-                if (a.u) slots.ask(stage, 1, (const T*)a.u + off, a, t);
-                if (a.gate_full) slots.ask(stage, 2, (const T*)a.gate + off, a, t);
-            }
-            slots.close();
-        }
-    };
-    int turn = 0, stage = 0;
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) ask(i, begin + i * step);
+    int turn = 0;
     for (long long base = begin; base < end; base += step) {
         const long long row = base + slot;
         const bool live = row < end;
         const long long off = (live ? row : base) * a.d;
         float y[K], u[K], z[K];
-        if constexpr (VEC) {
-            slots.wait();
-            slots.take(stage, 0, a, t, y);
-            if (a.u) slots.take(stage, 1, a, t, u);
-            if (a.gate_full) slots.take(stage, 2, a, t, z);
-            ask(stage == 0 ? kStages - 1 : stage - 1, base + (kStages - 1) * step);
-            stage = stage == kStages - 1 ? 0 : stage + 1;
-        } else {
-            get<T, VEC>((const T*)a.x + off, a, t, y);
-            if (a.u) get<T, VEC>((const T*)a.u + off, a, t, u);
-            if (a.gate_full) get<T, VEC>((const T*)a.gate + off, a, t, z);
-        }
+        get<T, VEC>((const T*)a.x + off, a, t, y);
+        if (a.u) get<T, VEC>((const T*)a.u + off, a, t, u);
+        if (a.gate_full) get<T, VEC>((const T*)a.gate + off, a, t, z);
         if (a.gate_group) get<T, VEC>((const T*)a.gate + group * a.d, a, t, z);
         float mu_u = 0.0f, r_u = 0.0f, mu_y = 0.0f, r_y = 0.0f;
         if (a.codes) {
@@ -354,12 +243,8 @@ __global__ void __launch_bounds__(BLOCK, BLOCK <= 256 ? 3 : 1) forward_kernel(co
 template <typename T, bool VEC, bool WIDE, int BLOCK>
 __global__ void __launch_bounds__(BLOCK, BLOCK <= 256 ? 2 : 1) backward_kernel(const Args a) {
     constexpr bool kSharedSums = BLOCK > 256;                              // rows of up to 1024 threads: 64 registers each, sums in shared memory
-    constexpr bool kAsync = VEC && !kSharedSums;
-    constexpr int kStages = kStagesOf<T>;
-    extern __shared__ __align__(16) unsigned char dynamic[];
+    extern __shared__ float dyn[];
     __shared__ float sm[2 * 32 * 2];
-    const Slots<T, kAsync, 5, kStages> slots = {dynamic};
-    float* dyn = reinterpret_cast<float*>(dynamic);                        // the sums, once the rows are done
     const int rpb = blockDim.x / a.tpr, slot = threadIdx.x / a.tpr, t = threadIdx.x - slot * a.tpr;
     const long long group = blockIdx.x / a.nb;
     const int j = blockIdx.x - (int)(group * a.nb);
@@ -379,79 +264,24 @@ __global__ void __launch_bounds__(BLOCK, BLOCK <= 256 ? 2 : 1) backward_kernel(c
         if constexpr (kSharedSums) dyn[(i * K + k) * blockDim.x + threadIdx.x] += v;
         else acc[i][k] += v;
     };
-    // statistics and scale bytes of a row; asked for one row ahead
-    float4 st_next = {};
-    unsigned sc_next = 0;
-    auto small = [&](long long base) {
-        const long long row = base + slot;
-        if (row >= end) return;
-        st_next = __ldg(a.stats + row);
-        if (kAsync && a.fmt && t * K < a.d) {
-            const unsigned char* sc = a.scales + row * blocks + (t >> 2);
-            sc_next = (a.dh ? __ldg(sc) : 0u) | (a.u ? __ldg(sc + nb) : 0u) << 8 | (a.gate_full ? __ldg(sc + 2 * nb) : 0u) << 16;
-        }
-    };
-    auto ask = [&](int stage, long long base) {
-        if constexpr (kAsync) {
-            const long long row = base + slot;
-            if (row < end) {
-                const long long off = row * a.d;
-                if (a.dy) slots.ask(stage, 0, (const T*)a.dy + off, a, t);
-                if (a.dh) slots.ask(stage, 1, (const T*)a.dh + off, a, t);
-                if (a.fmt) {
-                    if (a.dh) slots.ask_codes(stage, 2, a.codes + off, a, t);
-                    if (a.u) slots.ask_codes(stage, 3, a.codes + n + off, a, t);
-                    if (a.gate_full) slots.ask_codes(stage, 4, a.codes + 2 * n + off, a, t);
-                } else {
-                    if (a.dh) slots.ask(stage, 2, (const T*)a.x + off, a, t);
-                    if (a.u) slots.ask(stage, 3, (const T*)a.u + off, a, t);
-                    if (a.gate_full) slots.ask(stage, 4, (const T*)a.gate + off, a, t);
-                }
-            }
-            slots.close();
-        }
-    };
-    int turn = 0, stage = 0;
-    small(begin);
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) ask(i, begin + i * step);
+    int turn = 0;
     for (long long base = begin; base < end; base += step) {
         const long long row = base + slot;
         const bool live = row < end;
-        const long long off = (live ? row : base) * a.d;
-        const float4 st = st_next;
-        const unsigned sc = sc_next;
+        const long long at = live ? row : base, off = at * a.d, so = at * blocks;
+        const float4 st = __ldg(a.stats + at);
         float g[K], y[K], u[K], z[K], dh[K];
-        if constexpr (kAsync) {
-            slots.wait();
-            if (a.dy) slots.take(stage, 0, a, t, g);
-            if (a.dh) slots.take(stage, 1, a, t, dh);
-            if (a.fmt) {
-                if (a.dh) slots.take_codes(stage, 2, ckpt8::scale_exponent((unsigned char)sc), a, t, y);
-                if (a.u) slots.take_codes(stage, 3, ckpt8::scale_exponent((unsigned char)(sc >> 8)), a, t, u);
-                if (a.gate_full) slots.take_codes(stage, 4, ckpt8::scale_exponent((unsigned char)(sc >> 16)), a, t, z);
-            } else {
-                if (a.dh) slots.take(stage, 2, a, t, y);
-                if (a.u) slots.take(stage, 3, a, t, u);
-                if (a.gate_full) slots.take(stage, 4, a, t, z);
-            }
-            ask(stage == 0 ? kStages - 1 : stage - 1, base + (kStages - 1) * step);
-            stage = stage == kStages - 1 ? 0 : stage + 1;
+        if (a.fmt) {
+            if (a.dh) get_codes<VEC>(a.codes + off, a.scales + so, a, t, y);
+            if (a.u) get_codes<VEC>(a.codes + n + off, a.scales + nb + so, a, t, u);
+            if (a.gate_full) get_codes<VEC>(a.codes + 2 * n + off, a.scales + 2 * nb + so, a, t, z);
         } else {
-            const long long so = (live ? row : base) * blocks;
-            if (a.fmt) {
-                if (a.dh) get_codes<VEC>(a.codes + off, a.scales + so, a, t, y);
-                if (a.u) get_codes<VEC>(a.codes + n + off, a.scales + nb + so, a, t, u);
-                if (a.gate_full) get_codes<VEC>(a.codes + 2 * n + off, a.scales + 2 * nb + so, a, t, z);
-            } else {
-                if (a.dh) get<T, VEC>((const T*)a.x + off, a, t, y);
-                if (a.u) get<T, VEC>((const T*)a.u + off, a, t, u);
-                if (a.gate_full) get<T, VEC>((const T*)a.gate + off, a, t, z);
-            }
-            if (a.dy) get<T, VEC>((const T*)a.dy + off, a, t, g);
-            if (a.dh) get<T, VEC>((const T*)a.dh + off, a, t, dh);
+            if (a.dh) get<T, VEC>((const T*)a.x + off, a, t, y);
+            if (a.u) get<T, VEC>((const T*)a.u + off, a, t, u);
+            if (a.gate_full) get<T, VEC>((const T*)a.gate + off, a, t, z);
         }
-        small(base + step);
+        if (a.dy) get<T, VEC>((const T*)a.dy + off, a, t, g);
+        if (a.dh) get<T, VEC>((const T*)a.dh + off, a, t, dh);
         if (a.gate_group) get<T, VEC>((const T*)a.gate + group * a.d, a, t, z);
         if (!a.dy) {
 #pragma unroll
@@ -522,8 +352,6 @@ __global__ void __launch_bounds__(BLOCK, BLOCK <= 256 ? 2 : 1) backward_kernel(c
                 if (slot == 0 && c < a.d) out[i * a.d + c] = dyn[(i * K + k) * blockDim.x + threadIdx.x];
             }
     } else {
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncthreads();                                                   // the slots become the sums' room
         const int unit = WIDE ? a.tpr : 32, units = WIDE ? rpb : blockDim.x >> 5;
 #pragma unroll
         for (int i = 0; i < kSums; ++i) {
@@ -555,7 +383,7 @@ struct SumArgs {
     float* per_group;                             // [groups][4][d] when there are several groups
     const void *gate, *scale, *w2, *b2;
     void *dgate, *dscale, *dw2, *db2, *dw1, *db1;
-    int d, nb, groups, gate_group, sigmoid, w_f32;
+    int d, nb, groups, gate_group, sigmoid, w_f32, need_b;
 };
 
 template <typename T>
@@ -570,11 +398,11 @@ __device__ __forceinline__ void put_param(void* p, int w_f32, int c, float v) {
 }
 
 // 32 channels x 32 threads over `count` rows of [4][d] sums; the threads' sums are joined in order, in 64 bits
-__device__ __forceinline__ void column_sums(const float* src, long long count, int d, int c, double (*sm)[32][33], double (&v)[kSums]) {
+__device__ __forceinline__ void column_sums(const float* src, long long count, int d, int c, int need_b, double (*sm)[32][33], double (&v)[kSums]) {
 #pragma unroll
     for (int i = 0; i < kSums; ++i) {
         double s = 0.0;
-        if (c < d)
+        if (c < d && (need_b || !(i & 1)))                                 // B and db1 are not written where nothing asks for them
             for (long long p = threadIdx.y; p < count; p += 32) s += (double)src[(p * kSums + i) * d + c];
         sm[i][threadIdx.y][threadIdx.x] = s;
     }
@@ -605,7 +433,7 @@ __global__ void __launch_bounds__(1024) sum_blocks_kernel(const SumArgs a) {
     const int c = blockIdx.x * 32 + threadIdx.x;
     const long long group = blockIdx.y;
     double v[kSums];
-    column_sums(a.partial + group * a.nb * kSums * a.d, a.nb, a.d, c, sm, v);
+    column_sums(a.partial + group * a.nb * kSums * a.d, a.nb, a.d, c, a.need_b, sm, v);
     if (threadIdx.y != 0 || c >= a.d) return;
     float A = (float)v[0], B = (float)v[1];
     if (a.gate_group) {
@@ -632,16 +460,11 @@ __global__ void __launch_bounds__(1024) sum_groups_kernel(const SumArgs a) {
     __shared__ double sm[kSums][32][33];
     const int c = blockIdx.x * 32 + threadIdx.x;
     double v[kSums];
-    column_sums(a.per_group, a.groups, a.d, c, sm, v);
+    column_sums(a.per_group, a.groups, a.d, c, a.need_b, sm, v);
     if (threadIdx.y == 0 && c < a.d) finish<T>(a, c, (float)v[0], (float)v[1], (float)v[2], (float)v[3]);
 }
 
 // ---- launch -----------------------------------------------------------------------------------------------------
-struct Plan {
-    int tpr, block, rpb, nb;
-    long long groups;
-};
-
 // threads of a row: a power of two up to a warp, whole warps above; unaligned rows take whole warps
 inline int plan(long long rows, int d, long long groups, bool vec, int blocks_wanted, Plan* p) {
     const int need = (d + K - 1) / K;
@@ -678,13 +501,14 @@ inline bool aligned_all(const void* const* p, int n) {
     return true;
 }
 
+// Rows without vectors, or over kVecMaxD channels.
 template <typename T, bool VEC>
 int launch_forward(const Args& a, const Plan& p, cudaStream_t st) {
     const unsigned grid = (unsigned)(p.groups * p.nb);
-    const int bytes = Slots<T, VEC, 3, kStagesOf<T>>::bytes * p.block;
-    auto* kernel = p.tpr <= 32 ? forward_kernel<T, VEC, false, 256> : p.tpr <= 256 ? forward_kernel<T, VEC, true, 256> : forward_kernel<T, VEC, true, 1024>;
-    CNL_TRY(ensure_dynamic_smem(kernel, bytes));
-    kernel<<<grid, p.block, bytes, st>>>(a);
+    if constexpr (VEC) forward_kernel<T, true, true, 1024><<<grid, p.block, 0, st>>>(a);
+    else if (p.tpr <= 32) forward_kernel<T, false, false, 256><<<grid, p.block, 0, st>>>(a);
+    else if (p.tpr <= 256) forward_kernel<T, false, true, 256><<<grid, p.block, 0, st>>>(a);
+    else forward_kernel<T, false, true, 1024><<<grid, p.block, 0, st>>>(a);
     return after_launch("blocknorm forward");
 }
 
@@ -692,9 +516,10 @@ template <typename T, bool VEC>
 int launch_backward(const Args& a, const Plan& p, cudaStream_t st) {
     const unsigned grid = (unsigned)(p.groups * p.nb);
     const int join = K * p.block * (int)sizeof(float);                   // the block's join of one of the four sums
-    const int slots = p.tpr <= 256 ? Slots<T, VEC, 5, kStagesOf<T>>::bytes * p.block : kSums * join;
-    const int bytes = slots > join ? slots : join;
-    auto* kernel = p.tpr <= 32 ? backward_kernel<T, VEC, false, 256> : p.tpr <= 256 ? backward_kernel<T, VEC, true, 256> : backward_kernel<T, VEC, true, 1024>;
+    const int bytes = p.tpr <= 256 ? join : kSums * join;
+    void (*kernel)(const Args);
+    if constexpr (VEC) kernel = backward_kernel<T, true, true, 1024>;
+    else kernel = p.tpr <= 32 ? backward_kernel<T, false, false, 256> : p.tpr <= 256 ? backward_kernel<T, false, true, 256> : backward_kernel<T, false, true, 1024>;
     CNL_TRY(ensure_dynamic_smem(kernel, bytes));
     kernel<<<grid, p.block, bytes, st>>>(a);
     return after_launch("blocknorm backward");
@@ -768,11 +593,12 @@ extern "C" int cnl_blocknorm_forward(const void* x, const void* u, const void* g
     int sms = 0;
     CNL_TRY(sm_count(&sms));
     Plan p;
-    CNL_TRY(plan(rows, d, gate_mode == 2 ? groups : 1, vec, d > 256 * K ? sms : 3 * sms, &p));      // as many blocks as are resident
+    CNL_TRY(plan(rows, d, gate_mode == 2 ? groups : 1, vec, d > 256 * K ? sms : vec ? 2 * sms : 3 * sms, &p));      // as many blocks as are resident
     a.rows = rows; a.per = rows / p.groups; a.d = d; a.tpr = p.tpr; a.nb = p.nb; a.eps = eps; a.inv_d = 1.0f / (float)d;
     a.layer = layer; a.gate_full = gate_mode == 1; a.gate_group = gate_mode == 2; a.sigmoid = sigmoid_gate;
     a.w_f32 = wdtype == CNL_F32; a.fmt = fmt;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (vec && d <= kVecMaxD) return run_forward_vec(a, p, dtype, st);
     if (dtype == CNL_F32) return vec ? launch_forward<float, true>(a, p, st) : launch_forward<float, false>(a, p, st);
     if (dtype == CNL_F16) return vec ? launch_forward<__half, true>(a, p, st) : launch_forward<__half, false>(a, p, st);
     return vec ? launch_forward<__nv_bfloat16, true>(a, p, st) : launch_forward<__nv_bfloat16, false>(a, p, st);
@@ -810,9 +636,11 @@ extern "C" int cnl_blocknorm_backward(const void* x, const void* u, const void* 
     a.rows = rows; a.per = rows / p.groups; a.d = d; a.tpr = p.tpr; a.nb = p.nb; a.inv_d = 1.0f / (float)d;
     a.layer = layer; a.gate_full = gate_mode == 1; a.gate_group = gate_mode == 2; a.sigmoid = sigmoid_gate;
     a.w_f32 = wdtype == CNL_F32; a.fmt = fmt;
+    a.need_b = b_post || b_pre || g_b_post || g_b_pre;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (rows > 0) {
-        if (dtype == CNL_F32) CNL_TRY((vec ? launch_backward<float, true>(a, p, st) : launch_backward<float, false>(a, p, st)));
+        if (vec && d <= kVecMaxD) CNL_TRY(run_backward_vec(a, p, dtype, st));
+        else if (dtype == CNL_F32) CNL_TRY((vec ? launch_backward<float, true>(a, p, st) : launch_backward<float, false>(a, p, st)));
         else if (dtype == CNL_F16) CNL_TRY((vec ? launch_backward<__half, true>(a, p, st) : launch_backward<__half, false>(a, p, st)));
         else CNL_TRY((vec ? launch_backward<__nv_bfloat16, true>(a, p, st) : launch_backward<__nv_bfloat16, false>(a, p, st)));
     }
@@ -820,7 +648,7 @@ extern "C" int cnl_blocknorm_backward(const void* x, const void* u, const void* 
     s.partial = a.partial; s.per_group = a.partial + (long long)p.groups * p.nb * kSums * d;
     s.gate = gate; s.scale = scale; s.w2 = w_post; s.b2 = b_post;
     s.dgate = gate_mode == 2 ? g_gate : nullptr; s.dscale = g_scale; s.dw2 = g_w_post; s.db2 = g_b_post; s.dw1 = g_w_pre; s.db1 = g_b_pre;
-    s.d = d; s.nb = rows > 0 ? p.nb : 0; s.groups = (int)p.groups; s.gate_group = gate_mode == 2; s.sigmoid = sigmoid_gate; s.w_f32 = a.w_f32;
+    s.d = d; s.nb = rows > 0 ? p.nb : 0; s.groups = (int)p.groups; s.gate_group = gate_mode == 2; s.sigmoid = sigmoid_gate; s.w_f32 = a.w_f32; s.need_b = a.need_b;
     if (dtype == CNL_F32) return sums<float>(s, st);
     if (dtype == CNL_F16) return sums<__half>(s, st);
     return sums<__nv_bfloat16>(s, st);

@@ -71,6 +71,19 @@ __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&v)[N]
     }
 }
 
+// 2^x and 1/x by the special-function unit (2 ulp and 1 ulp), subnormals to zero: the plain intrinsics spend three more
+// instructions each on subnormals, which no value here needs.
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<size_t>(p) & 15) == 0; }
 
 inline int check_dtype(int dtype) {
