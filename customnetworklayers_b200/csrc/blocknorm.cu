@@ -76,24 +76,21 @@ template <bool VEC>
 __device__ __forceinline__ void put_codes(unsigned char* __restrict__ codes, unsigned char* __restrict__ scales, const Args& a, int t,
                                           bool live, const float (&v)[K]) {
     if constexpr (VEC) {
-        unsigned char c[K];
+        unsigned c[2];
         const int s = a.fmt == CNL_CKPT_INT8 ? ckpt8::encode<CNL_CKPT_INT8, 4, K>(v, c) : ckpt8::encode<CNL_CKPT_E4M3, 4, K>(v, c);
         if (live && t * K < a.d) {
-            uint2 w;
-            w.x = c[0] | c[1] << 8 | c[2] << 16 | (unsigned)c[3] << 24;
-            w.y = c[4] | c[5] << 8 | c[6] << 16 | (unsigned)c[7] << 24;
-            *reinterpret_cast<uint2*>(codes + t * K) = w;
+            *reinterpret_cast<uint2*>(codes + t * K) = make_uint2(c[0], c[1]);
             if ((t & 3) == 0) scales[t >> 2] = ckpt8::scale_byte(s);
         }
     } else {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const float one[1] = {v[k]};
-            unsigned char c[1];
+            unsigned c[1];
             const int s = a.fmt == CNL_CKPT_INT8 ? ckpt8::encode<CNL_CKPT_INT8, 32, 1>(one, c) : ckpt8::encode<CNL_CKPT_E4M3, 32, 1>(one, c);
             const int col = t + k * a.tpr;
             if (live && col < a.d) {
-                codes[col] = c[0];
+                codes[col] = (unsigned char)c[0];
                 if ((col & 31) == 0) scales[col >> 5] = ckpt8::scale_byte(s);
             }
         }
@@ -399,13 +396,26 @@ __device__ __forceinline__ void put_param(void* p, int w_f32, int c, float v) {
 
 // 32 channels x 32 threads over `count` rows of [4][d] sums; the threads' sums are joined in order, in 64 bits
 __device__ __forceinline__ void column_sums(const float* src, long long count, int d, int c, int need_b, double (*sm)[32][33], double (&v)[kSums]) {
+    double s[kSums] = {0.0, 0.0, 0.0, 0.0};
+    if (c < d) {
+        constexpr int kAhead = 4;                                          // rows whose sums are asked for together
+        for (long long p0 = threadIdx.y; p0 < count; p0 += 32 * kAhead) {
+            float f[kAhead][kSums];
 #pragma unroll
-    for (int i = 0; i < kSums; ++i) {
-        double s = 0.0;
-        if (c < d && (need_b || !(i & 1)))                                 // B and db1 are not written where nothing asks for them
-            for (long long p = threadIdx.y; p < count; p += 32) s += (double)src[(p * kSums + i) * d + c];
-        sm[i][threadIdx.y][threadIdx.x] = s;
+            for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+                for (int i = 0; i < kSums; ++i) {                          // B and db1 are not written where nothing asks for them
+                    const long long p = p0 + 32 * k;
+                    f[k][i] = p < count && (need_b || !(i & 1)) ? src[(p * kSums + i) * d + c] : 0.0f;
+                }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+                for (int i = 0; i < kSums; ++i) s[i] += (double)f[k][i];
+        }
     }
+#pragma unroll
+    for (int i = 0; i < kSums; ++i) sm[i][threadIdx.y][threadIdx.x] = s[i];
     __syncthreads();
     for (int half = 16; half > 0; half >>= 1) {
         if (threadIdx.y < half)
@@ -593,7 +603,7 @@ extern "C" int cnl_blocknorm_forward(const void* x, const void* u, const void* g
     int sms = 0;
     CNL_TRY(sm_count(&sms));
     Plan p;
-    CNL_TRY(plan(rows, d, gate_mode == 2 ? groups : 1, vec, d > 256 * K ? sms : vec ? 2 * sms : 3 * sms, &p));      // as many blocks as are resident
+    CNL_TRY(plan(rows, d, gate_mode == 2 ? groups : 1, vec, d > 256 * K ? sms : vec && (b_post || b_pre) ? 2 * sms : 3 * sms, &p));      // as many blocks as are resident
     a.rows = rows; a.per = rows / p.groups; a.d = d; a.tpr = p.tpr; a.nb = p.nb; a.eps = eps; a.inv_d = 1.0f / (float)d;
     a.layer = layer; a.gate_full = gate_mode == 1; a.gate_group = gate_mode == 2; a.sigmoid = sigmoid_gate;
     a.w_f32 = wdtype == CNL_F32; a.fmt = fmt;

@@ -86,10 +86,10 @@ __device__ __forceinline__ void vector8(const void* p, int wide, int c, float ot
 
 __device__ __forceinline__ void put_codes(unsigned char* codes, unsigned char* scale, int fmt, bool on, bool first, const float2 (&v)[4]) {
     const float f[8] = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
-    unsigned char c[8];
+    unsigned c[2];
     const int s = fmt == CNL_CKPT_INT8 ? ckpt8::encode<CNL_CKPT_INT8, 4, 8>(f, c) : ckpt8::encode<CNL_CKPT_E4M3, 4, 8>(f, c);
     if (on) {
-        *reinterpret_cast<uint2*>(codes) = make_uint2(c[0] | c[1] << 8 | c[2] << 16 | (unsigned)c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | (unsigned)c[7] << 24);
+        *reinterpret_cast<uint2*>(codes) = make_uint2(c[0], c[1]);
         if (first) *scale = ckpt8::scale_byte(s);
     }
 }
@@ -162,8 +162,9 @@ __device__ __forceinline__ float2 gate2(float2 z, int sig) {
 }
 
 // ---- forward --------------------------------------------------------------------------------------------------------
-template <typename T, bool WIDE, bool LAYER, int BLOCK>
-__global__ void __launch_bounds__(BLOCK, 512 / BLOCK) forward_vec(const Args a) {
+// BIAS: a bias takes part.  Without one the registers allow three blocks of 256 an SM.
+template <typename T, bool WIDE, bool LAYER, bool BIAS, int BLOCK>
+__global__ void __launch_bounds__(BLOCK, BLOCK == 512 ? 1 : BIAS ? 2 : 3) forward_vec(const Args a) {
     using S = Slots<T, 3, BLOCK>;
     extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ float meet[128];
@@ -196,15 +197,15 @@ __global__ void __launch_bounds__(BLOCK, 512 / BLOCK) forward_vec(const Args a) 
 #pragma unroll
     for (int i = 0; i < S::kStages - 1; ++i) ask();
 
-    float2 sw[4], sb[4], w1[4], b1[4], z[4], x[4], u[4];
+    float2 sw[4], sb[4], w1[4], b1[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) sw[k] = sb[k] = w1[k] = b1[k] = z[k] = x[k] = u[k] = f2(0.0f);
+    for (int k = 0; k < 4; ++k) sw[k] = sb[k] = w1[k] = b1[k] = f2(0.0f);
     if (in) {
         if (has_u) {
             float2 s[4];
             vector8<T>(a.scale, a.w_f32, c, 1.0f, s);
             vector8<T>(a.w2, a.w_f32, c, 0.0f, sw);
-            vector8<T>(a.b2, a.w_f32, c, 0.0f, sb);
+            if constexpr (BIAS) vector8<T>(a.b2, a.w_f32, c, 0.0f, sb);
 #pragma unroll
             for (int k = 0; k < 4; ++k) { sw[k] = __fmul2_rn(sw[k], s[k]); sb[k] = __fmul2_rn(sb[k], s[k]); }
             if (a.gate_group) {                                            // one gate for all rows of this block: part of s
@@ -220,12 +221,15 @@ __global__ void __launch_bounds__(BLOCK, 512 / BLOCK) forward_vec(const Args a) 
         }
         if (has_h) {
             vector8<T>(a.w1, a.w_f32, c, 0.0f, w1);
-            vector8<T>(a.b1, a.w_f32, c, 0.0f, b1);
+            if constexpr (BIAS) vector8<T>(a.b1, a.w_f32, c, 0.0f, b1);
         }
     }
     const int blocks = (a.d + 31) >> 5;
     for (int it = 0; it < count; ++it) {
         const bool on = in && it < mine;
+        float2 z[4], x[4], u[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) z[k] = x[k] = u[k] = f2(0.0f);
         S::wait();
         if (on) {
             slots.take(from, 0, x);
@@ -245,17 +249,17 @@ __global__ void __launch_bounds__(BLOCK, 512 / BLOCK) forward_vec(const Args a) 
             normalise<WIDE, LAYER>(u, in, a, row, mu_u, r_u);
             if (a.gate_full) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) x[k] = __ffma2_rn(gate2(z[k], a.sigmoid), __ffma2_rn(u[k], sw[k], sb[k]), x[k]);
+                for (int k = 0; k < 4; ++k) x[k] = __ffma2_rn(gate2(z[k], a.sigmoid), BIAS ? __ffma2_rn(u[k], sw[k], sb[k]) : __fmul2_rn(u[k], sw[k]), x[k]);
             } else {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) x[k] = __fadd2_rn(__ffma2_rn(u[k], sw[k], sb[k]), x[k]);
+                for (int k = 0; k < 4; ++k) x[k] = BIAS ? __fadd2_rn(__ffma2_rn(u[k], sw[k], sb[k]), x[k]) : __ffma2_rn(u[k], sw[k], x[k]);
             }
             if (on) put<T>((T*)a.y + at, x);
         }
         if (has_h) {
             normalise<WIDE, LAYER>(x, in, a, row, mu_y, r_y);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = __ffma2_rn(x[k], w1[k], b1[k]);
+            for (int k = 0; k < 4; ++k) x[k] = BIAS ? __ffma2_rn(x[k], w1[k], b1[k]) : __fmul2_rn(x[k], w1[k]);
             if (on) put<T>((T*)a.h + at, x);
         }
         if (a.stats && on && t == 0) a.stats[begin + it * step] = make_float4(mu_u, r_u, mu_y, r_y);
@@ -489,7 +493,9 @@ __global__ void __launch_bounds__(BLOCK, 512 / BLOCK) backward_vec(const Args a)
 
 template <typename T, bool WIDE, int BLOCK>
 int forward_as(const Args& a, const Plan& p, cudaStream_t st) {
-    auto* kernel = a.layer ? forward_vec<T, WIDE, true, BLOCK> : forward_vec<T, WIDE, false, BLOCK>;
+    const bool bias = a.b2 || a.b1;
+    auto* kernel = bias ? (a.layer ? forward_vec<T, WIDE, true, true, BLOCK> : forward_vec<T, WIDE, false, true, BLOCK>)
+                        : (a.layer ? forward_vec<T, WIDE, true, false, BLOCK> : forward_vec<T, WIDE, false, false, BLOCK>);
     constexpr int bytes = Slots<T, 3, BLOCK>::kBytes;
     CNL_TRY(ensure_dynamic_smem(kernel, bytes));
     kernel<<<(unsigned)(p.groups * p.nb), p.block, bytes, st>>>(a);

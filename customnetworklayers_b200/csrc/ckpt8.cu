@@ -15,52 +15,65 @@ namespace ckpt8 {
 constexpr int kThreads = 256;
 constexpr int kUnroll = 4;
 
+__device__ __forceinline__ float2 pair(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float relu(float x) { return x > 0.0f ? x : (x == x ? 0.0f : x); }      // keeps NaN
+
 // Phi(x) = exp(-x^2/2) t P(t) for x <= 0, t = 1 / (1 + 0.3 |x|), and 1 - that for x > 0.  P was fitted here to the scaled
 // complementary error function by least squares with weights moved towards an even relative error over |x| <= 14:
 // 8.2e-6 with degree 5 (a 64th of fp16's half step), 1.6e-7 with degree 7.
+// Two at a time: packed fp32 arithmetic takes both in one issue slot, and at 5 bytes an element (16-bit types) an SM has some
+// 27 slots an element.
 template <typename T>
-__device__ __forceinline__ float cdf_tail(float x) {                     // t P(t)
-    const float t = __fdividef(1.0f, fmaf(0.3f, fabsf(x), 1.0f));
-    float p;
+__device__ __forceinline__ float2 cdf_tail(float2 x, float2 magnitude) {                 // Phi(-|x|)
+    const float2 k = __fmul2_rn(__fmul2_rn(x, x), pair(-0.7213475204444817f));           // -x^2 / 2 in powers of two
+    const float2 d = __ffma2_rn(magnitude, pair(0.3f), pair(1.0f));
+    const float2 t = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+    float2 p;
     if constexpr (sizeof(T) == 4) {
-        p = fmaf(t, 0.03567475825548172f, -0.15720295906066895f);
-        p = fmaf(t, p, 0.20635318756103516f);
-        p = fmaf(t, p, -0.053683266043663025f);
-        p = fmaf(t, p, 0.12856139242649078f);
-        p = fmaf(t, p, 0.0999135747551918f);
-        p = fmaf(t, p, 0.1207539439201355f);
-        p = fmaf(t, p, 0.11962930113077164f);
+        p = __ffma2_rn(t, pair(0.03567475825548172f), pair(-0.15720295906066895f));
+        p = __ffma2_rn(t, p, pair(0.20635318756103516f));
+        p = __ffma2_rn(t, p, pair(-0.053683266043663025f));
+        p = __ffma2_rn(t, p, pair(0.12856139242649078f));
+        p = __ffma2_rn(t, p, pair(0.0999135747551918f));
+        p = __ffma2_rn(t, p, pair(0.1207539439201355f));
+        p = __ffma2_rn(t, p, pair(0.11962930113077164f));
     } else {
-        p = fmaf(t, -0.0770978331565857f, 0.21603818237781525f);
-        p = fmaf(t, p, -0.0169492457062006f);
-        p = fmaf(t, p, 0.14419695734977722f);
-        p = fmaf(t, p, 0.11374179273843765f);
-        p = fmaf(t, p, 0.12007424235343933f);
+        p = __ffma2_rn(t, pair(-0.0770978331565857f), pair(0.21603818237781525f));
+        p = __ffma2_rn(t, p, pair(-0.0169492457062006f));
+        p = __ffma2_rn(t, p, pair(0.14419695734977722f));
+        p = __ffma2_rn(t, p, pair(0.11374179273843765f));
+        p = __ffma2_rn(t, p, pair(0.12007424235343933f));
     }
-    return t * p;
+    return __fmul2_rn(__fmul2_rn(t, p), make_float2(exp2_approx(k.x), exp2_approx(k.y)));
+}
+
+__device__ __forceinline__ float2 logistic(float2 x) {
+    const float2 e = __fmul2_rn(x, pair(-1.4426950408889634f));
+    const float2 d = __fadd2_rn(make_float2(exp2_approx(e.x), exp2_approx(e.y)), pair(1.0f));
+    return make_float2(rcp_approx(d.x), rcp_approx(d.y));
 }
 
 template <int ACT, typename T>
-__device__ __forceinline__ float act(float x) {
-    if constexpr (ACT == CNL_ACT_GELU) {
-        const float e = __expf(-0.5f * x * x);
-        const float q = cdf_tail<T>(x) * e;
-        return x * (x > 0.0f ? 1.0f - q : q);
+__device__ __forceinline__ float2 act(float2 x) {
+    if constexpr (ACT == CNL_ACT_GELU) {                                                 // x Phi(x) = max(x, 0) - |x| Phi(-|x|)
+        const float2 m = make_float2(fabsf(x.x), fabsf(x.y)), q = cdf_tail<T>(x, m);
+        return __ffma2_rn(make_float2(-m.x, -m.y), q, make_float2(relu(x.x), relu(x.y)));
     } else {
-        return __fdividef(x, 1.0f + __expf(-x));
+        return __fmul2_rn(x, logistic(x));
     }
 }
 
 template <int ACT, typename T>
-__device__ __forceinline__ float act_slope(float x) {
-    if constexpr (ACT == CNL_ACT_GELU) {
-        const float e = __expf(-0.5f * x * x);
-        const float q = cdf_tail<T>(x) * e;
-        return fmaf(x * 0.3989422804014327f, e, x > 0.0f ? 1.0f - q : q);
-    } else {
-        const float e = __expf(-fabsf(x));                       // never overflows; e / (1 + e)^2 is even in x
-        const float r = __fdividef(1.0f, 1.0f + e);
-        return fmaf(x * e, r * r, x >= 0.0f ? r : e * r);
+__device__ __forceinline__ float2 act_slope(float2 x) {
+    if constexpr (ACT == CNL_ACT_GELU) {                                                 // Phi(x) + x phi(x); Phi(x) = 1/2 + sign(x) (1/2 - Phi(-|x|))
+        const float2 m = make_float2(fabsf(x.x), fabsf(x.y)), q = cdf_tail<T>(x, m);
+        const float2 h = __fadd2_rn(pair(0.5f), make_float2(-q.x, -q.y));
+        const float2 k = __fmul2_rn(__fmul2_rn(x, x), pair(-0.7213475204444817f));
+        const float2 e = make_float2(exp2_approx(k.x), exp2_approx(k.y));               // the one in cdf_tail
+        return __ffma2_rn(__fmul2_rn(x, pair(0.3989422804014327f)), e, __fadd2_rn(make_float2(copysignf(h.x, x.x), copysignf(h.y, x.y)), pair(0.5f)));
+    } else {                                                                             // s + x s (1 - s)
+        const float2 g = logistic(x);
+        return __ffma2_rn(x, __ffma2_rn(make_float2(-g.x, -g.y), g, g), g);
     }
 }
 
@@ -87,17 +100,14 @@ __device__ __forceinline__ void write(T* __restrict__ x, long long at, long long
 }
 
 template <int V>
-__device__ __forceinline__ void write_codes(unsigned char* __restrict__ codes, long long at, long long count, const unsigned char (&c)[V]) {
+__device__ __forceinline__ void write_codes(unsigned char* __restrict__ codes, long long at, long long count, const unsigned (&w)[(V + 3) / 4]) {
     if (V > 1 && at + V <= count) {
-        unsigned w[(V + 3) / 4] = {};
-#pragma unroll
-        for (int i = 0; i < V; ++i) w[i / 4] |= (unsigned)c[i] << (8 * (i % 4));
-        if constexpr (V == 8) *reinterpret_cast<uint2*>(codes + at) = make_uint2(w[0], w[1]);
+        if constexpr (V == 8) *reinterpret_cast<uint2*>(codes + at) = make_uint2(w[0], w[(V + 3) / 4 - 1]);
         else *reinterpret_cast<unsigned*>(codes + at) = w[0];
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (at + i < count) codes[at + i] = c[i];
+            if (at + i < count) codes[at + i] = (unsigned char)(w[i / 4] >> (8 * (i % 4)));
     }
 }
 
@@ -130,14 +140,18 @@ __global__ void __launch_bounds__(kThreads) store_kernel(const T* __restrict__ x
     for (int j = 0; j < kUnroll; ++j) {
         const long long at = first + (long long)j * kThreads * V;
         if (codes) {                                              // the same for the whole grid
-            unsigned char c[V];
+            unsigned c[(V + 3) / 4];
             const int s = encode<FMT, kLanes, V>(v[j], c);
             write_codes<V>(codes, at, count, c);
             if (at < count && (threadIdx.x & (kLanes - 1)) == 0) scales[at / kBlock] = scale_byte(s);
         }
         if constexpr (ACT != 0) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[j][i] = act<ACT, T>(v[j][i]);
+            for (int i = 0; i < V; i += 2) {
+                const float2 f = act<ACT, T>(make_float2(v[j][i], v[j][i + (V > 1)]));
+                v[j][i] = f.x;
+                if (V > 1) v[j][i + (V > 1)] = f.y;
+            }
             write<T, V>(y, at, count, v[j]);
         }
     }
@@ -167,7 +181,11 @@ __global__ void __launch_bounds__(kThreads) restore_kernel(const unsigned char* 
         decode<FMT, V>(w[j], s[j], v);
         if constexpr (ACT != 0) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = gv[j][i] * act_slope<ACT, T>(v[i]);
+            for (int i = 0; i < V; i += 2) {
+                const float2 f = __fmul2_rn(make_float2(gv[j][i], gv[j][i + (V > 1)]), act_slope<ACT, T>(make_float2(v[i], v[i + (V > 1)])));
+                v[i] = f.x;
+                if (V > 1) v[i + (V > 1)] = f.y;
+            }
         } else if (s[j] > kSafe) {
 #pragma unroll
             for (int i = 0; i < V; ++i)

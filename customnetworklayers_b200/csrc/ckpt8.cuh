@@ -28,49 +28,65 @@ __device__ __forceinline__ int exponent_of(unsigned top) {
     return max(s, -126);
 }
 
-__device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 __device__ __forceinline__ bool not_finite(unsigned mag) { return mag >= 0x7f800000u; }
+__device__ __forceinline__ float max_nan(float a, float b) {             // NaN if one is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 
-// max over the `lanes` (a power of two) neighbouring lanes that hold one block
+// max over the LANES (a power of two) neighbouring lanes that hold one block
 template <int LANES>
-__device__ __forceinline__ unsigned lanes_max(unsigned v) {
+__device__ __forceinline__ float lanes_max(float v) {
 #pragma unroll
-    for (int o = 1; o < LANES; o <<= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    for (int o = 1; o < LANES; o <<= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
 
-// Codes of N elements of one block that LANES lanes hold together; returns s (the same in all of them).  N = 1, 4 or 8.
-// All lanes of the warp must call it together (v = 0 where a lane has nothing).
+// Codes of N elements of one block that LANES lanes hold together, four to a word (N = 1: in the low byte); returns s (the
+// same in all of the lanes).  All lanes of the warp must call it together (v = 0 where a lane has nothing).
 template <int FMT, int LANES, int N>
-__device__ __forceinline__ int encode(const float (&v)[N], unsigned char (&code)[N]) {
-    unsigned top = 0;
+__device__ __forceinline__ int encode(const float (&v)[N], unsigned (&word)[(N + 3) / 4]) {
+    float m = fabsf(v[0]);
 #pragma unroll
-    for (int i = 0; i < N; ++i) top = max(top, magnitude(v[i]));
-    top = lanes_max<LANES>(top);
+    for (int i = 1; i < N; ++i) m = max_nan(m, fabsf(v[i]));
+    unsigned top = __float_as_uint(lanes_max<LANES>(m));
     const bool odd = not_finite(top);
     if (__any_sync(0xffffffffu, odd)) {                          // the maximum again, over the finite elements (rare)
-        unsigned fin = 0;
+        m = 0.0f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) fin = max(fin, not_finite(magnitude(v[i])) ? 0u : magnitude(v[i]));
-        top = lanes_max<LANES>(fin);
+        for (int i = 0; i < N; ++i) m = fmaxf(m, not_finite(__float_as_uint(v[i]) & 0x7fffffffu) ? 0.0f : fabsf(v[i]));
+        top = __float_as_uint(lanes_max<LANES>(m));
     }
     const int s = exponent_of<FMT>(top);
     const float inv = __uint_as_float((unsigned)(127 - s) << 23);
-    if constexpr (FMT == CNL_CKPT_INT8) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) code[i] = (unsigned char)__float_as_uint(fmaf(v[i], inv, 12582912.0f));   // 1.5 * 2^23: rne in the low byte
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const __nv_fp8x2_storage_t p = __nv_cvt_float2_to_fp8x2(make_float2(v[i] * inv, i + 1 < N ? v[i + (N > 1)] * inv : 0.0f), __NV_SATFINITE, __NV_E4M3);
-            code[i] = (unsigned char)p;
-            if (i + 1 < N) code[i + (N > 1)] = (unsigned char)(p >> 8);
+    for (int w = 0; w < (N + 3) / 4; ++w) {
+        if constexpr (FMT == CNL_CKPT_INT8) {
+            // 1.5 * 2^23 + c: the addition rounds to nearest even and leaves c in the low byte
+            const float2 c = make_float2(12582912.0f, 12582912.0f), k = make_float2(inv, inv);
+            const float2 f = __ffma2_rn(make_float2(v[4 * w], N > 1 ? v[4 * w + (N > 1)] : 0.0f), k, c);
+            word[w] = __float_as_uint(f.x);
+            if constexpr (N > 1) {
+                const float2 g = __ffma2_rn(make_float2(v[4 * w + 2], v[4 * w + 3]), k, c);
+                word[w] = __byte_perm(__byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x0040), __byte_perm(__float_as_uint(g.x), __float_as_uint(g.y), 0x0040), 0x5410);
+            } else word[w] &= 0xffu;
+        } else {
+            const float2 k = make_float2(inv, inv), f = __fmul2_rn(make_float2(v[4 * w], N > 1 ? v[4 * w + (N > 1)] : 0.0f), k);
+            word[w] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+            if constexpr (N > 1) {
+                const float2 g = __fmul2_rn(make_float2(v[4 * w + 2], v[4 * w + 3]), k);
+                word[w] = __byte_perm(word[w], __nv_cvt_float2_to_fp8x2(g, __NV_SATFINITE, __NV_E4M3), 0x5410);
+            } else word[w] &= 0xffu;
         }
     }
     if (odd) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (not_finite(magnitude(v[i]))) code[i] = FMT == CNL_CKPT_INT8 ? 0x80 : 0x7f;
+            if (not_finite(__float_as_uint(v[i]) & 0x7fffffffu)) {
+                const int at = 8 * (i % 4);
+                word[i / 4] = (word[i / 4] & ~(0xffu << at)) | (FMT == CNL_CKPT_INT8 ? 0x80u : 0x7fu) << at;
+            }
     }
     return s;
 }
@@ -80,24 +96,37 @@ __device__ __forceinline__ int encode(const float (&v)[N], unsigned char (&code)
 template <int FMT, int N>
 __device__ __forceinline__ void decode(const unsigned* word, int s, float (&v)[N]) {
     const float unit = __uint_as_float((unsigned)(s + 127) << 23);
+    bool rare = s > 118;                                                  // may leave fp32's range
+    if constexpr (FMT == CNL_CKPT_INT8) {
+        // a byte c + 128 under the exponent of 2^23 is the float 2^23 + c + 128
 #pragma unroll
-    for (int i = 0; i < N; i += (N == 1 ? 1 : 2)) {
-        const unsigned w = word[i / 4] >> (8 * (i % 4));
-        if constexpr (FMT == CNL_CKPT_INT8) {
+        for (int i = 0; i < (N + 3) / 4; ++i) {
+            const unsigned w = word[i] ^ 0x80808080u;                     // c + 128
+            rare |= ((w - 0x01010101u) & ~w & 0x80808080u) != 0 && (N > 1 || (w & 0xffu) == 0);       // some code is -128
 #pragma unroll
-            for (int j = 0; j < (N == 1 ? 1 : 2); ++j) {
-                const unsigned c = (w >> (8 * j)) & 0xffu;
-                const float f = __uint_as_float(0x4b000000u | (c ^ 0x80u)) - 8388736.0f;          // 2^23 + (c + 128)
-                v[i + j] = (c == 0x80u ? __uint_as_float(0x7fffffffu) : f) * unit;
+            for (int j = 0; j < (N < 4 ? N : 4); j += 2) {
+                const float2 f = __fadd2_rn(make_float2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + j)), __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7441 + j))),
+                                            make_float2(-8388736.0f, -8388736.0f));
+                const float2 r = __fmul2_rn(f, make_float2(unit, unit));
+                v[4 * i + j] = r.x;
+                if (4 * i + j + 1 < N) v[4 * i + j + (N > 1)] = r.y;
             }
-        } else {
-            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
-            const float2 f = __half22float2(__half2(h));
-            v[i] = f.x * unit;
-            if constexpr (N > 1) v[i + 1] = f.y * unit;
+        }
+        if (rare) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if ((word[i / 4] >> (8 * (i % 4)) & 0xffu) == 0x80u) v[i] = __uint_as_float(0x7fffffffu);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(word[i / 4] >> (8 * (i % 4)) & 0xffffu), __NV_E4M3);
+            const float2 f = __fmul2_rn(__half22float2(__half2(h)), make_float2(unit, unit));
+            v[i] = f.x;
+            if (i + 1 < N) v[i + (N > 1)] = f.y;
         }
     }
-    if (s > 118) {
+    if (rare) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
             if (fabsf(v[i]) > 3.402823466e38f) v[i] = copysignf(3.402823466e38f, v[i]);
