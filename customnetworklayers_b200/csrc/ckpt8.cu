@@ -3,7 +3,7 @@
 //
 // Every kernel is one pass over memory and HBM bound: b + 1 + 1/32 bytes an element for store and restore, 2 b + 1 + 1/32
 // for the activations (b = 2 or 4).  A lane holds one 16-byte vector, so a block of 32 elements lies in 4 (16-bit types) or
-// 8 (fp32) neighbouring lanes and its maximum costs two or three shuffles; four vectors a thread are loaded before the first
+// 8 (fp32) neighbouring lanes and its maximum costs two or three shuffles; a thread's vectors are all loaded before the first
 // is used.  Addresses that are not 16-byte aligned take the same code with one element a lane.
 #include "ckpt8.cuh"
 
@@ -13,7 +13,9 @@ namespace cnl {
 namespace ckpt8 {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;
+// Vectors a thread has under way.  Store and restore are short and want four (restore bf16 64 us, with two 76 us, for 126M
+// elements); the activations need the registers and want two (silu backward 98 us, with four 127 us).
+template <int ACT> constexpr int kUnrollOf = ACT ? 2 : 4;
 
 __device__ __forceinline__ float2 pair(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float relu(float x) { return x > 0.0f ? x : (x == x ? 0.0f : x); }      // keeps NaN
@@ -131,7 +133,7 @@ __device__ __forceinline__ void read_codes(const unsigned char* __restrict__ cod
 template <typename T, int V, int FMT, int ACT>
 __global__ void __launch_bounds__(kThreads) store_kernel(const T* __restrict__ x, T* __restrict__ y, unsigned char* __restrict__ codes,
                                                          unsigned char* __restrict__ scales, long long count) {
-    constexpr int kLanes = kBlock / V;
+    constexpr int kLanes = kBlock / V, kUnroll = kUnrollOf<ACT>;
     const long long first = ((long long)blockIdx.x * kUnroll * kThreads + threadIdx.x) * V;
     float v[kUnroll][V];
 #pragma unroll
@@ -161,6 +163,7 @@ __global__ void __launch_bounds__(kThreads) store_kernel(const T* __restrict__ x
 template <typename T, int V, int FMT, int ACT>
 __global__ void __launch_bounds__(kThreads) restore_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
                                                            const T* __restrict__ g, T* __restrict__ out, long long count) {
+    constexpr int kUnroll = kUnrollOf<ACT>;
     const long long first = ((long long)blockIdx.x * kUnroll * kThreads + threadIdx.x) * V;
     unsigned w[kUnroll][(V + 3) / 4];
     int s[kUnroll];
@@ -195,9 +198,9 @@ __global__ void __launch_bounds__(kThreads) restore_kernel(const unsigned char* 
     }
 }
 
-template <int V>
+template <int V, int ACT>
 inline int grid_for(long long count, unsigned* grid) {
-    const long long per = (long long)kThreads * kUnroll * V, blocks = (count + per - 1) / per;
+    const long long per = (long long)kThreads * kUnrollOf<ACT> * V, blocks = (count + per - 1) / per;
     if (blocks > 0x7fffffffLL) return fail(CNL_ERR_BAD_SHAPE, "count %lld is too large", count);
     *grid = (unsigned)blocks;
     return CNL_OK;
@@ -209,10 +212,10 @@ int run_store(const void* x, void* y, unsigned char* codes, unsigned char* scale
     unsigned grid = 0;
     // one element a lane where a pointer is not aligned (a view that starts at an odd element)
     if (aligned16(x) && aligned16(y) && aligned16(codes)) {
-        CNL_TRY(grid_for<V>(count, &grid));
+        CNL_TRY((grid_for<V, ACT>(count, &grid)));
         store_kernel<T, V, FMT, ACT><<<grid, kThreads, 0, st>>>((const T*)x, (T*)y, codes, scales, count);
     } else {
-        CNL_TRY(grid_for<1>(count, &grid));
+        CNL_TRY((grid_for<1, ACT>(count, &grid)));
         store_kernel<T, 1, FMT, ACT><<<grid, kThreads, 0, st>>>((const T*)x, (T*)y, codes, scales, count);
     }
     return after_launch("ckpt8 store");
@@ -223,10 +226,10 @@ int run_restore(const unsigned char* codes, const unsigned char* scales, const v
     constexpr int V = 16 / (int)sizeof(T);
     unsigned grid = 0;
     if (aligned16(g) && aligned16(out) && aligned16(codes)) {
-        CNL_TRY(grid_for<V>(count, &grid));
+        CNL_TRY((grid_for<V, ACT>(count, &grid)));
         restore_kernel<T, V, FMT, ACT><<<grid, kThreads, 0, st>>>(codes, scales, (const T*)g, (T*)out, count);
     } else {
-        CNL_TRY(grid_for<1>(count, &grid));
+        CNL_TRY((grid_for<1, ACT>(count, &grid)));
         restore_kernel<T, 1, FMT, ACT><<<grid, kThreads, 0, st>>>(codes, scales, (const T*)g, (T*)out, count);
     }
     return after_launch("ckpt8 restore");
