@@ -317,12 +317,12 @@ extern "C" int cnl_linattn_forward(const void* q, const void* k, const void* v, 
     const Rows Q = {q, s[0], s[1], s[2]}, Kk = {k, s[3], s[4], s[5]}, V = {v, s[6], s[7], s[8]};
     Sweep w = {};
     w.log_decay = log_decay; w.lengths = lengths; w.batch = b; w.t = t; w.h = h; w.segments = segments; w.seg = seg;
-    w.b = Kk; w.c = V; w.da = dk; w.dc = dv; w.off = 1; w.in_scale = 1.0f; w.out_scale = scale;
+    w.b = Kk; w.c = V; w.da = dk; w.dc = dv; w.off = 1; w.in_scale = 1.0f; w.out_scale = scale; w.exact = state_out != nullptr;
     if (segments > 1) {
         w.end = starts;
         CNL_TRY(run_sweep(w, dtype, st));
         CNL_TRY(run_scan(starts, state, state_out, log_decay, lengths, b, t, h, dk * dv, segments, seg, st));
-        w.start = starts; w.end = nullptr;
+        w.start = starts; w.end = nullptr; w.exact = 0;
     } else {
         w.start = state; w.end = state_out;
     }
@@ -351,18 +351,18 @@ extern "C" int cnl_linattn_backward(const void* q, const void* k, const void* v,
     CNL_TRY(run_sweep(w, dtype, st));
     // the reversed sweeps: W = sum of scale l^.. q do^T
     w.off = 0; w.reversed = 1; w.in_scale = scale; w.out_scale = 1.0f;
-    w.b = Q; w.c = G; w.da = dk; w.dc = dv; w.transposed = 0; w.start = nullptr; w.out = nullptr;
+    w.b = Q; w.c = G; w.da = dk; w.dc = dv; w.transposed = 0; w.start = nullptr; w.out = nullptr; w.exact = g_state != nullptr;
     if (segments > 1) {
         w.end = scratch;
         CNL_TRY(run_sweep(w, dtype, st));
         CNL_TRY(run_scan(scratch, g_state_out, g_state, log_decay, lengths, b, t, h, dk * dv, segments, seg, st));
-        w.start = scratch; w.end = nullptr;
+        w.start = scratch; w.end = nullptr; w.exact = 0;
     } else {
         w.start = g_state_out; w.end = g_state;
     }
     w.a = Kk; w.out = g_v;
     CNL_TRY(run_sweep(w, dtype, st));
-    w.end = nullptr;
+    w.end = nullptr; w.exact = 0;
     w.a = V; w.b = G; w.c = Q; w.da = dv; w.dc = dk; w.transposed = 1; w.out = g_k;
     return run_sweep(w, dtype, st);
 }

@@ -33,6 +33,7 @@ struct Sweep {
     int reversed, off;
     int transposed;                  // `start` is stored [dc][da]
     float in_scale, out_scale;
+    int exact;                       // W at the end is a result, not only what later outputs are rounded from
 };
 
 __device__ __forceinline__ float clamp_log(float a) { return a < -1e30f ? -1e30f : a; }   // l = 0 keeps l^0 = 1; NaN stays

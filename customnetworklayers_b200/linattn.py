@@ -67,8 +67,9 @@ def forward(q, k, v, log_decay, state=None, lengths=None, scale: Optional[float]
     return out, end, starts
 
 
-def backward(grad_out, grad_state, q, k, v, log_decay, state, lengths, starts, scale: Optional[float] = None):
-    """(g_q, g_k, g_v, g_state) from the gradients of the output and of the end state (the latter may be None)."""
+def backward(grad_out, grad_state, q, k, v, log_decay, state, lengths, starts, scale: Optional[float] = None, want_state: bool = True):
+    """(g_q, g_k, g_v, g_state) from the gradients of the output and of the end state (the latter may be None); g_state, the
+    gradient of the carried state, is None unless wanted."""
     _check(q, k, v, log_decay, state, lengths, 4)
     b, t, h, dk = q.shape
     dv = v.shape[-1]
@@ -80,11 +81,11 @@ def backward(grad_out, grad_state, q, k, v, log_decay, state, lengths, starts, s
         check_tensor(grad_state, "grad_state", torch.float32, q.device, (b, h, dk, dv))
     new = lambda *s, dtype=q.dtype: torch.empty(s, dtype=dtype, device=q.device)  # noqa: E731
     g_q, g_k, g_v = new(b, t, h, dk), new(b, t, h, dk), new(b, t, h, dv)
-    g_state = new(b, h, dk, dv, dtype=torch.float32)
+    g_state = new(b, h, dk, dv, dtype=torch.float32) if want_state else None
     scratch = None if starts is None else torch.empty_like(starts)
     launch("linear attention backward", _lib.load().cnl_linattn_backward, q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(),
            grad_out.data_ptr(), _strides(q, k, v, grad_out), log_decay.data_ptr(), ptr(lengths), ptr(state), ptr(starts),
-           ptr(grad_state), g_q.data_ptr(), g_k.data_ptr(), g_v.data_ptr(), g_state.data_ptr(), ptr(scratch), b, t, h, dk, dv, scale,
+           ptr(grad_state), g_q.data_ptr(), g_k.data_ptr(), g_v.data_ptr(), ptr(g_state), ptr(scratch), b, t, h, dk, dv, scale,
            DTYPES[q.dtype])
     return g_q, g_k, g_v, g_state
 
@@ -114,8 +115,9 @@ class LinearAttentionFunction(Function):
         if grad_out is None:
             grad_out = torch.zeros((*q.shape[:-1], v.shape[-1]), dtype=q.dtype, device=q.device)
         grad_state = None if grad_state is None else grad_state.contiguous()
-        g_q, g_k, g_v, g_state = backward(_rows(grad_out), grad_state, q, k, v, log_decay, state, lengths, starts, ctx.scale)
-        return g_q, g_k, g_v, None, g_state if state is not None else None, None, None
+        g_q, g_k, g_v, g_state = backward(_rows(grad_out), grad_state, q, k, v, log_decay, state, lengths, starts, ctx.scale,
+                                          ctx.needs_input_grad[4])
+        return g_q, g_k, g_v, None, g_state, None, None
 
 
 def linear_attention(q, k, v, log_decay, *, state=None, lengths=None, scale: Optional[float] = None):
