@@ -155,7 +155,8 @@ int launch_sweep(const Sweep& s, cudaStream_t st) {
 }
 
 int run_sweep(const Sweep& s, int dtype, cudaStream_t st) {
-    return dtype == CNL_F32 ? launch_sweep<float>(s, st) : run_sweep_mma(s, dtype, st);
+    if (dtype == CNL_F32) return launch_sweep<float>(s, st);
+    return tc_serves(s, dtype) ? run_sweep_tc(s, st) : run_sweep_mma(s, dtype, st);
 }
 
 // ---- scan over the segments -------------------------------------------------------------------------------------

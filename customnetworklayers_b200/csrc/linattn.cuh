@@ -42,7 +42,9 @@ __device__ __forceinline__ float clamp_log(float a) { return a < -1e30f ? -1e30f
 __device__ __forceinline__ float power(float a, int n) { return expf(a * (float)n); }
 
 int run_sweep(const Sweep& s, int dtype, cudaStream_t st);          // dispatches to the kernel that serves the type and sizes
-int run_sweep_mma(const Sweep& s, int dtype, cudaStream_t st);      // fp16, bf16: tensor cores
+int run_sweep_mma(const Sweep& s, int dtype, cudaStream_t st);      // fp16, bf16: mma.sync
+bool tc_serves(const Sweep& s, int dtype);                          // bf16 rows that TMA can take, 128 tokens or more
+int run_sweep_tc(const Sweep& s, cudaStream_t st);                  // ... on the fifth-generation tensor cores
 
 }  // namespace lin
 }  // namespace cnl

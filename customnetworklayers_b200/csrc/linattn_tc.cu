@@ -1,0 +1,522 @@
+// Linear attention sweep for bf16 on the fifth-generation tensor cores (formulas: linattn.cuh).
+//
+// A block of ten warps walks one segment of one head in chunks of 128 tokens.  One warp brings a, b, c rows by TMA (128-byte
+// swizzle), one thread issues the products, eight warps do what lies between.  Per chunk, accumulators in tensor memory:
+//     P = a b^T                 [128 tokens x 128 tokens]   -> weighted, masked, rounded, written back as an operand
+//     X = a W                   [128 tokens x dc]           W as the sweep has it before the chunk
+//     O = P c                   [128 tokens x dc]
+//     T = (weighted c)^T b      [dc x da]                   what the chunk adds to W^T
+// and in registers W^T <- l^m W^T + T (fp32), out = l^{pos + off} X + O.  Nothing of the recurrence passes through the tensor
+// cores: T needs only the chunk's own rows, so the products of a chunk run while the warps finish the one before.
+// Reversed sweeps take the tokens of a chunk in their order in memory and turn the mask and the weights around instead.
+//
+// Operands: a and b for P, P, and W lie with the summed dimension contiguous; c and the weighted c, and b for T, with it
+// strided (their rows are tokens), which the descriptors say.  Heads of up to 64 fill 128 rows of T with the two parts of
+// the weighted c (first part: rows 0..63, what it leaves out: rows 64..127), so the state is kept as two addends and both
+// meet a in X; heads of up to 128 add the parts in T.  Roundings: as in the mma.sync kernel (P once, W once, the weighted c
+// to 16 or, where the state is a result, 24 bits).
+//
+// Every wait is bounded: a block that gives up marks the status word, fills what it owes with NaN, and returns after its
+// copies and products have ended.
+#include <cuda.h>
+
+#include "linattn.cuh"
+
+namespace cnl {
+namespace lin {
+
+__device__ int g_gave_up = 0;
+
+constexpr int kTok = 128;                       // tokens of a chunk
+constexpr int kBlk = kTok * 128;                // bytes of 128 rows of 64 elements
+constexpr int kWorkers = 8;                     // warps between the products
+constexpr int kTcThreads = (kWorkers + 2) * 32;
+constexpr int kSpins = 1 << 22;
+
+// ---- the machine's words ------------------------------------------------------------------------------------------
+__device__ __forceinline__ unsigned smem_at(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(unsigned bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
+__device__ __forceinline__ void bar_arrive(unsigned bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void bar_expect(unsigned bar, int bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
+__device__ __forceinline__ bool bar_try(unsigned bar, unsigned parity) {
+    unsigned ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// true when the phase has ended; false when it did not within the limit or another warp has given up
+__device__ __forceinline__ bool bar_wait(unsigned bar, unsigned parity, volatile int* dead) {
+    for (int i = 0; i < kSpins; ++i) {
+        if (bar_try(bar, parity)) return true;
+        if ((i & 255) == 255 && *dead) return false;
+    }
+    *dead = 1;
+    return false;
+}
+__device__ __forceinline__ void tma_load(unsigned to, const CUtensorMap* map, int x, int h, int t, int b, unsigned bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to), "l"(map), "r"(x), "r"(h), "r"(t), "r"(b), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(unsigned bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void tc_mma(unsigned d, unsigned long long a, unsigned long long b, unsigned what, bool add) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(what), "r"((unsigned)add) : "memory");
+}
+__device__ __forceinline__ void tc_load(unsigned at, float (&v)[32]) {
+    unsigned r[32];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+                   "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+                   "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(at));
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tc_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// Descriptor of an operand in shared memory, 128-byte swizzle.  Summed dimension contiguous: `step` is the distance of
+// groups of 8 rows.  Summed dimension strided: `step` that of groups of 8 summed rows, `block` that of 64-element columns.
+__device__ __forceinline__ unsigned long long operand(unsigned at, unsigned block, unsigned step) {
+    return (unsigned long long)((at & 0x3ffffu) >> 4) | (unsigned long long)(block >> 4) << 16 | (unsigned long long)(step >> 4) << 32 | 1ULL << 46 | 2ULL << 61;
+}
+// Instruction word: fp32 sums of bf16 products, 128 rows, n columns; strided a / b
+__host__ __device__ constexpr unsigned product(int n, int strided_a, int strided_b) {
+    return 1u << 4 | 1u << 7 | 1u << 10 | (unsigned)strided_a << 15 | (unsigned)strided_b << 16 | (unsigned)(n >> 3) << 17 | 8u << 24;
+}
+
+template <int D, bool OUT, int PARTS>
+struct Map {                                    // shared memory in bytes from a 1024-byte boundary
+    static constexpr int nb = D / 64;
+    static constexpr int stages = D == 64 || !OUT ? 2 : 1;
+    static constexpr int a = 0, b = OUT ? nb * kBlk : 0, c = b + nb * kBlk, stage = c + nb * kBlk;
+    static constexpr int p = stages * stage, w = p + (OUT ? 2 * kBlk : 0);
+    static constexpr int parts = w + (OUT ? (D == 128 ? 2 * kBlk : kBlk) : 0);
+    static constexpr int part_blocks = D == 128 ? 2 * PARTS : PARTS == 3 ? 4 : 2;
+    static constexpr int bars = parts + part_blocks * kBlk;
+    static constexpr int bytes = bars + 256 + 1024;              // and the way to the boundary
+};
+
+// ---- the sweep -----------------------------------------------------------------------------------------------------
+template <int D, bool OUT, int PARTS>
+__global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                                                           const __grid_constant__ CUtensorMap map_c) {
+    using M = Map<D, OUT, PARTS>;
+    constexpr int NB = M::nb, S = M::stages;
+    extern __shared__ unsigned char raw[];
+    unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<size_t>(raw) + 1023) & ~(size_t)1023);
+    const unsigned base = smem_at(sm), bars = base + M::bars;
+    volatile int* dead = reinterpret_cast<volatile int*>(sm + M::bars + 240);
+    unsigned* tmem_word = reinterpret_cast<unsigned*>(sm + M::bars + 244);
+    // barriers, one of each for every stage
+    enum { FULL_A, FULL_B, FULL_C, DONE_P, DONE_X, DONE_T, DONE_O, HAS_C, HAS_P, HAS_W, HAS_O, KINDS };
+    auto bar = [&](int kind, int stage) { return bars + (unsigned)(kind * S + stage) * 8; };
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int seg = blockIdx.x % s.segments, bh = blockIdx.x / s.segments, head = bh % s.h, bat = bh / s.h;
+    const int n = s.lengths ? min(max(s.lengths[bat], 0), s.t) : s.t;
+    const long long first = (long long)seg * s.seg;
+    const int lo = (int)(first < n ? first : n), hi = (int)(first + s.seg < n ? first + s.seg : n);
+    const int chunks = (hi - lo + kTok - 1) / kTok;
+    const int da = s.da, dc = s.dc;
+    const long long size = (long long)da * dc;
+    // first token of chunk i; positions lo + 128 i ... of the sweep
+    auto token0 = [&](int i) { return s.reversed ? n - (lo + i * kTok) - kTok : lo + i * kTok; };
+
+    if (tid == 0) {
+        *dead = 0;
+        for (int i = 0; i < S; ++i) {
+            for (int k = FULL_A; k <= DONE_O; ++k) bar_init(bar(k, i), 1);
+            for (int k = HAS_C; k <= HAS_O; ++k) bar_init(bar(k, i), kWorkers);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kWorkers + 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_at(tmem_word)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tc_before();
+    }
+    __syncthreads();
+    tc_after();
+    const unsigned tmem = *tmem_word, tP = tmem, tX = tmem + 128, tO = tmem + 256, tT = tmem + 384;
+
+    if (warp == kWorkers) {
+        // ---- rows arrive
+        if (lane == 0) {
+            int i = 0;
+            for (; i < chunks; ++i) {
+                const int st = i % S, t0 = token0(i);
+                const unsigned at = base + st * M::stage;
+                const unsigned before = (unsigned)((i / S) - 1) & 1u;
+                auto take = [&](int full, int done, const CUtensorMap* map, const Rows& r, int offset) {
+                    if (i >= S && !bar_wait(bar(done, st), before, dead)) return false;
+                    bar_expect(bar(full, st), NB * kBlk);
+                    for (int x = 0; x < NB; ++x) tma_load(at + offset + x * kBlk, map, x * 64, r.sh ? head : 0, t0, r.sb ? bat : 0, bar(full, st));
+                    return true;
+                };
+                if (OUT && !take(FULL_A, DONE_X, &map_a, s.a, M::a)) break;
+                if (!take(FULL_B, DONE_T, &map_b, s.b, M::b)) break;
+                if (!take(FULL_C, OUT ? DONE_O : DONE_T, &map_c, s.c, M::c)) break;
+            }
+            if (*dead) {                                         // what was asked for has to land before the block leaves
+                int never = 0;
+                for (int j = max(0, i - S); j <= min(i, chunks - 1); ++j)
+                    for (int k = OUT ? FULL_A : FULL_B; k <= FULL_C; ++k)
+                        for (int spin = 0; spin < 4096 && !bar_try(bar(k, j % S), (unsigned)(j / S) & 1u); ++spin) ++never;
+                (void)never;
+            }
+        }
+        __syncwarp();
+    } else if (warp == kWorkers + 1) {
+        // ---- products
+        if (lane == 0) {
+            for (int i = 0; i < chunks; ++i) {
+                const int st = i % S;
+                const unsigned ph = (unsigned)(i / S) & 1u, at = base + st * M::stage;
+                const bool cut = hi - lo - i * kTok < kTok && !s.reversed;       // rows behind the end are cleared first
+                const unsigned A = at + M::a, B = at + M::b, C = at + M::c, P = base + M::p, W = base + M::w, Q = base + M::parts;
+                if constexpr (OUT) {
+                    if (!bar_wait(bar(FULL_A, st), ph, dead) || !bar_wait(bar(FULL_B, st), ph, dead)) break;
+                    if (cut && !bar_wait(bar(HAS_C, st), ph, dead)) break;
+                    tc_after();
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        const unsigned o = (k / 4) * kBlk + (k % 4) * 32;
+                        tc_mma(tP, operand(A + o, 16, 1024), operand(B + o, 16, 1024), product(128, 0, 0), k > 0);
+                    }
+                    tc_commit(bar(DONE_P, st));
+                    if (!bar_wait(bar(HAS_W, st), ph, dead)) break;
+                    if (i > 0 && !bar_wait(bar(HAS_O, (i - 1) % S), (unsigned)((i - 1) / S) & 1u, dead)) break;
+                    tc_after();
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        const unsigned o = (k / 4) * kBlk + (k % 4) * 32;
+                        tc_mma(tX, operand(A + o, 16, 1024), operand(W + o, 16, 1024), product(D, 0, 0), k > 0);
+                    }
+                    if constexpr (D == 64) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) tc_mma(tX, operand(A + k * 32, 16, 1024), operand(W + kBlk / 2 + k * 32, 16, 1024), product(D, 0, 0), true);
+                    }
+                    tc_commit(bar(DONE_X, st));
+                } else {
+                    if (!bar_wait(bar(FULL_B, st), ph, dead)) break;
+                    if (i > 0 && !bar_wait(bar(HAS_W, (i - 1) % S), (unsigned)((i - 1) / S) & 1u, dead)) break;       // T has been read
+                }
+                if (!bar_wait(bar(HAS_C, st), ph, dead)) break;
+                tc_after();
+                // small parts first
+                if constexpr (D == 128) {
+#pragma unroll
+                    for (int p = PARTS - 1; p >= 0; --p)
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            tc_mma(tT, operand(Q + p * 2 * kBlk + k * 2048, kBlk, 1024), operand(B + k * 2048, kBlk, 1024), product(128, 1, 1), p < PARTS - 1 || k > 0);
+                } else {
+#pragma unroll
+                    for (int p = PARTS == 3 ? 1 : 0; p >= 0; --p)
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            tc_mma(tT, operand(Q + p * 2 * kBlk + k * 2048, kBlk, 1024), operand(B + k * 2048, kBlk, 1024), product(64, 1, 1), p < (PARTS == 3 ? 1 : 0) || k > 0);
+                }
+                tc_commit(bar(DONE_T, st));
+                if constexpr (OUT) {
+                    if (!bar_wait(bar(HAS_P, st), ph, dead)) break;
+                    tc_after();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        tc_mma(tO, operand(P + (k / 4) * kBlk + (k % 4) * 32, 16, 1024), operand(C + k * 2048, kBlk, 1024), product(D, 0, 1), k > 0);
+                    tc_commit(bar(DONE_O, st));
+                }
+            }
+            if (*dead) {                                         // products under way end before the tensor memory goes
+                tc_commit(bar(DONE_P, 0));
+                for (int spin = 0; spin < 4096; ++spin)
+                    if (bar_try(bar(DONE_P, 0), 0) && bar_try(bar(DONE_P, 0), 1)) break;
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- between the products: warp w holds lanes 32 (w mod 4) .. of tensor memory and one half of the columns
+        constexpr int HC = D / 2;                                // columns of X, O and T that a thread holds
+        const int q = warp & 3, half = warp >> 2, row = q * 32 + lane;
+        const unsigned lanes = (unsigned)(q * 32) << 16;
+        const float ld = clamp_log(s.log_decay[head]), a2 = ld * 1.4426950408889634f, both = s.in_scale * s.out_scale;
+        const float keep_full = power(ld, kTok);
+        const int pos = s.reversed ? kTok - 1 - row : row;
+        const float far = s.out_scale * power(ld, pos + s.off);
+        // weights of the token rows of this thread's pieces: rows tid / 8 + 32 k of 128-byte rows
+        const int prow = tid >> 3;
+        float wt[4];
+        auto weigh = [&](int m) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int r = prow + 32 * k, j = s.reversed ? kTok - 1 - r : r;
+                wt[k] = j < m ? power(ld, m - s.off - j) * s.in_scale : 0.0f;
+            }
+        };
+        weigh(kTok);
+        // W^T: D = 128: row = column of c, 64 columns from 64 half; D = 64: rows 0..63 first addend, 64..127 second
+        const int wrow = D == 128 ? row : row & 63, wcol = half * HC;
+        float w[HC];
+        {
+            const float* w0 = s.start ? s.start + ((long long)bh * s.segments + seg) * size : nullptr;
+            const bool has = w0 && wrow < dc && (D == 128 || row < 64);
+#pragma unroll
+            for (int x = 0; x < HC; ++x) {
+                const int i = wcol + x;
+                w[x] = has && i < da ? (s.transposed ? w0[(long long)wrow * da + i] : w0[(long long)i * dc + wrow]) : 0.0f;
+            }
+        }
+        auto put_row = [&](unsigned char* tile, int r, int first_piece, const float* v, int pieces) {       // 16-byte pieces of a swizzled 128-byte row
+            for (int x = 0; x < pieces; ++x)
+                *reinterpret_cast<uint4*>(tile + r * 128 + (((first_piece + x) ^ (r & 7)) << 4)) =
+                    make_uint4(pack2<__nv_bfloat16>(v[8 * x], v[8 * x + 1]), pack2<__nv_bfloat16>(v[8 * x + 2], v[8 * x + 3]), pack2<__nv_bfloat16>(v[8 * x + 4], v[8 * x + 5]), pack2<__nv_bfloat16>(v[8 * x + 6], v[8 * x + 7]));
+        };
+        auto tell = [&](int kind, int stage) {
+            tc_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(bar(kind, stage));
+        };
+        auto put_w = [&](int i) {                                // W as the operand of chunk i
+            if constexpr (OUT) {
+                unsigned char* W = sm + M::w;
+#pragma unroll
+                for (int x = 0; x < HC / 8; ++x) {
+                    const float* v = w + 8 * x;
+                    if constexpr (D == 128) put_row(W + half * kBlk, wrow, x, v, 1);
+                    else put_row(W + (row >> 6) * (kBlk / 2), wrow, half * 4 + x, v, 1);
+                }
+                fence_async();
+            }
+            tell(HAS_W, i % S);
+        };
+        if constexpr (PARTS == 3 && D == 64) {                   // the rows that stand beside the third part
+            for (int x = tid; x < kBlk / 16; x += kWorkers * 32) reinterpret_cast<uint4*>(sm + M::parts + 3 * kBlk)[x] = make_uint4(0, 0, 0, 0);
+            fence_async();
+        }
+        if (OUT && chunks > 0) put_w(0);
+
+        for (int i = 0; i < chunks; ++i) {
+            const int st = i % S;
+            const unsigned ph = (unsigned)(i / S) & 1u;
+            const int left = hi - lo - i * kTok, m = left < kTok ? left : kTok;
+            unsigned char* at = sm + st * M::stage;
+            // the weighted c in parts
+            if (!bar_wait(bar(FULL_C, st), ph, dead)) break;
+            const bool cut = m < kTok && !s.reversed;
+            if (m < kTok) weigh(m);
+            if (cut && (!bar_wait(bar(FULL_B, st), ph, dead) || (OUT && !bar_wait(bar(FULL_A, st), ph, dead)))) break;
+#pragma unroll
+            for (int x = 0; x < NB; ++x)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int off = x * kBlk + (tid + 256 * k) * 16;
+                    uint4 v = *reinterpret_cast<const uint4*>(at + M::c + off);
+                    if (cut && prow + 32 * k >= m) {             // rows behind the end: nothing, whatever they hold
+                        v = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4*>(at + M::c + off) = v;
+                        *reinterpret_cast<uint4*>(at + M::b + off) = v;
+                        if (OUT) *reinterpret_cast<uint4*>(at + M::a + off) = v;
+                    }
+                    unsigned in[4] = {v.x, v.y, v.z, v.w}, part[PARTS][4];
+                    const float2 f = make_float2(wt[k], wt[k]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float2 y = __fmul2_rn(unpack2(in[e], __nv_bfloat16()), f);
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p) {
+                            part[p][e] = pack2<__nv_bfloat16>(y.x, y.y);
+                            const float2 z = unpack2(part[p][e], __nv_bfloat16());
+                            y = __fadd2_rn(y, make_float2(-z.x, -z.y));
+                        }
+                    }
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p)
+                        *reinterpret_cast<uint4*>(sm + M::parts + p * NB * kBlk + off) = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
+                }
+            fence_async();
+            tell(HAS_C, st);
+            if constexpr (OUT) {
+                // P: weights and mask
+                if (!bar_wait(bar(DONE_P, st), ph, dead)) break;
+                tc_after();
+                const int d0 = s.reversed ? half * 64 - row : row - half * 64;          // positions from column 64 half to this row
+                const bool none = s.reversed ? (q >= 2 && half == 0) : (q < 2 && half == 1);   // all above the diagonal
+                unsigned char* to = sm + M::p + half * kBlk;
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    float v[32];
+                    if (none) {
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) v[x] = 0.0f;
+                    } else {
+                        tc_load(tP + lanes + half * 64 + y * 32, v);
+                        tc_wait_load();
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) {
+                            const int d = s.reversed ? d0 + y * 32 + x : d0 - y * 32 - x;
+                            const float f = exp2_approx(a2 * (float)d) * both;
+                            v[x] = d >= 0 ? v[x] * f : 0.0f;
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) put_row(to, row, y * 4 + x, v + 8 * x, 1);
+                }
+                fence_async();
+                tell(HAS_P, st);
+            }
+            // W^T <- l^m W^T + T
+            if (!bar_wait(bar(DONE_T, st), ph, dead)) break;
+            tc_after();
+            const float keep = m < kTok ? power(ld, m) : keep_full;
+#pragma unroll
+            for (int y = 0; y < HC / 32; ++y) {
+                float v[32];
+                tc_load(tT + lanes + wcol + y * 32, v);
+                tc_wait_load();
+#pragma unroll
+                for (int x = 0; x < 32; ++x) w[y * 32 + x] = fmaf(keep, w[y * 32 + x], v[x]);
+            }
+            if constexpr (OUT) {
+                if (!bar_wait(bar(DONE_X, st), ph, dead)) break;
+            }
+            if (i + 1 < chunks) {
+                if constexpr (OUT) put_w(i + 1);
+                else tell(HAS_W, st);
+            }
+            if constexpr (OUT) {
+                // out = l^{pos + off} X + O
+                if (!bar_wait(bar(DONE_O, st), ph, dead)) break;
+                tc_after();
+                const bool live = pos < m;
+                const long long tok = token0(i) + row;
+                __nv_bfloat16* out = (__nv_bfloat16*)s.out + (((long long)bat * s.t + tok) * s.h + head) * dc + wcol;
+#pragma unroll
+                for (int y = 0; y < HC / 32; ++y) {
+                    float x1[32], x2[32];
+                    tc_load(tX + lanes + wcol + y * 32, x1);
+                    tc_load(tO + lanes + wcol + y * 32, x2);
+                    tc_wait_load();
+                    if (y == HC / 32 - 1) tell(HAS_O, st);
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) x1[x] = fmaf(far, x1[x], x2[x]);
+                    if (live) {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            if (wcol + y * 32 + x * 8 < dc)
+                                *reinterpret_cast<uint4*>(out + y * 32 + x * 8) =
+                                    make_uint4(pack2<__nv_bfloat16>(x1[8 * x], x1[8 * x + 1]), pack2<__nv_bfloat16>(x1[8 * x + 2], x1[8 * x + 3]), pack2<__nv_bfloat16>(x1[8 * x + 4], x1[8 * x + 5]), pack2<__nv_bfloat16>(x1[8 * x + 6], x1[8 * x + 7]));
+                    }
+                }
+            }
+        }
+        if (s.end) {
+            float* w1 = s.end + ((long long)bh * s.segments + seg) * size;
+            if constexpr (D == 64) {                             // the two addends meet in shared memory (the parts' room)
+                asm volatile("bar.sync 1, %0;" ::"n"(kWorkers * 32) : "memory");
+                float* meet = reinterpret_cast<float*>(sm + M::parts);
+                if (row >= 64)
+#pragma unroll
+                    for (int x = 0; x < HC; ++x) meet[(wcol + x) * 64 + wrow] = w[x];
+                asm volatile("bar.sync 1, %0;" ::"n"(kWorkers * 32) : "memory");
+                if (row < 64)
+#pragma unroll
+                    for (int x = 0; x < HC; ++x) w[x] += meet[(wcol + x) * 64 + wrow];
+            }
+            if (wrow < dc && (D == 128 || row < 64))
+#pragma unroll
+                for (int x = 0; x < HC; ++x)
+                    if (wcol + x < da) w1[(long long)(wcol + x) * dc + wrow] = *dead ? __uint_as_float(0x7fffffffu) : w[x];
+        }
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    if (warp == kWorkers + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    const bool lost = *dead != 0;
+    if (lost && tid == 0) g_gave_up = 1;
+    if constexpr (OUT) {                                         // rows behind the sequence's end; all rows of a block that gave up
+        const long long zlo = lost ? lo : (first > n ? first : n), zhi = first + s.seg < s.t ? first + s.seg : s.t;
+        for (long long e = zlo * dc + tid; e < zhi * dc; e += kTcThreads) {
+            const long long i = e / dc, tok = i < n && s.reversed ? n - 1 - i : i;
+            ((__nv_bfloat16*)s.out)[(((long long)bat * s.t + tok) * s.h + head) * dc + (e - i * dc)] = from_f32<__nv_bfloat16>(i < n ? __uint_as_float(0x7fffffffu) : 0.0f);
+        }
+    }
+}
+
+// ---- launch --------------------------------------------------------------------------------------------------------
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                            CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+int encoder(Encode* out) {
+    static Encode fn = nullptr;
+    if (!fn) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        CNL_TRY(check_cuda(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found), "cudaGetDriverEntryPoint"));
+        if (!p || found != cudaDriverEntryPointSuccess) return fail(CNL_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+        fn = reinterpret_cast<Encode>(p);
+    }
+    *out = fn;
+    return CNL_OK;
+}
+
+// [b][t][h][d] in boxes of 64 elements x 128 tokens of one head; what lies outside reads as 0.  A head or batch stride of 0
+// (rows shared by all heads or sequences) is a dimension of one element, whose coordinate stays 0.
+int encode(CUtensorMap* map, const Rows& r, int b, int t, int h, int d) {
+    Encode fn = nullptr;
+    CNL_TRY(encoder(&fn));
+    if (r.sh == 0) h = 1;
+    if (r.sb == 0) b = 1;
+    const long long some = 16;                                   // the stride of a dimension of one element is not used
+    const cuuint64_t sizes[4] = {(cuuint64_t)d, (cuuint64_t)h, (cuuint64_t)t, (cuuint64_t)b};
+    const cuuint64_t strides[3] = {(cuuint64_t)(h > 1 ? 2 * r.sh : some), (cuuint64_t)(t > 1 ? 2 * r.st : some), (cuuint64_t)(b > 1 ? 2 * r.sb : some)};
+    const cuuint32_t box[4] = {64, 1, (cuuint32_t)kTok, 1}, ones[4] = {1, 1, 1, 1};
+    const CUresult e = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(r.p), sizes, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (e != CUDA_SUCCESS) return fail(CNL_ERR_CUDA, "cuTensorMapEncodeTiled: error %d", (int)e);
+    return CNL_OK;
+}
+
+template <int D, bool OUT, int PARTS>
+int launch_tc(const Sweep& s, cudaStream_t st) {
+    CUtensorMap a = {}, b, c;
+    if (OUT) CNL_TRY(encode(&a, s.a, s.batch, s.t, s.h, s.da));
+    CNL_TRY(encode(&b, s.b, s.batch, s.t, s.h, s.da));
+    CNL_TRY(encode(&c, s.c, s.batch, s.t, s.h, s.dc));
+    constexpr int bytes = Map<D, OUT, PARTS>::bytes;
+    static_assert(bytes <= 232448, "more shared memory than a block may have");
+    CNL_TRY(ensure_dynamic_smem(tc_kernel<D, OUT, PARTS>, bytes));
+    tc_kernel<D, OUT, PARTS><<<(unsigned)((long long)s.batch * s.h * s.segments), kTcThreads, bytes, st>>>(s, a, b, c);
+    return after_launch("linear attention sweep");
+}
+
+template <int D>
+int run_tc(Sweep s, cudaStream_t st) {
+    if (s.end) {                                                 // the state on its own, then the outputs
+        Sweep only = s;
+        only.out = nullptr;
+        CNL_TRY(s.exact ? (launch_tc<D, false, 3>(only, st)) : (launch_tc<D, false, 2>(only, st)));
+        if (!s.out) return CNL_OK;
+        s.end = nullptr;
+    }
+    return launch_tc<D, true, 2>(s, st);
+}
+
+bool tc_serves(const Sweep& s, int dtype) {
+    auto fits = [&](const Rows& r, int d) {
+        auto ok = [](long long n, long long stride) { return n <= 1 || (stride >= 0 && stride % 8 == 0 && stride < (1LL << 38)); };
+        return !r.p || (aligned16(r.p) && d % 8 == 0 && ok(s.h, r.sh) && ok(s.t, r.st) && r.st > 0 && ok(s.batch, r.sb));
+    };
+    return dtype == CNL_BF16 && s.t >= kTok && s.da > 32 && s.dc > 32 && fits(s.a, s.da) && fits(s.b, s.da) && fits(s.c, s.dc) && aligned16(s.out);
+}
+
+int run_sweep_tc(const Sweep& s, cudaStream_t st) { return s.da <= 64 && s.dc <= 64 ? run_tc<64>(s, st) : run_tc<128>(s, st); }
+
+}  // namespace lin
+}  // namespace cnl
+
+extern "C" int cnl_linattn_status(void) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, cnl::lin::g_gave_up, sizeof(int)) != cudaSuccess) { cudaGetLastError(); return -1; }
+    return v;
+}
