@@ -53,7 +53,7 @@ SIGNATURES = {
     "cnl_blocknorm_scratch_bytes": (c_longlong, [c_longlong, c_int, c_longlong]),
     "cnl_blocknorm_forward": (c_int, [c_void_p] * 13 + [c_longlong, c_int, c_longlong] + [c_int] * 3 + [c_float] + [c_int] * 3 + [c_void_p]),
     "cnl_blocknorm_backward": (c_int, [c_void_p] * 22 + [c_longlong, c_int, c_longlong] + [c_int] * 6 + [c_void_p]),
-    "cnl_linattn_segments": (c_int, [c_int] * 3),
+    "cnl_linattn_segments": (c_int, [c_int] * 6),
     "cnl_linattn_status": (c_int, []),
     "cnl_linattn_forward": (c_int, [c_void_p] * 10 + [c_int] * 5 + [c_float, c_int, c_void_p]),
     "cnl_linattn_backward": (c_int, [c_void_p] * 15 + [c_int] * 5 + [c_float, c_int, c_void_p]),

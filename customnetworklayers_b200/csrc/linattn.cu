@@ -274,20 +274,31 @@ int check(int b, int t, int h, int dk, int dv, int dtype) {
     return check_dtype(dtype);
 }
 
-// Segments of a sequence: enough blocks for two an SM, but none shorter than 256 positions (a segment costs a round trip of
-// its state, dk x dv floats, through memory).
-int segment_plan(int b, int t, int h, int* segments, int* seg) {
+// Segments of a sequence.  All blocks take about the same time, so a launch lasts as many rounds as it has blocks for one
+// place: the segment count with the fewest rounds times positions wins, a segment counting `kExtra` positions more for its
+// state's way through memory.
+int segment_plan(int b, int t, int h, int dk, int dv, int dtype, int* segments, int* seg) {
+    constexpr int kExtra = 128;
     int sms = 0;
     CNL_TRY(sm_count(&sms));
+    const int d = dk > dv ? dk : dv;
     const long long heads = (long long)b * h > 0 ? (long long)b * h : 1;
-    long long want = (2LL * sms + heads - 1) / heads, most = (t + 255) / 256;
-    if (want > most) want = most;
-    if (want < 1) want = 1;
-    long long len = ((long long)t + want - 1) / want;
-    len = (len + 127) / 128 * 128;
-    if (len < 128) len = 128;
-    *seg = (int)len;
-    *segments = (int)(t > 0 ? (t + len - 1) / len : 1);
+    // blocks that an SM holds of the kernel that serves these sizes
+    const int each = dtype == CNL_F32 ? (d > 64 ? 1 : 4) : tc_sizes(t, dk, dv, dtype) ? 1 : d > 64 ? 2 : d > 32 ? 4 : 8;
+    const long long places = (long long)sms * each, most = (t + 127) / 128;
+    long long best = 0;
+    *segments = 1;
+    *seg = (int)(((long long)t + 127) / 128 * 128);
+    if (*seg < 128) *seg = 128;
+    for (long long want = 1; want <= most && (want - 1) * heads < 4 * places; ++want) {
+        const long long len = ((t + want - 1) / want + 127) / 128 * 128, have = (t + len - 1) / len;
+        const long long cost = (heads * have + places - 1) / places * (len + kExtra);
+        if (best == 0 || cost < best) {
+            best = cost;
+            *segments = (int)have;
+            *seg = (int)len;
+        }
+    }
     return CNL_OK;
 }
 
@@ -297,10 +308,9 @@ int segment_plan(int b, int t, int h, int* segments, int* seg) {
 using namespace cnl;
 using namespace cnl::lin;
 
-extern "C" int cnl_linattn_segments(int b, int t, int h) {
+extern "C" int cnl_linattn_segments(int b, int t, int h, int dk, int dv, int dtype) {
     int segments = 0, seg = 0;
-    if (b < 0 || t < 0 || h < 1) return 1;
-    if (segment_plan(b, t, h, &segments, &seg) != CNL_OK) return -1;
+    if (lin::check(b, t, h, dk, dv, dtype) != CNL_OK || segment_plan(b, t, h, dk, dv, dtype, &segments, &seg) != CNL_OK) return -1;
     return segments;
 }
 
@@ -312,7 +322,7 @@ extern "C" int cnl_linattn_forward(const void* q, const void* k, const void* v, 
     if ((t > 0 && (!q || !k || !v || !out)) || !strides_host || !log_decay) return fail(CNL_ERR_NULL, "null pointer argument");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     int segments = 0, seg = 0;
-    CNL_TRY(segment_plan(b, t, h, &segments, &seg));
+    CNL_TRY(segment_plan(b, t, h, dk, dv, dtype, &segments, &seg));
     if (segments > 1 && !starts) return fail(CNL_ERR_NULL, "%d segments need the starts buffer", segments);
     const long long* s = strides_host;
     const Rows Q = {q, s[0], s[1], s[2]}, Kk = {k, s[3], s[4], s[5]}, V = {v, s[6], s[7], s[8]};
@@ -340,7 +350,7 @@ extern "C" int cnl_linattn_backward(const void* q, const void* k, const void* v,
     if ((t > 0 && (!q || !k || !v || !g_out || !g_q || !g_k || !g_v)) || !strides_host || !log_decay) return fail(CNL_ERR_NULL, "null pointer argument");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     int segments = 0, seg = 0;
-    CNL_TRY(segment_plan(b, t, h, &segments, &seg));
+    CNL_TRY(segment_plan(b, t, h, dk, dv, dtype, &segments, &seg));
     if (segments > 1 && (!starts || !scratch)) return fail(CNL_ERR_NULL, "%d segments need starts and scratch", segments);
     const long long* s = strides_host;
     const Rows Q = {q, s[0], s[1], s[2]}, Kk = {k, s[3], s[4], s[5]}, V = {v, s[6], s[7], s[8]}, G = {g_out, s[9], s[10], s[11]};

@@ -43,7 +43,8 @@ __device__ __forceinline__ float power(float a, int n) { return expf(a * (float)
 
 int run_sweep(const Sweep& s, int dtype, cudaStream_t st);          // dispatches to the kernel that serves the type and sizes
 int run_sweep_mma(const Sweep& s, int dtype, cudaStream_t st);      // fp16, bf16: mma.sync
-bool tc_serves(const Sweep& s, int dtype);                          // bf16 rows that TMA can take, 128 tokens or more
+bool tc_sizes(int t, int da, int dc, int dtype);                    // sizes that the tcgen05 sweep serves
+bool tc_serves(const Sweep& s, int dtype);                          // ... and rows that TMA can take
 int run_sweep_tc(const Sweep& s, cudaStream_t st);                  // ... on the fifth-generation tensor cores
 
 }  // namespace lin

@@ -502,12 +502,14 @@ int run_tc(Sweep s, cudaStream_t st) {
     return launch_tc<D, true, 2>(s, st);
 }
 
+bool tc_sizes(int t, int da, int dc, int dtype) { return dtype == CNL_BF16 && t >= kTok && da > 32 && dc > 32 && da % 8 == 0 && dc % 8 == 0; }
+
 bool tc_serves(const Sweep& s, int dtype) {
-    auto fits = [&](const Rows& r, int d) {
+    auto fits = [&](const Rows& r) {
         auto ok = [](long long n, long long stride) { return n <= 1 || (stride >= 0 && stride % 8 == 0 && stride < (1LL << 38)); };
-        return !r.p || (aligned16(r.p) && d % 8 == 0 && ok(s.h, r.sh) && ok(s.t, r.st) && r.st > 0 && ok(s.batch, r.sb));
+        return !r.p || (aligned16(r.p) && ok(s.h, r.sh) && ok(s.t, r.st) && r.st > 0 && ok(s.batch, r.sb));
     };
-    return dtype == CNL_BF16 && s.t >= kTok && s.da > 32 && s.dc > 32 && fits(s.a, s.da) && fits(s.b, s.da) && fits(s.c, s.dc) && aligned16(s.out);
+    return tc_sizes(s.t, s.da, s.dc, dtype) && fits(s.a) && fits(s.b) && fits(s.c) && aligned16(s.out);
 }
 
 int run_sweep_tc(const Sweep& s, cudaStream_t st) { return s.da <= 64 && s.dc <= 64 ? run_tc<64>(s, st) : run_tc<128>(s, st); }

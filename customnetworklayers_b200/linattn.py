@@ -57,7 +57,7 @@ def forward(q, k, v, log_decay, state=None, lengths=None, scale: Optional[float]
     lib = _lib.load()
     out = torch.empty((b, t, h, dv), dtype=q.dtype, device=q.device)
     end = torch.empty((b, h, dk, dv), dtype=torch.float32, device=q.device)
-    segments = on_device(q.device, lib.cnl_linattn_segments, b, t, h)
+    segments = on_device(q.device, lib.cnl_linattn_segments, b, t, h, dk, dv, DTYPES[q.dtype])
     if segments < 1:
         raise RuntimeError("linear attention: " + _lib.last_error())
     starts = torch.empty((b, h, segments, dk, dv), dtype=torch.float32, device=q.device) if segments > 1 else None

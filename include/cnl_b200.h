@@ -326,13 +326,13 @@ int cnl_blocknorm_backward(const void* x, const void* u, const void* gate, const
  * log_decay [h] fp32, at most 0 (-inf: no memory; not checked).  lengths [b] int (null: t): tokens at or behind lengths[b]
  * are not read, give zero rows and zero gradients; values are held to 0..t.  state, state_out, g_state_out, g_state
  * [b][h][dk][dv] fp32, each may be null.  dk, dv within 1..128.
- * starts: cnl_linattn_segments(b, t, h) * b * h * dk * dv floats, filled by the forward call (states at the start of the
+ * starts: cnl_linattn_segments(b, t, h, dk, dv, dtype) * b * h * dk * dv floats, filled by the forward call (states at the start of the
  * segments that run in parallel) and read by the backward call; scratch: as many floats.  Both may be null where
  * cnl_linattn_segments is 1; the backward call then reads `state`.
  * cnl_linattn_step: one token, q, k [b][h][dk], v [b][h][dv], strides_host the batch and head strides of q, k, v; state is
  * updated in place.
  */
-int cnl_linattn_segments(int b, int t, int h);
+int cnl_linattn_segments(int b, int t, int h, int dk, int dv, int dtype);
 /* 1 if a block of the current device's sweeps has ever given up waiting for its own copies or products (its outputs are NaN
  * then), 0 if none, negative on error.  Waits for the device. */
 int cnl_linattn_status(void);
