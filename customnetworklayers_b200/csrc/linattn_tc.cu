@@ -1,8 +1,8 @@
 // Linear attention sweep for bf16 on the fifth-generation tensor cores (formulas: linattn.cuh).
 //
-// A block of ten warps walks one segment of one head in chunks of 128 tokens.  One warp brings a, b, c rows by TMA (128-byte
-// swizzle), one thread issues the products, eight warps do what lies between.  Per chunk, accumulators in tensor memory:
-//     P = a b^T                 [128 tokens x 128 tokens]   -> weighted, masked, rounded, written back as an operand
+// A block of 18 warps walks one segment of one head in chunks of 128 tokens.  One warp brings a, b, c rows by TMA (128-byte
+// swizzle), one thread issues the products, sixteen warps do what lies between.  Per chunk, accumulators in tensor memory:
+//     P = a b^T                 [128 tokens x 128 tokens]   -> weighted, masked, rounded, put back in tensor memory
 //     X = a W                   [128 tokens x dc]           W as the sweep has it before the chunk
 //     O = P c                   [128 tokens x dc]
 //     T = (weighted c)^T b      [dc x da]                   what the chunk adds to W^T
@@ -29,7 +29,7 @@ __device__ int g_gave_up = 0;
 
 constexpr int kTok = 128;                       // tokens of a chunk
 constexpr int kBlk = kTok * 128;                // bytes of 128 rows of 64 elements
-constexpr int kWorkers = 8;                     // warps between the products
+constexpr int kWorkers = 16;                    // warps between the products
 constexpr int kTcThreads = (kWorkers + 2) * 32;
 constexpr int kSpins = 1 << 22;
 
@@ -62,16 +62,25 @@ __device__ __forceinline__ void tc_commit(unsigned bar) { asm volatile("tcgen05.
 __device__ __forceinline__ void tc_mma(unsigned d, unsigned long long a, unsigned long long b, unsigned what, bool add) {
     asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(what), "r"((unsigned)add) : "memory");
 }
-__device__ __forceinline__ void tc_load(unsigned at, float (&v)[32]) {
-    unsigned r[32];
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-                   "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
-                   "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-                 : "r"(at));
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+// the same with the rows' operand in tensor memory: 128 lanes, two summed elements a column
+__device__ __forceinline__ void tc_mma_t(unsigned d, unsigned a, unsigned long long b, unsigned what, bool add) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(what), "r"((unsigned)add) : "memory");
 }
+// 32 lanes of the warp's quarter, 16 or 32 columns
+__device__ __forceinline__ void tc_load(unsigned at, unsigned (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(at));
+}
+__device__ __forceinline__ void tc_load(unsigned at, unsigned (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(at));
+}
+__device__ __forceinline__ void tc_store(unsigned at, const unsigned (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(at) : "memory");
+}
+__device__ __forceinline__ void tc_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // Descriptor of an operand in shared memory, 128-byte swizzle.  Summed dimension contiguous: `step` is the distance of
@@ -86,13 +95,14 @@ __host__ __device__ constexpr unsigned product(int n, int strided_a, int strided
 
 template <int D, bool OUT, int PARTS>
 struct Map {                                    // shared memory in bytes from a 1024-byte boundary
-    static constexpr int nb = D / 64;
-    static constexpr int stages = D == 64 || !OUT ? 2 : 1;
-    static constexpr int a = 0, b = OUT ? nb * kBlk : 0, c = b + nb * kBlk, stage = c + nb * kBlk;
-    static constexpr int p = stages * stage, w = p + (OUT ? 2 * kBlk : 0);
+    static constexpr int nb = D / 64, one = nb * kBlk;           // one operand's rows
+    // heads of 128 with outputs leave no room for two of everything: c is held longest, so it has two
+    static constexpr int two_ab = D == 64 || !OUT ? 2 : 1, two_c = 2;
+    static constexpr int a = 0, b = a + (OUT ? two_ab * one : 0), c = b + two_ab * one, w = c + two_c * one;
     static constexpr int parts = w + (OUT ? (D == 128 ? 2 * kBlk : kBlk) : 0);
     static constexpr int part_blocks = D == 128 ? 2 * PARTS : PARTS == 3 ? 4 : 2;
-    static constexpr int bars = parts + part_blocks * kBlk;
+    static constexpr int tables = parts + part_blocks * kBlk;    // powers of the decay for P: 32 for whole tiles, 64 for diagonal ones
+    static constexpr int bars = tables + 96 * 4;
     static constexpr int bytes = bars + 256 + 1024;              // and the way to the boundary
 };
 
@@ -101,15 +111,20 @@ template <int D, bool OUT, int PARTS>
 __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                            const __grid_constant__ CUtensorMap map_c) {
     using M = Map<D, OUT, PARTS>;
-    constexpr int NB = M::nb, S = M::stages;
+    constexpr int NB = M::nb;
     extern __shared__ unsigned char raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<size_t>(raw) + 1023) & ~(size_t)1023);
     const unsigned base = smem_at(sm), bars = base + M::bars;
     volatile int* dead = reinterpret_cast<volatile int*>(sm + M::bars + 240);
     unsigned* tmem_word = reinterpret_cast<unsigned*>(sm + M::bars + 244);
-    // barriers, one of each for every stage
+    // barriers, two of each: chunk i uses number i mod 2, whose phase is then i / 2
     enum { FULL_A, FULL_B, FULL_C, DONE_P, DONE_X, DONE_T, DONE_O, HAS_C, HAS_P, HAS_W, HAS_O, KINDS };
-    auto bar = [&](int kind, int stage) { return bars + (unsigned)(kind * S + stage) * 8; };
+    auto read_p = [&](int quarter) { return bars + (unsigned)(KINDS * 2 + quarter) * 8; };      // P's fp32 columns of these lanes have been read
+    auto bar = [&](int kind, int i) { return bars + (unsigned)(kind * 2 + (i & 1)) * 8; };
+    auto phase = [](int i) { return (unsigned)(i >> 1) & 1u; };
+    auto at_a = [](int i) { return M::a + i % M::two_ab * M::one; };
+    auto at_b = [](int i) { return M::b + i % M::two_ab * M::one; };
+    auto at_c = [](int i) { return M::c + i % M::two_c * M::one; };
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int seg = blockIdx.x % s.segments, bh = blockIdx.x / s.segments, head = bh % s.h, bat = bh / s.h;
@@ -124,10 +139,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
 
     if (tid == 0) {
         *dead = 0;
-        for (int i = 0; i < S; ++i) {
+        for (int i = 0; i < 2; ++i) {
             for (int k = FULL_A; k <= DONE_O; ++k) bar_init(bar(k, i), 1);
             for (int k = HAS_C; k <= HAS_O; ++k) bar_init(bar(k, i), kWorkers);
         }
+        for (int k = 0; k < 4; ++k) bar_init(read_p(k), kWorkers / 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kWorkers + 1) {
@@ -144,25 +160,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
         if (lane == 0) {
             int i = 0;
             for (; i < chunks; ++i) {
-                const int st = i % S, t0 = token0(i);
-                const unsigned at = base + st * M::stage;
-                const unsigned before = (unsigned)((i / S) - 1) & 1u;
-                auto take = [&](int full, int done, const CUtensorMap* map, const Rows& r, int offset) {
-                    if (i >= S && !bar_wait(bar(done, st), before, dead)) return false;
-                    bar_expect(bar(full, st), NB * kBlk);
-                    for (int x = 0; x < NB; ++x) tma_load(at + offset + x * kBlk, map, x * 64, r.sh ? head : 0, t0, r.sb ? bat : 0, bar(full, st));
+                const int t0 = token0(i);
+                auto take = [&](int full, int done, int room, const CUtensorMap* map, const Rows& r, int to) {
+                    if (i >= room && !bar_wait(bar(done, i - room), phase(i - room), dead)) return false;
+                    bar_expect(bar(full, i), M::one);
+                    for (int x = 0; x < NB; ++x) tma_load(base + to + x * kBlk, map, x * 64, r.sh ? head : 0, t0, r.sb ? bat : 0, bar(full, i));
                     return true;
                 };
-                if (OUT && !take(FULL_A, DONE_X, &map_a, s.a, M::a)) break;
-                if (!take(FULL_B, DONE_T, &map_b, s.b, M::b)) break;
-                if (!take(FULL_C, OUT ? DONE_O : DONE_T, &map_c, s.c, M::c)) break;
+                if (OUT && !take(FULL_A, DONE_X, M::two_ab, &map_a, s.a, at_a(i))) break;
+                if (!take(FULL_B, DONE_T, M::two_ab, &map_b, s.b, at_b(i))) break;
+                if (!take(FULL_C, OUT ? DONE_O : DONE_T, M::two_c, &map_c, s.c, at_c(i))) break;
             }
             if (*dead) {                                         // what was asked for has to land before the block leaves
-                int never = 0;
-                for (int j = max(0, i - S); j <= min(i, chunks - 1); ++j)
+                for (int j = max(0, i - 2); j <= min(i, chunks - 1); ++j)
                     for (int k = OUT ? FULL_A : FULL_B; k <= FULL_C; ++k)
-                        for (int spin = 0; spin < 4096 && !bar_try(bar(k, j % S), (unsigned)(j / S) & 1u); ++spin) ++never;
-                (void)never;
+                        for (int spin = 0; spin < 4096 && !bar_try(bar(k, j), phase(j)); ++spin) {}
             }
         }
         __syncwarp();
@@ -170,22 +182,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
         // ---- products
         if (lane == 0) {
             for (int i = 0; i < chunks; ++i) {
-                const int st = i % S;
-                const unsigned ph = (unsigned)(i / S) & 1u, at = base + st * M::stage;
+                const unsigned ph = phase(i);
                 const bool cut = hi - lo - i * kTok < kTok && !s.reversed;       // rows behind the end are cleared first
-                const unsigned A = at + M::a, B = at + M::b, C = at + M::c, P = base + M::p, W = base + M::w, Q = base + M::parts;
+                const unsigned A = base + at_a(i), B = base + at_b(i), C = base + at_c(i), W = base + M::w, Q = base + M::parts;
                 if constexpr (OUT) {
-                    if (!bar_wait(bar(FULL_A, st), ph, dead) || !bar_wait(bar(FULL_B, st), ph, dead)) break;
-                    if (cut && !bar_wait(bar(HAS_C, st), ph, dead)) break;
+                    if (!bar_wait(bar(FULL_A, i), ph, dead) || !bar_wait(bar(FULL_B, i), ph, dead)) break;
+                    if (cut && !bar_wait(bar(HAS_C, i), ph, dead)) break;
+                    if (i > 0 && !bar_wait(bar(DONE_O, i - 1), phase(i - 1), dead)) break;       // O has read the P before
                     tc_after();
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) {
                         const unsigned o = (k / 4) * kBlk + (k % 4) * 32;
                         tc_mma(tP, operand(A + o, 16, 1024), operand(B + o, 16, 1024), product(128, 0, 0), k > 0);
                     }
-                    tc_commit(bar(DONE_P, st));
-                    if (!bar_wait(bar(HAS_W, st), ph, dead)) break;
-                    if (i > 0 && !bar_wait(bar(HAS_O, (i - 1) % S), (unsigned)((i - 1) / S) & 1u, dead)) break;
+                    tc_commit(bar(DONE_P, i));
+                    if (!bar_wait(bar(HAS_W, i), ph, dead)) break;
+                    if (i > 0 && !bar_wait(bar(HAS_O, i - 1), phase(i - 1), dead)) break;
                     tc_after();
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) {
@@ -196,35 +208,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
 #pragma unroll
                         for (int k = 0; k < 4; ++k) tc_mma(tX, operand(A + k * 32, 16, 1024), operand(W + kBlk / 2 + k * 32, 16, 1024), product(D, 0, 0), true);
                     }
-                    tc_commit(bar(DONE_X, st));
+                    tc_commit(bar(DONE_X, i));
                 } else {
-                    if (!bar_wait(bar(FULL_B, st), ph, dead)) break;
-                    if (i > 0 && !bar_wait(bar(HAS_W, (i - 1) % S), (unsigned)((i - 1) / S) & 1u, dead)) break;       // T has been read
+                    if (!bar_wait(bar(FULL_B, i), ph, dead)) break;
+                    if (i > 0 && !bar_wait(bar(HAS_W, i - 1), phase(i - 1), dead)) break;       // T has been read
                 }
-                if (!bar_wait(bar(HAS_C, st), ph, dead)) break;
+                if (!bar_wait(bar(HAS_C, i), ph, dead)) break;
                 tc_after();
                 // small parts first
-                if constexpr (D == 128) {
 #pragma unroll
-                    for (int p = PARTS - 1; p >= 0; --p)
-#pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            tc_mma(tT, operand(Q + p * 2 * kBlk + k * 2048, kBlk, 1024), operand(B + k * 2048, kBlk, 1024), product(128, 1, 1), p < PARTS - 1 || k > 0);
-                } else {
-#pragma unroll
-                    for (int p = PARTS == 3 ? 1 : 0; p >= 0; --p)
-#pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            tc_mma(tT, operand(Q + p * 2 * kBlk + k * 2048, kBlk, 1024), operand(B + k * 2048, kBlk, 1024), product(64, 1, 1), p < (PARTS == 3 ? 1 : 0) || k > 0);
-                }
-                tc_commit(bar(DONE_T, st));
-                if constexpr (OUT) {
-                    if (!bar_wait(bar(HAS_P, st), ph, dead)) break;
-                    tc_after();
+                for (int p = (D == 128 ? PARTS : PARTS - 1) - 1; p >= 0; --p)
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
-                        tc_mma(tO, operand(P + (k / 4) * kBlk + (k % 4) * 32, 16, 1024), operand(C + k * 2048, kBlk, 1024), product(D, 0, 1), k > 0);
-                    tc_commit(bar(DONE_O, st));
+                        tc_mma(tT, operand(Q + p * 2 * kBlk + k * 2048, kBlk, 1024), operand(B + k * 2048, kBlk, 1024), product(D, 1, 1), p < (D == 128 ? PARTS : PARTS - 1) - 1 || k > 0);
+                tc_commit(bar(DONE_T, i));
+                if constexpr (OUT) {
+                    if (!bar_wait(bar(HAS_P, i), ph, dead)) break;
+                    tc_after();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) tc_mma_t(tO, tP + k * 8, operand(C + k * 2048, kBlk, 1024), product(D, 0, 1), k > 0);
+                    tc_commit(bar(DONE_O, i));
                 }
             }
             if (*dead) {                                         // products under way end before the tensor memory goes
@@ -235,87 +238,93 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
         }
         __syncwarp();
     } else {
-        // ---- between the products: warp w holds lanes 32 (w mod 4) .. of tensor memory and one half of the columns
-        constexpr int HC = D / 2;                                // columns of X, O and T that a thread holds
-        const int q = warp & 3, half = warp >> 2, row = q * 32 + lane;
+        // ---- between the products: warp w holds lanes 32 (w mod 4) .. of tensor memory and a quarter of the columns
+        constexpr int HC = D / 4;                                // columns of X, O and T that a thread holds
+        constexpr int kAll = kWorkers * 32;
+        const int q = warp & 3, cq = warp >> 2, row = q * 32 + lane;
         const unsigned lanes = (unsigned)(q * 32) << 16;
-        const float ld = clamp_log(s.log_decay[head]), a2 = ld * 1.4426950408889634f, both = s.in_scale * s.out_scale;
+        const float ld = clamp_log(s.log_decay[head]), both = s.in_scale * s.out_scale;
         const float keep_full = power(ld, kTok);
         const int pos = s.reversed ? kTok - 1 - row : row;
         const float far = s.out_scale * power(ld, pos + s.off);
-        // weights of the token rows of this thread's pieces: rows tid / 8 + 32 k of 128-byte rows
+        // P: a tile of 32 x 32 that lies off the diagonal weighs u (this thread's) times a row of 32; one on it l^(lane - x)
+        float* whole = reinterpret_cast<float*>(sm + M::tables);
+        float* edge = whole + 32;                                // edge[32 + d] = l^d, 0 for d < 0
+        const int behind = s.reversed ? 32 * cq - row : row - 32 * cq - 31;
+        const float u = behind > 0 ? both * power(ld, behind) : both;
+        if (OUT && tid < 96) {
+            if (tid < 32) whole[tid] = power(ld, s.reversed ? tid : 31 - tid);
+            else edge[tid - 32] = tid < 64 ? 0.0f : power(ld, tid - 64);
+        }
+        // weights of the token rows of this thread's pieces: rows tid / 8 and 64 more
         const int prow = tid >> 3;
-        float wt[4];
+        float wt[2];
         auto weigh = [&](int m) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int r = prow + 32 * k, j = s.reversed ? kTok - 1 - r : r;
+            for (int k = 0; k < 2; ++k) {
+                const int r = prow + 64 * k, j = s.reversed ? kTok - 1 - r : r;
                 wt[k] = j < m ? power(ld, m - s.off - j) * s.in_scale : 0.0f;
             }
         };
         weigh(kTok);
-        // W^T: D = 128: row = column of c, 64 columns from 64 half; D = 64: rows 0..63 first addend, 64..127 second
-        const int wrow = D == 128 ? row : row & 63, wcol = half * HC;
-        float w[HC];
+        // W^T: D = 128: row = column of c; D = 64: rows 0..63 first addend, 64..127 second
+        const int wrow = D == 128 ? row : row & 63, wcol = cq * HC;
+        float2 w[HC / 2];
         {
             const float* w0 = s.start ? s.start + ((long long)bh * s.segments + seg) * size : nullptr;
             const bool has = w0 && wrow < dc && (D == 128 || row < 64);
 #pragma unroll
             for (int x = 0; x < HC; ++x) {
                 const int i = wcol + x;
-                w[x] = has && i < da ? (s.transposed ? w0[(long long)wrow * da + i] : w0[(long long)i * dc + wrow]) : 0.0f;
+                const float v = has && i < da ? (s.transposed ? w0[(long long)wrow * da + i] : w0[(long long)i * dc + wrow]) : 0.0f;
+                if (x & 1) w[x / 2].y = v;
+                else w[x / 2].x = v;
             }
         }
-        auto put_row = [&](unsigned char* tile, int r, int first_piece, const float* v, int pieces) {       // 16-byte pieces of a swizzled 128-byte row
-            for (int x = 0; x < pieces; ++x)
-                *reinterpret_cast<uint4*>(tile + r * 128 + (((first_piece + x) ^ (r & 7)) << 4)) =
-                    make_uint4(pack2<__nv_bfloat16>(v[8 * x], v[8 * x + 1]), pack2<__nv_bfloat16>(v[8 * x + 2], v[8 * x + 3]), pack2<__nv_bfloat16>(v[8 * x + 4], v[8 * x + 5]), pack2<__nv_bfloat16>(v[8 * x + 6], v[8 * x + 7]));
+        auto four = [](const float2* v) {                        // eight numbers as a 16-byte piece
+            return make_uint4(pack2<__nv_bfloat16>(v[0].x, v[0].y), pack2<__nv_bfloat16>(v[1].x, v[1].y), pack2<__nv_bfloat16>(v[2].x, v[2].y), pack2<__nv_bfloat16>(v[3].x, v[3].y));
         };
-        auto tell = [&](int kind, int stage) {
+        auto tell = [&](int kind, int i) {
             tc_before();
             __syncwarp();
-            if (lane == 0) bar_arrive(bar(kind, stage));
+            if (lane == 0) bar_arrive(bar(kind, i));
         };
         auto put_w = [&](int i) {                                // W as the operand of chunk i
             if constexpr (OUT) {
-                unsigned char* W = sm + M::w;
+                unsigned char* to = sm + M::w + (D == 128 ? (cq >> 1) * kBlk : (row >> 6) * (kBlk / 2)) + wrow * 128;
+                const int piece = D == 128 ? (cq & 1) * 4 : cq * 2;
 #pragma unroll
-                for (int x = 0; x < HC / 8; ++x) {
-                    const float* v = w + 8 * x;
-                    if constexpr (D == 128) put_row(W + half * kBlk, wrow, x, v, 1);
-                    else put_row(W + (row >> 6) * (kBlk / 2), wrow, half * 4 + x, v, 1);
-                }
+                for (int x = 0; x < HC / 8; ++x) *reinterpret_cast<uint4*>(to + (((piece + x) ^ (wrow & 7)) << 4)) = four(w + 4 * x);
                 fence_async();
             }
-            tell(HAS_W, i % S);
+            tell(HAS_W, i);
         };
         if constexpr (PARTS == 3 && D == 64) {                   // the rows that stand beside the third part
-            for (int x = tid; x < kBlk / 16; x += kWorkers * 32) reinterpret_cast<uint4*>(sm + M::parts + 3 * kBlk)[x] = make_uint4(0, 0, 0, 0);
+            for (int x = tid; x < kBlk / 16; x += kAll) reinterpret_cast<uint4*>(sm + M::parts + 3 * kBlk)[x] = make_uint4(0, 0, 0, 0);
             fence_async();
         }
+        asm volatile("bar.sync 1, %0;" ::"n"(kAll) : "memory");  // the tables
         if (OUT && chunks > 0) put_w(0);
 
         for (int i = 0; i < chunks; ++i) {
-            const int st = i % S;
-            const unsigned ph = (unsigned)(i / S) & 1u;
+            const unsigned ph = phase(i);
             const int left = hi - lo - i * kTok, m = left < kTok ? left : kTok;
-            unsigned char* at = sm + st * M::stage;
             // the weighted c in parts
-            if (!bar_wait(bar(FULL_C, st), ph, dead)) break;
+            if (!bar_wait(bar(FULL_C, i), ph, dead)) break;
             const bool cut = m < kTok && !s.reversed;
             if (m < kTok) weigh(m);
-            if (cut && (!bar_wait(bar(FULL_B, st), ph, dead) || (OUT && !bar_wait(bar(FULL_A, st), ph, dead)))) break;
+            if (cut && (!bar_wait(bar(FULL_B, i), ph, dead) || (OUT && !bar_wait(bar(FULL_A, i), ph, dead)))) break;
 #pragma unroll
             for (int x = 0; x < NB; ++x)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int off = x * kBlk + (tid + 256 * k) * 16;
-                    uint4 v = *reinterpret_cast<const uint4*>(at + M::c + off);
-                    if (cut && prow + 32 * k >= m) {             // rows behind the end: nothing, whatever they hold
+                for (int k = 0; k < 2; ++k) {
+                    const int off = x * kBlk + (tid + kAll * k) * 16;
+                    uint4 v = *reinterpret_cast<const uint4*>(sm + at_c(i) + off);
+                    if (cut && prow + 64 * k >= m) {             // rows behind the end: nothing, whatever they hold
                         v = make_uint4(0, 0, 0, 0);
-                        *reinterpret_cast<uint4*>(at + M::c + off) = v;
-                        *reinterpret_cast<uint4*>(at + M::b + off) = v;
-                        if (OUT) *reinterpret_cast<uint4*>(at + M::a + off) = v;
+                        *reinterpret_cast<uint4*>(sm + at_c(i) + off) = v;
+                        *reinterpret_cast<uint4*>(sm + at_b(i) + off) = v;
+                        if (OUT) *reinterpret_cast<uint4*>(sm + at_a(i) + off) = v;
                     }
                     unsigned in[4] = {v.x, v.y, v.z, v.w}, part[PARTS][4];
                     const float2 f = make_float2(wt[k], wt[k]);
@@ -325,107 +334,117 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
 #pragma unroll
                         for (int p = 0; p < PARTS; ++p) {
                             part[p][e] = pack2<__nv_bfloat16>(y.x, y.y);
-                            const float2 z = unpack2(part[p][e], __nv_bfloat16());
-                            y = __fadd2_rn(y, make_float2(-z.x, -z.y));
+                            if (p + 1 < PARTS) {
+                                const float2 z = unpack2(part[p][e], __nv_bfloat16());
+                                y = __fadd2_rn(y, make_float2(-z.x, -z.y));
+                            }
                         }
                     }
 #pragma unroll
                     for (int p = 0; p < PARTS; ++p)
-                        *reinterpret_cast<uint4*>(sm + M::parts + p * NB * kBlk + off) = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
+                        *reinterpret_cast<uint4*>(sm + M::parts + p * M::one + off) = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
                 }
             fence_async();
-            tell(HAS_C, st);
+            tell(HAS_C, i);
             if constexpr (OUT) {
-                // P: weights and mask
-                if (!bar_wait(bar(DONE_P, st), ph, dead)) break;
+                // P: weights and mask; back into tensor memory, two columns in one, once the four warps of these lanes have read it
+                if (!bar_wait(bar(DONE_P, i), ph, dead)) break;
                 tc_after();
-                const int d0 = s.reversed ? half * 64 - row : row - half * 64;          // positions from column 64 half to this row
-                const bool none = s.reversed ? (q >= 2 && half == 0) : (q < 2 && half == 1);   // all above the diagonal
-                unsigned char* to = sm + M::p + half * kBlk;
+                unsigned r[32], to[16];
+                if (s.reversed ? cq < q : cq > q) {              // above the diagonal
 #pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    float v[32];
-                    if (none) {
+                    for (int x = 0; x < 16; ++x) to[x] = 0;
+                } else {
+                    tc_load(tP + lanes + cq * 32, r);
+                    tc_wait_load();
+                    if (cq == q) {
+                        const float* e = edge + 32 + (s.reversed ? -lane : lane);
 #pragma unroll
-                        for (int x = 0; x < 32; ++x) v[x] = 0.0f;
+                        for (int x = 0; x < 16; ++x) {
+                            const float2 f = s.reversed ? make_float2(e[2 * x], e[2 * x + 1]) : make_float2(e[-2 * x], e[-2 * x - 1]);
+                            const float2 y = __fmul2_rn(__fmul2_rn(make_float2(__uint_as_float(r[2 * x]), __uint_as_float(r[2 * x + 1])), make_float2(both, both)), f);
+                            to[x] = pack2<__nv_bfloat16>(y.x, y.y);
+                        }
                     } else {
-                        tc_load(tP + lanes + half * 64 + y * 32, v);
-                        tc_wait_load();
 #pragma unroll
-                        for (int x = 0; x < 32; ++x) {
-                            const int d = s.reversed ? d0 + y * 32 + x : d0 - y * 32 - x;
-                            const float f = exp2_approx(a2 * (float)d) * both;
-                            v[x] = d >= 0 ? v[x] * f : 0.0f;
+                        for (int x = 0; x < 16; ++x) {
+                            const float2 f = *reinterpret_cast<const float2*>(whole + 2 * x);
+                            const float2 y = __fmul2_rn(__fmul2_rn(make_float2(__uint_as_float(r[2 * x]), __uint_as_float(r[2 * x + 1])), make_float2(u, u)), f);
+                            to[x] = pack2<__nv_bfloat16>(y.x, y.y);
                         }
                     }
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) put_row(to, row, y * 4 + x, v + 8 * x, 1);
                 }
-                fence_async();
-                tell(HAS_P, st);
+                tc_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(read_p(q));
+                if (!bar_wait(read_p(q), (unsigned)i & 1u, dead)) break;
+                tc_after();
+                tc_store(tP + lanes + cq * 16, to);
+                tc_wait_store();
+                tell(HAS_P, i);
             }
             // W^T <- l^m W^T + T
-            if (!bar_wait(bar(DONE_T, st), ph, dead)) break;
+            if (!bar_wait(bar(DONE_T, i), ph, dead)) break;
             tc_after();
-            const float keep = m < kTok ? power(ld, m) : keep_full;
-#pragma unroll
-            for (int y = 0; y < HC / 32; ++y) {
-                float v[32];
-                tc_load(tT + lanes + wcol + y * 32, v);
+            {
+                const float keep = m < kTok ? power(ld, m) : keep_full;
+                unsigned r[HC];
+                tc_load(tT + lanes + wcol, r);
                 tc_wait_load();
 #pragma unroll
-                for (int x = 0; x < 32; ++x) w[y * 32 + x] = fmaf(keep, w[y * 32 + x], v[x]);
+                for (int x = 0; x < HC / 2; ++x) w[x] = __ffma2_rn(make_float2(keep, keep), w[x], make_float2(__uint_as_float(r[2 * x]), __uint_as_float(r[2 * x + 1])));
             }
             if constexpr (OUT) {
-                if (!bar_wait(bar(DONE_X, st), ph, dead)) break;
-            }
-            if (i + 1 < chunks) {
-                if constexpr (OUT) put_w(i + 1);
-                else tell(HAS_W, st);
-            }
-            if constexpr (OUT) {
+                if (!bar_wait(bar(DONE_X, i), ph, dead)) break;
+                if (i + 1 < chunks) put_w(i + 1);
                 // out = l^{pos + off} X + O
-                if (!bar_wait(bar(DONE_O, st), ph, dead)) break;
+                if (!bar_wait(bar(DONE_O, i), ph, dead)) break;
                 tc_after();
                 const bool live = pos < m;
-                const long long tok = token0(i) + row;
-                __nv_bfloat16* out = (__nv_bfloat16*)s.out + (((long long)bat * s.t + tok) * s.h + head) * dc + wcol;
+                __nv_bfloat16* out = (__nv_bfloat16*)s.out + (((long long)bat * s.t + token0(i) + row) * s.h + head) * dc + wcol;
 #pragma unroll
-                for (int y = 0; y < HC / 32; ++y) {
-                    float x1[32], x2[32];
-                    tc_load(tX + lanes + wcol + y * 32, x1);
-                    tc_load(tO + lanes + wcol + y * 32, x2);
+                for (int y = 0; y < HC / 16; ++y) {
+                    unsigned r1[16], r2[16];
+                    tc_load(tX + lanes + wcol + y * 16, r1);
+                    tc_load(tO + lanes + wcol + y * 16, r2);
                     tc_wait_load();
-                    if (y == HC / 32 - 1) tell(HAS_O, st);
+                    if (y == HC / 16 - 1) tell(HAS_O, i);
+                    float2 v[8];
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) x1[x] = fmaf(far, x1[x], x2[x]);
+                    for (int x = 0; x < 8; ++x)
+                        v[x] = __ffma2_rn(make_float2(far, far), make_float2(__uint_as_float(r1[2 * x]), __uint_as_float(r1[2 * x + 1])), make_float2(__uint_as_float(r2[2 * x]), __uint_as_float(r2[2 * x + 1])));
                     if (live) {
 #pragma unroll
-                        for (int x = 0; x < 4; ++x)
-                            if (wcol + y * 32 + x * 8 < dc)
-                                *reinterpret_cast<uint4*>(out + y * 32 + x * 8) =
-                                    make_uint4(pack2<__nv_bfloat16>(x1[8 * x], x1[8 * x + 1]), pack2<__nv_bfloat16>(x1[8 * x + 2], x1[8 * x + 3]), pack2<__nv_bfloat16>(x1[8 * x + 4], x1[8 * x + 5]), pack2<__nv_bfloat16>(x1[8 * x + 6], x1[8 * x + 7]));
+                        for (int x = 0; x < 2; ++x)
+                            if (wcol + y * 16 + x * 8 < dc) *reinterpret_cast<uint4*>(out + y * 16 + x * 8) = four(v + 4 * x);
                     }
                 }
-            }
+            } else if (i + 1 < chunks) tell(HAS_W, i);
         }
         if (s.end) {
             float* w1 = s.end + ((long long)bh * s.segments + seg) * size;
             if constexpr (D == 64) {                             // the two addends meet in shared memory (the parts' room)
-                asm volatile("bar.sync 1, %0;" ::"n"(kWorkers * 32) : "memory");
+                asm volatile("bar.sync 1, %0;" ::"n"(kAll) : "memory");
                 float* meet = reinterpret_cast<float*>(sm + M::parts);
                 if (row >= 64)
 #pragma unroll
-                    for (int x = 0; x < HC; ++x) meet[(wcol + x) * 64 + wrow] = w[x];
-                asm volatile("bar.sync 1, %0;" ::"n"(kWorkers * 32) : "memory");
+                    for (int x = 0; x < HC / 2; ++x) {
+                        meet[(wcol + 2 * x) * 64 + wrow] = w[x].x;
+                        meet[(wcol + 2 * x + 1) * 64 + wrow] = w[x].y;
+                    }
+                asm volatile("bar.sync 1, %0;" ::"n"(kAll) : "memory");
                 if (row < 64)
 #pragma unroll
-                    for (int x = 0; x < HC; ++x) w[x] += meet[(wcol + x) * 64 + wrow];
+                    for (int x = 0; x < HC / 2; ++x) {
+                        w[x].x += meet[(wcol + 2 * x) * 64 + wrow];
+                        w[x].y += meet[(wcol + 2 * x + 1) * 64 + wrow];
+                    }
             }
+            const bool lost = *dead != 0;
             if (wrow < dc && (D == 128 || row < 64))
 #pragma unroll
                 for (int x = 0; x < HC; ++x)
-                    if (wcol + x < da) w1[(long long)(wcol + x) * dc + wrow] = *dead ? __uint_as_float(0x7fffffffu) : w[x];
+                    if (wcol + x < da) w1[(long long)(wcol + x) * dc + wrow] = lost ? __uint_as_float(0x7fffffffu) : x & 1 ? w[x / 2].y : w[x / 2].x;
         }
     }
     tc_before();
