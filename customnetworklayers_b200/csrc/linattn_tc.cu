@@ -400,8 +400,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
                 // out = l^{pos + off} X + O
                 if (!bar_wait(bar(DONE_O, i), ph, dead)) break;
                 tc_after();
-                const bool live = pos < m;
-                __nv_bfloat16* out = (__nv_bfloat16*)s.out + (((long long)bat * s.t + token0(i) + row) * s.h + head) * dc + wcol;
+                // the warp's 32 rows turn in shared memory (the pieces of the parts that only this warp writes: T has been summed),
+                // so that neighbouring lanes store neighbouring 16 bytes
+                constexpr int kPieces = HC / 8, kRows = 512 / (HC * 2);            // 16-byte pieces of a row; rows in 512 bytes
+                auto turn = [&](int r, int x) {
+                    const int c = r / kRows, in = r % kRows * HC * 2 + ((x ^ (kPieces == 4 ? r >> 1 & 3 : r >> 2 & 1)) << 4);
+                    return sm + M::parts + (c >> 1) * kBlk + (c & 1) * (kAll * 16) + warp * 512 + in;
+                };
 #pragma unroll
                 for (int y = 0; y < HC / 16; ++y) {
                     unsigned r1[16], r2[16];
@@ -413,12 +418,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
 #pragma unroll
                     for (int x = 0; x < 8; ++x)
                         v[x] = __ffma2_rn(make_float2(far, far), make_float2(__uint_as_float(r1[2 * x]), __uint_as_float(r1[2 * x + 1])), make_float2(__uint_as_float(r2[2 * x]), __uint_as_float(r2[2 * x + 1])));
-                    if (live) {
 #pragma unroll
-                        for (int x = 0; x < 2; ++x)
-                            if (wcol + y * 16 + x * 8 < dc) *reinterpret_cast<uint4*>(out + y * 16 + x * 8) = four(v + 4 * x);
-                    }
+                    for (int x = 0; x < 2; ++x) *reinterpret_cast<uint4*>(turn(lane, y * 2 + x)) = four(v + 4 * x);
                 }
+                __syncwarp();
+                const int r0 = lane / kPieces, x0 = lane % kPieces;
+                const long long by = (long long)s.h * dc;
+                __nv_bfloat16* out = (__nv_bfloat16*)s.out + ((long long)bat * s.t * s.h + head) * dc + (token0(i) + q * 32 + r0) * by + wcol + x0 * 8;
+#pragma unroll
+                for (int y = 0; y < kPieces; ++y) {
+                    constexpr int kEach = 32 / kPieces;
+                    const int r = q * 32 + r0 + y * kEach;
+                    if ((s.reversed ? kTok - 1 - r : r) < m && wcol + x0 * 8 < dc)
+                        *reinterpret_cast<uint4*>(out + y * kEach * by) = *reinterpret_cast<const uint4*>(turn(r0 + y * kEach, x0));
+                }
+                __syncwarp();
             } else if (i + 1 < chunks) tell(HAS_W, i);
         }
         if (s.end) {
