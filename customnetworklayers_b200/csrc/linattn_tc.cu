@@ -96,9 +96,9 @@ __host__ __device__ constexpr unsigned product(int n, int strided_a, int strided
 template <int D, bool OUT, int PARTS>
 struct Map {                                    // shared memory in bytes from a 1024-byte boundary
     static constexpr int nb = D / 64, one = nb * kBlk;           // one operand's rows
-    // heads of 128 with outputs leave no room for two of everything: c is held longest, so it has two
-    static constexpr int two_ab = D == 64 || !OUT ? 2 : 1, two_c = 2;
-    static constexpr int a = 0, b = a + (OUT ? two_ab * one : 0), c = b + two_ab * one, w = c + two_c * one;
+    // heads of 128 with outputs leave no room for two of everything: b is held longest, so it has two
+    static constexpr int two_ac = D == 64 || !OUT ? 2 : 1, two_b = 2;
+    static constexpr int a = 0, b = a + (OUT ? two_ac * one : 0), c = b + two_b * one, w = c + two_ac * one;
     static constexpr int parts = w + (OUT ? (D == 128 ? 2 * kBlk : kBlk) : 0);
     static constexpr int part_blocks = D == 128 ? 2 * PARTS : PARTS == 3 ? 4 : 2;
     static constexpr int tables = parts + part_blocks * kBlk;    // powers of the decay for P: 32 for whole tiles, 64 for diagonal ones
@@ -115,16 +115,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
     extern __shared__ unsigned char raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<size_t>(raw) + 1023) & ~(size_t)1023);
     const unsigned base = smem_at(sm), bars = base + M::bars;
-    volatile int* dead = reinterpret_cast<volatile int*>(sm + M::bars + 240);
-    unsigned* tmem_word = reinterpret_cast<unsigned*>(sm + M::bars + 244);
+    volatile int* dead = reinterpret_cast<volatile int*>(sm + M::bars + 248);
+    unsigned* tmem_word = reinterpret_cast<unsigned*>(sm + M::bars + 252);
     // barriers, two of each: chunk i uses number i mod 2, whose phase is then i / 2
-    enum { FULL_A, FULL_B, FULL_C, DONE_P, DONE_X, DONE_T, DONE_O, HAS_C, HAS_P, HAS_W, HAS_O, KINDS };
+    enum { FULL_A, FULL_B, FULL_C, DONE_P, DONE_X, DONE_T, DONE_O, HAS_C, HAS_P, HAS_W, HAS_O, CLEARED, KINDS };
     auto read_p = [&](int quarter) { return bars + (unsigned)(KINDS * 2 + quarter) * 8; };      // P's fp32 columns of these lanes have been read
     auto bar = [&](int kind, int i) { return bars + (unsigned)(kind * 2 + (i & 1)) * 8; };
     auto phase = [](int i) { return (unsigned)(i >> 1) & 1u; };
-    auto at_a = [](int i) { return M::a + i % M::two_ab * M::one; };
-    auto at_b = [](int i) { return M::b + i % M::two_ab * M::one; };
-    auto at_c = [](int i) { return M::c + i % M::two_c * M::one; };
+    auto at_a = [](int i) { return M::a + i % M::two_ac * M::one; };
+    auto at_b = [](int i) { return M::b + i % M::two_b * M::one; };
+    auto at_c = [](int i) { return M::c + i % M::two_ac * M::one; };
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int seg = blockIdx.x % s.segments, bh = blockIdx.x / s.segments, head = bh % s.h, bat = bh / s.h;
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
         *dead = 0;
         for (int i = 0; i < 2; ++i) {
             for (int k = FULL_A; k <= DONE_O; ++k) bar_init(bar(k, i), 1);
-            for (int k = HAS_C; k <= HAS_O; ++k) bar_init(bar(k, i), kWorkers);
+            for (int k = HAS_C; k <= CLEARED; ++k) bar_init(bar(k, i), kWorkers);
         }
         for (int k = 0; k < 4; ++k) bar_init(read_p(k), kWorkers / 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -163,13 +163,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
                 const int t0 = token0(i);
                 auto take = [&](int full, int done, int room, const CUtensorMap* map, const Rows& r, int to) {
                     if (i >= room && !bar_wait(bar(done, i - room), phase(i - room), dead)) return false;
+                    if (i >= room && full == FULL_C && !bar_wait(bar(HAS_C, i - room), phase(i - room), dead)) return false;
                     bar_expect(bar(full, i), M::one);
                     for (int x = 0; x < NB; ++x) tma_load(base + to + x * kBlk, map, x * 64, r.sh ? head : 0, t0, r.sb ? bat : 0, bar(full, i));
                     return true;
                 };
-                if (OUT && !take(FULL_A, DONE_X, M::two_ab, &map_a, s.a, at_a(i))) break;
-                if (!take(FULL_B, DONE_T, M::two_ab, &map_b, s.b, at_b(i))) break;
-                if (!take(FULL_C, OUT ? DONE_O : DONE_T, M::two_c, &map_c, s.c, at_c(i))) break;
+                // in the order in which room comes free: b two chunks ago, a after X, c after O (and its parts, which O waits for)
+                if (!take(FULL_B, DONE_T, M::two_b, &map_b, s.b, at_b(i))) break;
+                if (OUT && !take(FULL_A, DONE_X, M::two_ac, &map_a, s.a, at_a(i))) break;
+                if (!take(FULL_C, OUT ? DONE_O : DONE_T, M::two_ac, &map_c, s.c, at_c(i))) break;
             }
             if (*dead) {                                         // what was asked for has to land before the block leaves
                 for (int j = max(0, i - 2); j <= min(i, chunks - 1); ++j)
@@ -187,7 +189,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
                 const unsigned A = base + at_a(i), B = base + at_b(i), C = base + at_c(i), W = base + M::w, Q = base + M::parts;
                 if constexpr (OUT) {
                     if (!bar_wait(bar(FULL_A, i), ph, dead) || !bar_wait(bar(FULL_B, i), ph, dead)) break;
-                    if (cut && !bar_wait(bar(HAS_C, i), ph, dead)) break;
+                    if (cut && !bar_wait(bar(CLEARED, i), 0, dead)) break;          // once in a sweep
                     if (i > 0 && !bar_wait(bar(DONE_O, i - 1), phase(i - 1), dead)) break;       // O has read the P before
                     tc_after();
 #pragma unroll
@@ -209,6 +211,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
                         for (int k = 0; k < 4; ++k) tc_mma(tX, operand(A + k * 32, 16, 1024), operand(W + kBlk / 2 + k * 32, 16, 1024), product(D, 0, 0), true);
                     }
                     tc_commit(bar(DONE_X, i));
+                    if (!bar_wait(bar(HAS_P, i), ph, dead) || !bar_wait(bar(FULL_C, i), ph, dead)) break;
+                    tc_after();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) tc_mma_t(tO, tP + k * 8, operand(C + k * 2048, kBlk, 1024), product(D, 0, 1), k > 0);
+                    tc_commit(bar(DONE_O, i));
                 } else {
                     if (!bar_wait(bar(FULL_B, i), ph, dead)) break;
                     if (i > 0 && !bar_wait(bar(HAS_W, i - 1), phase(i - 1), dead)) break;       // T has been read
@@ -222,13 +229,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
                     for (int k = 0; k < 8; ++k)
                         tc_mma(tT, operand(Q + p * 2 * kBlk + k * 2048, kBlk, 1024), operand(B + k * 2048, kBlk, 1024), product(D, 1, 1), p < (D == 128 ? PARTS : PARTS - 1) - 1 || k > 0);
                 tc_commit(bar(DONE_T, i));
-                if constexpr (OUT) {
-                    if (!bar_wait(bar(HAS_P, i), ph, dead)) break;
-                    tc_after();
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) tc_mma_t(tO, tP + k * 8, operand(C + k * 2048, kBlk, 1024), product(D, 0, 1), k > 0);
-                    tc_commit(bar(DONE_O, i));
-                }
             }
             if (*dead) {                                         // products under way end before the tensor memory goes
                 tc_commit(bar(DONE_P, 0));
@@ -303,49 +303,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
             for (int x = tid; x < kBlk / 16; x += kAll) reinterpret_cast<uint4*>(sm + M::parts + 3 * kBlk)[x] = make_uint4(0, 0, 0, 0);
             fence_async();
         }
+        const long long by = (long long)s.h * dc;
+        __nv_bfloat16* first_out = (__nv_bfloat16*)s.out + ((long long)bat * s.t * s.h + head) * dc + wcol;
+        const bool wide = dc % 16 == 0 && (reinterpret_cast<size_t>(s.out) & 31) == 0;       // rows of whole 32-byte sectors
         asm volatile("bar.sync 1, %0;" ::"n"(kAll) : "memory");  // the tables
         if (OUT && chunks > 0) put_w(0);
 
         for (int i = 0; i < chunks; ++i) {
             const unsigned ph = phase(i);
             const int left = hi - lo - i * kTok, m = left < kTok ? left : kTok;
-            // the weighted c in parts
-            if (!bar_wait(bar(FULL_C, i), ph, dead)) break;
-            const bool cut = m < kTok && !s.reversed;
-            if (m < kTok) weigh(m);
-            if (cut && (!bar_wait(bar(FULL_B, i), ph, dead) || (OUT && !bar_wait(bar(FULL_A, i), ph, dead)))) break;
-#pragma unroll
-            for (int x = 0; x < NB; ++x)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const int off = x * kBlk + (tid + kAll * k) * 16;
-                    uint4 v = *reinterpret_cast<const uint4*>(sm + at_c(i) + off);
-                    if (cut && prow + 64 * k >= m) {             // rows behind the end: nothing, whatever they hold
-                        v = make_uint4(0, 0, 0, 0);
-                        *reinterpret_cast<uint4*>(sm + at_c(i) + off) = v;
-                        *reinterpret_cast<uint4*>(sm + at_b(i) + off) = v;
-                        if (OUT) *reinterpret_cast<uint4*>(sm + at_a(i) + off) = v;
+            if (m < kTok && !s.reversed) {                       // rows behind the end become nothing, whatever they hold
+                if (!bar_wait(bar(FULL_B, i), ph, dead) || !bar_wait(bar(FULL_C, i), ph, dead) || (OUT && !bar_wait(bar(FULL_A, i), ph, dead))) break;
+                for (int e = tid; e < M::one / 16; e += kAll)
+                    if ((e >> 3 & 127) >= m) {
+                        *reinterpret_cast<uint4*>(sm + at_b(i) + e * 16) = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4*>(sm + at_c(i) + e * 16) = make_uint4(0, 0, 0, 0);
+                        if (OUT) *reinterpret_cast<uint4*>(sm + at_a(i) + e * 16) = make_uint4(0, 0, 0, 0);
                     }
-                    unsigned in[4] = {v.x, v.y, v.z, v.w}, part[PARTS][4];
-                    const float2 f = make_float2(wt[k], wt[k]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float2 y = __fmul2_rn(unpack2(in[e], __nv_bfloat16()), f);
-#pragma unroll
-                        for (int p = 0; p < PARTS; ++p) {
-                            part[p][e] = pack2<__nv_bfloat16>(y.x, y.y);
-                            if (p + 1 < PARTS) {
-                                const float2 z = unpack2(part[p][e], __nv_bfloat16());
-                                y = __fadd2_rn(y, make_float2(-z.x, -z.y));
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int p = 0; p < PARTS; ++p)
-                        *reinterpret_cast<uint4*>(sm + M::parts + p * M::one + off) = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
-                }
-            fence_async();
-            tell(HAS_C, i);
+                fence_async();
+                tell(CLEARED, i);
+            }
             if constexpr (OUT) {
                 // P: weights and mask; back into tensor memory, two columns in one, once the four warps of these lanes have read it
                 if (!bar_wait(bar(DONE_P, i), ph, dead)) break;
@@ -383,30 +360,41 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
                 tc_wait_store();
                 tell(HAS_P, i);
             }
-            // W^T <- l^m W^T + T
-            if (!bar_wait(bar(DONE_T, i), ph, dead)) break;
-            tc_after();
-            {
-                const float keep = m < kTok ? power(ld, m) : keep_full;
-                unsigned r[HC];
-                tc_load(tT + lanes + wcol, r);
-                tc_wait_load();
+            // the weighted c in parts
+            if (!bar_wait(bar(FULL_C, i), ph, dead)) break;
+            if (m < kTok) weigh(m);
 #pragma unroll
-                for (int x = 0; x < HC / 2; ++x) w[x] = __ffma2_rn(make_float2(keep, keep), w[x], make_float2(__uint_as_float(r[2 * x]), __uint_as_float(r[2 * x + 1])));
-            }
+            for (int x = 0; x < NB; ++x)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int off = x * kBlk + (tid + kAll * k) * 16;
+                    const uint4 v = *reinterpret_cast<const uint4*>(sm + at_c(i) + off);
+                    unsigned in[4] = {v.x, v.y, v.z, v.w}, part[PARTS][4];
+                    const float2 f = make_float2(wt[k], wt[k]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float2 y = __fmul2_rn(unpack2(in[e], __nv_bfloat16()), f);
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p) {
+                            part[p][e] = pack2<__nv_bfloat16>(y.x, y.y);
+                            if (p + 1 < PARTS) {
+                                const float2 z = unpack2(part[p][e], __nv_bfloat16());
+                                y = __fadd2_rn(y, make_float2(-z.x, -z.y));
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p)
+                        *reinterpret_cast<uint4*>(sm + M::parts + p * M::one + off) = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
+                }
+            fence_async();
+            tell(HAS_C, i);
             if constexpr (OUT) {
-                if (!bar_wait(bar(DONE_X, i), ph, dead)) break;
-                if (i + 1 < chunks) put_w(i + 1);
                 // out = l^{pos + off} X + O
-                if (!bar_wait(bar(DONE_O, i), ph, dead)) break;
+                if (!bar_wait(bar(DONE_X, i), ph, dead) || !bar_wait(bar(DONE_O, i), ph, dead)) break;
                 tc_after();
-                // the warp's 32 rows turn in shared memory (the pieces of the parts that only this warp writes: T has been summed),
-                // so that neighbouring lanes store neighbouring 16 bytes
-                constexpr int kPieces = HC / 8, kRows = 512 / (HC * 2);            // 16-byte pieces of a row; rows in 512 bytes
-                auto turn = [&](int r, int x) {
-                    const int c = r / kRows, in = r % kRows * HC * 2 + ((x ^ (kPieces == 4 ? r >> 1 & 3 : r >> 2 & 1)) << 4);
-                    return sm + M::parts + (c >> 1) * kBlk + (c & 1) * (kAll * 16) + warp * 512 + in;
-                };
+                const bool live = pos < m;
+                __nv_bfloat16* out = first_out + (token0(i) + row) * by;
 #pragma unroll
                 for (int y = 0; y < HC / 16; ++y) {
                     unsigned r1[16], r2[16];
@@ -418,22 +406,32 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
 #pragma unroll
                     for (int x = 0; x < 8; ++x)
                         v[x] = __ffma2_rn(make_float2(far, far), make_float2(__uint_as_float(r1[2 * x]), __uint_as_float(r1[2 * x + 1])), make_float2(__uint_as_float(r2[2 * x]), __uint_as_float(r2[2 * x + 1])));
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) *reinterpret_cast<uint4*>(turn(lane, y * 2 + x)) = four(v + 4 * x);
+                    const uint4 lo8 = four(v), hi8 = four(v + 4);
+                    __nv_bfloat16* at = out + y * 16;
+                    if (live && wide) {
+                        if (wcol + y * 16 < dc)
+                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(at), "r"(lo8.x), "r"(lo8.y), "r"(lo8.z), "r"(lo8.w), "r"(hi8.x), "r"(hi8.y), "r"(hi8.z), "r"(hi8.w) : "memory");
+                    } else if (live) {
+                        if (wcol + y * 16 < dc) *reinterpret_cast<uint4*>(at) = lo8;
+                        if (wcol + y * 16 + 8 < dc) *reinterpret_cast<uint4*>(at + 8) = hi8;
+                    }
                 }
-                __syncwarp();
-                const int r0 = lane / kPieces, x0 = lane % kPieces;
-                const long long by = (long long)s.h * dc;
-                __nv_bfloat16* out = (__nv_bfloat16*)s.out + ((long long)bat * s.t * s.h + head) * dc + (token0(i) + q * 32 + r0) * by + wcol + x0 * 8;
+            }
+            // W^T <- l^m W^T + T
+            if (!bar_wait(bar(DONE_T, i), ph, dead)) break;
+            tc_after();
+            {
+                const float keep = m < kTok ? power(ld, m) : keep_full;
+                unsigned r[HC];
+                tc_load(tT + lanes + wcol, r);
+                tc_wait_load();
 #pragma unroll
-                for (int y = 0; y < kPieces; ++y) {
-                    constexpr int kEach = 32 / kPieces;
-                    const int r = q * 32 + r0 + y * kEach;
-                    if ((s.reversed ? kTok - 1 - r : r) < m && wcol + x0 * 8 < dc)
-                        *reinterpret_cast<uint4*>(out + y * kEach * by) = *reinterpret_cast<const uint4*>(turn(r0 + y * kEach, x0));
-                }
-                __syncwarp();
-            } else if (i + 1 < chunks) tell(HAS_W, i);
+                for (int x = 0; x < HC / 2; ++x) w[x] = __ffma2_rn(make_float2(keep, keep), w[x], make_float2(__uint_as_float(r[2 * x]), __uint_as_float(r[2 * x + 1])));
+            }
+            if (i + 1 < chunks) {
+                if constexpr (OUT) put_w(i + 1);                 // X has read the last one: waited for above
+                else tell(HAS_W, i);
+            }
         }
         if (s.end) {
             float* w1 = s.end + ((long long)bh * s.segments + seg) * size;
