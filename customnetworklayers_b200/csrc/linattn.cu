@@ -282,9 +282,10 @@ int segment_plan(int b, int t, int h, int dk, int dv, int dtype, int* segments, 
     int sms = 0;
     CNL_TRY(sm_count(&sms));
     const int d = dk > dv ? dk : dv;
-    const long long heads = (long long)b * h > 0 ? (long long)b * h : 1;
+    const bool tc = tc_sizes(t, dk, dv, dtype);
+    const long long heads = ((long long)b * h > 0 ? (long long)b * h : 1) * (tc && d > 64 ? 2 : 1);       // the tcgen05 sweep takes 64 columns a block
     // blocks that an SM holds of the kernel that serves these sizes
-    const int each = dtype == CNL_F32 ? (d > 64 ? 1 : 4) : tc_sizes(t, dk, dv, dtype) ? 1 : d > 64 ? 2 : d > 32 ? 4 : 8;
+    const int each = dtype == CNL_F32 ? (d > 64 ? 1 : 4) : tc ? 1 : d > 64 ? 2 : d > 32 ? 4 : 8;
     const long long places = (long long)sms * each, most = (t + 127) / 128;
     long long best = 0;
     *segments = 1;

@@ -1,20 +1,21 @@
 // Linear attention sweep for bf16 on the fifth-generation tensor cores (formulas: linattn.cuh).
 //
-// A block of 18 warps walks one segment of one head in chunks of 128 tokens.  One warp brings a, b, c rows by TMA (128-byte
-// swizzle), one thread issues the products, sixteen warps do what lies between.  Per chunk, accumulators in tensor memory:
+// A block of 18 warps walks one segment of one head, and 64 columns of its outputs, in chunks of 128 tokens.  One warp brings
+// a, b, c rows by TMA (128-byte swizzle), one thread issues the products, sixteen warps do what lies between.  Per chunk,
+// accumulators in tensor memory:
 //     P = a b^T                 [128 tokens x 128 tokens]   -> weighted, masked, rounded, put back in tensor memory
-//     X = a W                   [128 tokens x dc]           W as the sweep has it before the chunk
-//     O = P c                   [128 tokens x dc]
-//     T = (weighted c)^T b      [dc x da]                   what the chunk adds to W^T
-// and in registers W^T <- l^m W^T + T (fp32), out = l^{pos + off} X + O.  Nothing of the recurrence passes through the tensor
-// cores: T needs only the chunk's own rows, so the products of a chunk run while the warps finish the one before.
+//     X = a (W0 | W1)           [128 tokens x 64 + 64]      W as the sweep has it before the chunk, in two addends
+//     O = P c                   [128 tokens x 64]
+//     T = (c0 | c1)^T b         [64 + 64 x da]              what the chunk adds to W^T; c0, c1: the weighted c in two parts
+// and in registers W^T <- l^m W^T + T (fp32, both addends), out = l^{pos + off} (X0 + X1) + O.  Nothing of the recurrence
+// passes through the tensor cores: T needs only the chunk's own rows, so it is summed while the outputs are finished.
 // Reversed sweeps take the tokens of a chunk in their order in memory and turn the mask and the weights around instead.
 //
-// Operands: a and b for P, P, and W lie with the summed dimension contiguous; c and the weighted c, and b for T, with it
-// strided (their rows are tokens), which the descriptors say.  Heads of up to 64 fill 128 rows of T with the two parts of
-// the weighted c (first part: rows 0..63, what it leaves out: rows 64..127), so the state is kept as two addends and both
-// meet a in X; heads of up to 128 add the parts in T.  Roundings: as in the mma.sync kernel (P once, W once, the weighted c
-// to 16 or, where the state is a result, 24 bits).
+// Operands: a and b for P, P, and W lie with the summed dimension contiguous; c, its parts, and b for T with it strided
+// (their rows are tokens), which the descriptors say.  64 columns fill the 128 rows of T with both parts of the weighted c,
+// and twice the blocks leave fewer and longer segments: at 64 heads of 128 none is cut, which saves the pass for the states.
+// Reads of shared memory bound the products (128 x 128 x 16 reads 8 KB), so a is read once for both addends of W.
+// Roundings: as in the mma.sync kernel (P once, W once, the weighted c to 16 or, where the state is a result, 24 bits).
 //
 // Every wait is bounded: a block that gives up marks the status word, fills what it owes with NaN, and returns after its
 // copies and products have ended.
@@ -55,6 +56,19 @@ __device__ __forceinline__ bool bar_wait(unsigned bar, unsigned parity, volatile
 __device__ __forceinline__ void tma_load(unsigned to, const CUtensorMap* map, int x, int h, int t, int b, unsigned bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to), "l"(map), "r"(x), "r"(h), "r"(t), "r"(b), "r"(bar) : "memory");
 }
+// 16 bytes of shared memory by address: a generic pointer, which alignment by hand leaves, would cost the slower path
+__device__ __forceinline__ uint4 smem_get(unsigned at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void smem_put(unsigned at, uint4 v) { asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory"); }
+__device__ __forceinline__ void smem_put(unsigned at, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
+__device__ __forceinline__ float smem_get1(unsigned at) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -83,56 +97,66 @@ __device__ __forceinline__ void tc_store(unsigned at, const unsigned (&r)[16]) {
 __device__ __forceinline__ void tc_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-// Descriptor of an operand in shared memory, 128-byte swizzle.  Summed dimension contiguous: `step` is the distance of
-// groups of 8 rows.  Summed dimension strided: `step` that of groups of 8 summed rows, `block` that of 64-element columns.
-__device__ __forceinline__ unsigned long long operand(unsigned at, unsigned block, unsigned step) {
-    return (unsigned long long)((at & 0x3ffffu) >> 4) | (unsigned long long)(block >> 4) << 16 | (unsigned long long)(step >> 4) << 32 | 1ULL << 46 | 2ULL << 61;
+// Descriptor of an operand in shared memory, 128-byte swizzle, groups of 8 rows 1024 bytes apart.  Its upper word is the same
+// for all; the lower one is the address, and with the summed dimension strided the distance of 64-element columns.  Products
+// differ by a constant in it: built anew for every product, and by one lane on its own, the descriptors cost 150 to 200 clocks
+// a product, where the product itself takes 43 + n / 2 (10 + n / 2 with the rows' operand in tensor memory), measured.
+__device__ __forceinline__ unsigned rows_word(unsigned at) { return (at & 0x3ffffu) >> 4 | 1u << 16; }
+__device__ __forceinline__ unsigned columns_word(unsigned at) { return (at & 0x3ffffu) >> 4 | (unsigned)(kBlk >> 4) << 16; }
+__device__ __forceinline__ unsigned long long operand(unsigned word, int further) {
+    return (unsigned long long)(1024u >> 4 | 1u << 14 | 2u << 29) << 32 | (word + (unsigned)(further >> 4));
+}
+__device__ __forceinline__ bool elected() {                     // one lane of the warp
+    unsigned one;
+    asm volatile("{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\nselp.u32 %0, 1, 0, q;\n}" : "=r"(one));
+    return one != 0;
 }
 // Instruction word: fp32 sums of bf16 products, 128 rows, n columns; strided a / b
 __host__ __device__ constexpr unsigned product(int n, int strided_a, int strided_b) {
     return 1u << 4 | 1u << 7 | 1u << 10 | (unsigned)strided_a << 15 | (unsigned)strided_b << 16 | (unsigned)(n >> 3) << 17 | 8u << 24;
 }
 
-template <int D, bool OUT, int PARTS>
+constexpr int kCols = 64;                       // output columns of a block
+
+template <int DA, bool OUT, int PARTS>
 struct Map {                                    // shared memory in bytes from a 1024-byte boundary
-    static constexpr int nb = D / 64, one = nb * kBlk;           // one operand's rows
-    // heads of 128 with outputs leave no room for two of everything: b is held longest, so it has two
-    static constexpr int two_ac = D == 64 || !OUT ? 2 : 1, two_b = 2;
-    static constexpr int a = 0, b = a + (OUT ? two_ac * one : 0), c = b + two_b * one, w = c + two_ac * one;
-    static constexpr int parts = w + (OUT ? (D == 128 ? 2 * kBlk : kBlk) : 0);
-    static constexpr int part_blocks = D == 128 ? 2 * PARTS : PARTS == 3 ? 4 : 2;
-    static constexpr int tables = parts + part_blocks * kBlk;    // powers of the decay for P: 32 for whole tiles, 64 for diagonal ones
-    static constexpr int bars = tables + 96 * 4;
+    static constexpr int nb = DA / 64, one = nb * kBlk;          // a's or b's rows; c's are kBlk
+    static constexpr int two_a = DA == 128 && PARTS == 3 ? 1 : 2, two = 2;         // rooms for a; for b and c
+    static constexpr int a = 0, b = a + (OUT ? two_a * one : 0), c = b + two * one, w = c + two * kBlk;
+    static constexpr int parts = w + (OUT ? one : 0), part_blocks = PARTS == 3 ? 4 : 2;
+    static constexpr int bars = parts + part_blocks * kBlk;
     static constexpr int bytes = bars + 256 + 1024;              // and the way to the boundary
 };
 
 // ---- the sweep -----------------------------------------------------------------------------------------------------
-template <int D, bool OUT, int PARTS>
+template <int DA, bool OUT, int PARTS>
 __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                            const __grid_constant__ CUtensorMap map_c) {
-    using M = Map<D, OUT, PARTS>;
+    using M = Map<DA, OUT, PARTS>;
     constexpr int NB = M::nb;
     extern __shared__ unsigned char raw[];
-    unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<size_t>(raw) + 1023) & ~(size_t)1023);
-    const unsigned base = smem_at(sm), bars = base + M::bars;
-    volatile int* dead = reinterpret_cast<volatile int*>(sm + M::bars + 248);
-    unsigned* tmem_word = reinterpret_cast<unsigned*>(sm + M::bars + 252);
+    __shared__ float whole[32], edge[64];                        // powers of the decay for P: for whole tiles, for diagonal ones
+    __shared__ int dead_word;
+    __shared__ unsigned tmem_word;
+    const unsigned base = (smem_at(raw) + 1023u) & ~1023u, bars = base + M::bars;
+    volatile int* dead = &dead_word;
     // barriers, two of each: chunk i uses number i mod 2, whose phase is then i / 2
     enum { FULL_A, FULL_B, FULL_C, DONE_P, DONE_X, DONE_T, DONE_O, HAS_C, HAS_P, HAS_W, HAS_O, CLEARED, KINDS };
     auto read_p = [&](int quarter) { return bars + (unsigned)(KINDS * 2 + quarter) * 8; };      // P's fp32 columns of these lanes have been read
     auto bar = [&](int kind, int i) { return bars + (unsigned)(kind * 2 + (i & 1)) * 8; };
     auto phase = [](int i) { return (unsigned)(i >> 1) & 1u; };
-    auto at_a = [](int i) { return M::a + i % M::two_ac * M::one; };
-    auto at_b = [](int i) { return M::b + i % M::two_b * M::one; };
-    auto at_c = [](int i) { return M::c + i % M::two_ac * M::one; };
+    auto at_a = [](int i) { return M::a + i % M::two_a * M::one; };
+    auto at_b = [](int i) { return M::b + i % M::two * M::one; };
+    auto at_c = [](int i) { return M::c + i % M::two * kBlk; };
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int seg = blockIdx.x % s.segments, bh = blockIdx.x / s.segments, head = bh % s.h, bat = bh / s.h;
+    const int halves = s.dc > kCols ? 2 : 1;
+    const int seg = blockIdx.x % s.segments, col0 = blockIdx.x / s.segments % halves * kCols, bh = blockIdx.x / s.segments / halves, head = bh % s.h, bat = bh / s.h;
     const int n = s.lengths ? min(max(s.lengths[bat], 0), s.t) : s.t;
     const long long first = (long long)seg * s.seg;
     const int lo = (int)(first < n ? first : n), hi = (int)(first + s.seg < n ? first + s.seg : n);
     const int chunks = (hi - lo + kTok - 1) / kTok;
-    const int da = s.da, dc = s.dc;
+    const int da = s.da, dc = s.dc, cols = min(dc - col0, kCols);
     const long long size = (long long)da * dc;
     // first token of chunk i; positions lo + 128 i ... of the sweep
     auto token0 = [&](int i) { return s.reversed ? n - (lo + i * kTok) - kTok : lo + i * kTok; };
@@ -147,13 +171,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kWorkers + 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_at(tmem_word)) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_at(&tmem_word)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         tc_before();
     }
     __syncthreads();
     tc_after();
-    const unsigned tmem = *tmem_word, tP = tmem, tX = tmem + 128, tO = tmem + 256, tT = tmem + 384;
+    const unsigned tmem = tmem_word, tP = tmem, tX = tmem + 128, tO = tmem + 256, tT = tmem + 320;
 
     if (warp == kWorkers) {
         // ---- rows arrive
@@ -161,17 +185,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
             int i = 0;
             for (; i < chunks; ++i) {
                 const int t0 = token0(i);
-                auto take = [&](int full, int done, int room, const CUtensorMap* map, const Rows& r, int to) {
+                auto take = [&](int full, int done, int room, const CUtensorMap* map, const Rows& r, int to, int x0, int blocks) {
                     if (i >= room && !bar_wait(bar(done, i - room), phase(i - room), dead)) return false;
                     if (i >= room && full == FULL_C && !bar_wait(bar(HAS_C, i - room), phase(i - room), dead)) return false;
-                    bar_expect(bar(full, i), M::one);
-                    for (int x = 0; x < NB; ++x) tma_load(base + to + x * kBlk, map, x * 64, r.sh ? head : 0, t0, r.sb ? bat : 0, bar(full, i));
+                    bar_expect(bar(full, i), blocks * kBlk);
+                    for (int x = 0; x < blocks; ++x) tma_load(base + to + x * kBlk, map, x0 + x * 64, r.sh ? head : 0, t0, r.sb ? bat : 0, bar(full, i));
                     return true;
                 };
-                // in the order in which room comes free: b two chunks ago, a after X, c after O (and its parts, which O waits for)
-                if (!take(FULL_B, DONE_T, M::two_b, &map_b, s.b, at_b(i))) break;
-                if (OUT && !take(FULL_A, DONE_X, M::two_ac, &map_a, s.a, at_a(i))) break;
-                if (!take(FULL_C, OUT ? DONE_O : DONE_T, M::two_ac, &map_c, s.c, at_c(i))) break;
+                // room comes free: b after T, a after X, c after O and its parts
+                if (!take(FULL_B, DONE_T, M::two, &map_b, s.b, at_b(i), 0, NB)) break;
+                if (OUT && !take(FULL_A, DONE_X, M::two_a, &map_a, s.a, at_a(i), 0, NB)) break;
+                if (!take(FULL_C, OUT ? DONE_O : DONE_T, M::two, &map_c, s.c, at_c(i), col0, 1)) break;
             }
             if (*dead) {                                         // what was asked for has to land before the block leaves
                 for (int j = max(0, i - 2); j <= min(i, chunks - 1); ++j)
@@ -181,65 +205,66 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
         }
         __syncwarp();
     } else if (warp == kWorkers + 1) {
-        // ---- products
-        if (lane == 0) {
-            for (int i = 0; i < chunks; ++i) {
-                const unsigned ph = phase(i);
-                const bool cut = hi - lo - i * kTok < kTok && !s.reversed;       // rows behind the end are cleared first
-                const unsigned A = base + at_a(i), B = base + at_b(i), C = base + at_c(i), W = base + M::w, Q = base + M::parts;
-                if constexpr (OUT) {
-                    if (!bar_wait(bar(FULL_A, i), ph, dead) || !bar_wait(bar(FULL_B, i), ph, dead)) break;
-                    if (cut && !bar_wait(bar(CLEARED, i), 0, dead)) break;          // once in a sweep
-                    if (i > 0 && !bar_wait(bar(DONE_O, i - 1), phase(i - 1), dead)) break;       // O has read the P before
-                    tc_after();
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const unsigned o = (k / 4) * kBlk + (k % 4) * 32;
-                        tc_mma(tP, operand(A + o, 16, 1024), operand(B + o, 16, 1024), product(128, 0, 0), k > 0);
-                    }
-                    tc_commit(bar(DONE_P, i));
-                    if (!bar_wait(bar(HAS_W, i), ph, dead)) break;
-                    if (i > 0 && !bar_wait(bar(HAS_O, i - 1), phase(i - 1), dead)) break;
-                    tc_after();
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const unsigned o = (k / 4) * kBlk + (k % 4) * 32;
-                        tc_mma(tX, operand(A + o, 16, 1024), operand(W + o, 16, 1024), product(D, 0, 0), k > 0);
-                    }
-                    if constexpr (D == 64) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) tc_mma(tX, operand(A + k * 32, 16, 1024), operand(W + kBlk / 2 + k * 32, 16, 1024), product(D, 0, 0), true);
-                    }
-                    tc_commit(bar(DONE_X, i));
-                    if (!bar_wait(bar(HAS_P, i), ph, dead) || !bar_wait(bar(FULL_C, i), ph, dead)) break;
-                    tc_after();
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) tc_mma_t(tO, tP + k * 8, operand(C + k * 2048, kBlk, 1024), product(D, 0, 1), k > 0);
-                    tc_commit(bar(DONE_O, i));
-                } else {
-                    if (!bar_wait(bar(FULL_B, i), ph, dead)) break;
-                    if (i > 0 && !bar_wait(bar(HAS_W, i - 1), phase(i - 1), dead)) break;       // T has been read
-                }
-                if (!bar_wait(bar(HAS_C, i), ph, dead)) break;
+        // ---- products.  The warp runs as one, so that what the products are given is uniform; one lane issues them
+        const bool one = elected();
+        const unsigned W = rows_word(base + M::w), Q = columns_word(base + M::parts);
+        for (int i = 0; i < chunks; ++i) {
+            const unsigned ph = phase(i);
+            const bool cut = hi - lo - i * kTok < kTok && !s.reversed;       // rows behind the end are cleared first
+            const unsigned A = rows_word(base + at_a(i)), B = rows_word(base + at_b(i)), Bt = columns_word(base + at_b(i)), C = columns_word(base + at_c(i));
+            if constexpr (OUT) {
+                if (!bar_wait(bar(FULL_A, i), ph, dead) || !bar_wait(bar(FULL_B, i), ph, dead)) break;
+                if (cut && !bar_wait(bar(CLEARED, i), 0, dead)) break;          // once in a sweep
+                if (i > 0 && !bar_wait(bar(DONE_O, i - 1), phase(i - 1), dead)) break;       // O has read the P before
                 tc_after();
-                // small parts first
+                if (one) {
 #pragma unroll
-                for (int p = (D == 128 ? PARTS : PARTS - 1) - 1; p >= 0; --p)
+                    for (int k = 0; k < DA / 16; ++k) tc_mma(tP, operand(A, (k / 4) * kBlk + (k % 4) * 32), operand(B, (k / 4) * kBlk + (k % 4) * 32), product(128, 0, 0), k > 0);
+                    tc_commit(bar(DONE_P, i));
+                }
+                __syncwarp();
+                if (!bar_wait(bar(HAS_W, i), ph, dead)) break;
+                if (i > 0 && !bar_wait(bar(HAS_O, i - 1), phase(i - 1), dead)) break;
+                tc_after();
+                if (one) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        tc_mma(tT, operand(Q + p * 2 * kBlk + k * 2048, kBlk, 1024), operand(B + k * 2048, kBlk, 1024), product(D, 1, 1), p < (D == 128 ? PARTS : PARTS - 1) - 1 || k > 0);
+                    for (int k = 0; k < DA / 16; ++k) tc_mma(tX, operand(A, (k / 4) * kBlk + (k % 4) * 32), operand(W, (k / 4) * kBlk + (k % 4) * 32), product(128, 0, 0), k > 0);
+                    tc_commit(bar(DONE_X, i));
+                }
+                __syncwarp();
+                if (!bar_wait(bar(HAS_P, i), ph, dead) || !bar_wait(bar(FULL_C, i), ph, dead)) break;
+                tc_after();
+                if (one) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) tc_mma_t(tO, tP + k * 8, operand(C, k * 2048), product(kCols, 0, 1), k > 0);
+                    tc_commit(bar(DONE_O, i));
+                }
+                __syncwarp();
+            } else {
+                if (!bar_wait(bar(FULL_B, i), ph, dead)) break;
+                if (i > 0 && !bar_wait(bar(HAS_W, i - 1), phase(i - 1), dead)) break;       // T has been read
+            }
+            if (!bar_wait(bar(HAS_C, i), ph, dead)) break;
+            tc_after();
+            if (one) {
+                // the third part first
+#pragma unroll
+                for (int p = PARTS - 2; p >= 0; --p)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) tc_mma(tT, operand(Q, p * 2 * kBlk + k * 2048), operand(Bt, k * 2048), product(DA, 1, 1), p < PARTS - 2 || k > 0);
                 tc_commit(bar(DONE_T, i));
             }
-            if (*dead) {                                         // products under way end before the tensor memory goes
-                tc_commit(bar(DONE_P, 0));
-                for (int spin = 0; spin < 4096; ++spin)
-                    if (bar_try(bar(DONE_P, 0), 0) && bar_try(bar(DONE_P, 0), 1)) break;
-            }
+            __syncwarp();
+        }
+        if (*dead) {                                             // products under way end before the tensor memory goes
+            if (one) tc_commit(bar(DONE_P, 0));
+            for (int spin = 0; spin < 4096; ++spin)
+                if (bar_try(bar(DONE_P, 0), 0) && bar_try(bar(DONE_P, 0), 1)) break;
         }
         __syncwarp();
     } else {
         // ---- between the products: warp w holds lanes 32 (w mod 4) .. of tensor memory and a quarter of the columns
-        constexpr int HC = D / 4;                                // columns of X, O and T that a thread holds
+        constexpr int HC = DA / 4;                               // columns of T that a thread holds
         constexpr int kAll = kWorkers * 32;
         const int q = warp & 3, cq = warp >> 2, row = q * 32 + lane;
         const unsigned lanes = (unsigned)(q * 32) << 16;
@@ -248,13 +273,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
         const int pos = s.reversed ? kTok - 1 - row : row;
         const float far = s.out_scale * power(ld, pos + s.off);
         // P: a tile of 32 x 32 that lies off the diagonal weighs u (this thread's) times a row of 32; one on it l^(lane - x)
-        float* whole = reinterpret_cast<float*>(sm + M::tables);
-        float* edge = whole + 32;                                // edge[32 + d] = l^d, 0 for d < 0
         const int behind = s.reversed ? 32 * cq - row : row - 32 * cq - 31;
         const float u = behind > 0 ? both * power(ld, behind) : both;
         if (OUT && tid < 96) {
             if (tid < 32) whole[tid] = power(ld, s.reversed ? tid : 31 - tid);
-            else edge[tid - 32] = tid < 64 ? 0.0f : power(ld, tid - 64);
+            else edge[tid - 32] = tid < 64 ? 0.0f : power(ld, tid - 64);      // edge[32 + d] = l^d, 0 for d < 0
         }
         // weights of the token rows of this thread's pieces: rows tid / 8 and 64 more
         const int prow = tid >> 3;
@@ -267,12 +290,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
             }
         };
         weigh(kTok);
-        // W^T: D = 128: row = column of c; D = 64: rows 0..63 first addend, 64..127 second
-        const int wrow = D == 128 ? row : row & 63, wcol = cq * HC;
+        // W^T: rows 0..63 first addend, 64..127 second
+        const int wrow = col0 + (row & 63), wcol = cq * HC;
         float2 w[HC / 2];
         {
             const float* w0 = s.start ? s.start + ((long long)bh * s.segments + seg) * size : nullptr;
-            const bool has = w0 && wrow < dc && (D == 128 || row < 64);
+            const bool has = w0 && wrow < dc && row < 64;
 #pragma unroll
             for (int x = 0; x < HC; ++x) {
                 const int i = wcol + x;
@@ -291,20 +314,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
         };
         auto put_w = [&](int i) {                                // W as the operand of chunk i
             if constexpr (OUT) {
-                unsigned char* to = sm + M::w + (D == 128 ? (cq >> 1) * kBlk : (row >> 6) * (kBlk / 2)) + wrow * 128;
-                const int piece = D == 128 ? (cq & 1) * 4 : cq * 2;
+                const unsigned to = base + M::w + (DA == 128 ? (cq >> 1) * kBlk : 0) + row * 128;
+                const int piece = DA == 128 ? (cq & 1) * 4 : cq * 2;
 #pragma unroll
-                for (int x = 0; x < HC / 8; ++x) *reinterpret_cast<uint4*>(to + (((piece + x) ^ (wrow & 7)) << 4)) = four(w + 4 * x);
+                for (int x = 0; x < HC / 8; ++x) smem_put(to + (((piece + x) ^ (row & 7)) << 4), four(w + 4 * x));
                 fence_async();
             }
             tell(HAS_W, i);
         };
-        if constexpr (PARTS == 3 && D == 64) {                   // the rows that stand beside the third part
-            for (int x = tid; x < kBlk / 16; x += kAll) reinterpret_cast<uint4*>(sm + M::parts + 3 * kBlk)[x] = make_uint4(0, 0, 0, 0);
+        if constexpr (PARTS == 3) {                   // the rows that stand beside the third part
+            for (int x = tid; x < kBlk / 16; x += kAll) smem_put(base + M::parts + 3 * kBlk + x * 16, make_uint4(0, 0, 0, 0));
             fence_async();
         }
         const long long by = (long long)s.h * dc;
-        __nv_bfloat16* first_out = (__nv_bfloat16*)s.out + ((long long)bat * s.t * s.h + head) * dc + wcol;
+        const int ocol = cq * 16;                                // columns of X0, X1 and O
+        __nv_bfloat16* first_out = (__nv_bfloat16*)s.out + ((long long)bat * s.t * s.h + head) * dc + col0 + ocol;
         const bool wide = dc % 16 == 0 && (reinterpret_cast<size_t>(s.out) & 31) == 0;       // rows of whole 32-byte sectors
         asm volatile("bar.sync 1, %0;" ::"n"(kAll) : "memory");  // the tables
         if (OUT && chunks > 0) put_w(0);
@@ -316,9 +340,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
                 if (!bar_wait(bar(FULL_B, i), ph, dead) || !bar_wait(bar(FULL_C, i), ph, dead) || (OUT && !bar_wait(bar(FULL_A, i), ph, dead))) break;
                 for (int e = tid; e < M::one / 16; e += kAll)
                     if ((e >> 3 & 127) >= m) {
-                        *reinterpret_cast<uint4*>(sm + at_b(i) + e * 16) = make_uint4(0, 0, 0, 0);
-                        *reinterpret_cast<uint4*>(sm + at_c(i) + e * 16) = make_uint4(0, 0, 0, 0);
-                        if (OUT) *reinterpret_cast<uint4*>(sm + at_a(i) + e * 16) = make_uint4(0, 0, 0, 0);
+                        smem_put(base + at_b(i) + e * 16, make_uint4(0, 0, 0, 0));
+                        if (OUT) smem_put(base + at_a(i) + e * 16, make_uint4(0, 0, 0, 0));
+                        if (e < kBlk / 16) smem_put(base + at_c(i) + e * 16, make_uint4(0, 0, 0, 0));
                     }
                 fence_async();
                 tell(CLEARED, i);
@@ -364,11 +388,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
             if (!bar_wait(bar(FULL_C, i), ph, dead)) break;
             if (m < kTok) weigh(m);
 #pragma unroll
-            for (int x = 0; x < NB; ++x)
-#pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    const int off = x * kBlk + (tid + kAll * k) * 16;
-                    const uint4 v = *reinterpret_cast<const uint4*>(sm + at_c(i) + off);
+                    const int off = (tid + kAll * k) * 16;
+                    const uint4 v = smem_get(base + at_c(i) + off);
                     unsigned in[4] = {v.x, v.y, v.z, v.w}, part[PARTS][4];
                     const float2 f = make_float2(wt[k], wt[k]);
 #pragma unroll
@@ -385,7 +407,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
                     }
 #pragma unroll
                     for (int p = 0; p < PARTS; ++p)
-                        *reinterpret_cast<uint4*>(sm + M::parts + p * M::one + off) = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
+                        smem_put(base + M::parts + p * kBlk + off, make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]));
                 }
             fence_async();
             tell(HAS_C, i);
@@ -395,25 +417,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
                 tc_after();
                 const bool live = pos < m;
                 __nv_bfloat16* out = first_out + (token0(i) + row) * by;
-#pragma unroll
-                for (int y = 0; y < HC / 16; ++y) {
-                    unsigned r1[16], r2[16];
-                    tc_load(tX + lanes + wcol + y * 16, r1);
-                    tc_load(tO + lanes + wcol + y * 16, r2);
+                {
+                    unsigned r0[16], r1[16], r2[16];
+                    tc_load(tX + lanes + ocol, r0);
+                    tc_load(tX + lanes + kCols + ocol, r1);
+                    tc_load(tO + lanes + ocol, r2);
                     tc_wait_load();
-                    if (y == HC / 16 - 1) tell(HAS_O, i);
+                    tell(HAS_O, i);
                     float2 v[8];
 #pragma unroll
                     for (int x = 0; x < 8; ++x)
-                        v[x] = __ffma2_rn(make_float2(far, far), make_float2(__uint_as_float(r1[2 * x]), __uint_as_float(r1[2 * x + 1])), make_float2(__uint_as_float(r2[2 * x]), __uint_as_float(r2[2 * x + 1])));
+                        v[x] = __ffma2_rn(make_float2(far, far), __fadd2_rn(make_float2(__uint_as_float(r0[2 * x]), __uint_as_float(r0[2 * x + 1])), make_float2(__uint_as_float(r1[2 * x]), __uint_as_float(r1[2 * x + 1]))),
+                                          make_float2(__uint_as_float(r2[2 * x]), __uint_as_float(r2[2 * x + 1])));
                     const uint4 lo8 = four(v), hi8 = four(v + 4);
-                    __nv_bfloat16* at = out + y * 16;
                     if (live && wide) {
-                        if (wcol + y * 16 < dc)
-                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(at), "r"(lo8.x), "r"(lo8.y), "r"(lo8.z), "r"(lo8.w), "r"(hi8.x), "r"(hi8.y), "r"(hi8.z), "r"(hi8.w) : "memory");
+                        if (ocol < cols)
+                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out), "r"(lo8.x), "r"(lo8.y), "r"(lo8.z), "r"(lo8.w), "r"(hi8.x), "r"(hi8.y), "r"(hi8.z), "r"(hi8.w) : "memory");
                     } else if (live) {
-                        if (wcol + y * 16 < dc) *reinterpret_cast<uint4*>(at) = lo8;
-                        if (wcol + y * 16 + 8 < dc) *reinterpret_cast<uint4*>(at + 8) = hi8;
+                        if (ocol < cols) *reinterpret_cast<uint4*>(out) = lo8;
+                        if (ocol + 8 < cols) *reinterpret_cast<uint4*>(out + 8) = hi8;
                     }
                 }
             }
@@ -435,25 +457,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
         }
         if (s.end) {
             float* w1 = s.end + ((long long)bh * s.segments + seg) * size;
-            if constexpr (D == 64) {                             // the two addends meet in shared memory (the parts' room)
-                asm volatile("bar.sync 1, %0;" ::"n"(kAll) : "memory");
-                float* meet = reinterpret_cast<float*>(sm + M::parts);
-                if (row >= 64)
+            asm volatile("bar.sync 1, %0;" ::"n"(kAll) : "memory");
+            const unsigned meet = base + M::parts + (row & 63) * 4;        // the two addends meet in the parts' room
+            if (row >= 64)
 #pragma unroll
-                    for (int x = 0; x < HC / 2; ++x) {
-                        meet[(wcol + 2 * x) * 64 + wrow] = w[x].x;
-                        meet[(wcol + 2 * x + 1) * 64 + wrow] = w[x].y;
-                    }
-                asm volatile("bar.sync 1, %0;" ::"n"(kAll) : "memory");
-                if (row < 64)
+                for (int x = 0; x < HC / 2; ++x) {
+                    smem_put(meet + (wcol + 2 * x) * 256, w[x].x);
+                    smem_put(meet + (wcol + 2 * x + 1) * 256, w[x].y);
+                }
+            asm volatile("bar.sync 1, %0;" ::"n"(kAll) : "memory");
+            if (row < 64)
 #pragma unroll
-                    for (int x = 0; x < HC / 2; ++x) {
-                        w[x].x += meet[(wcol + 2 * x) * 64 + wrow];
-                        w[x].y += meet[(wcol + 2 * x + 1) * 64 + wrow];
-                    }
-            }
+                for (int x = 0; x < HC / 2; ++x) {
+                    w[x].x += smem_get1(meet + (wcol + 2 * x) * 256);
+                    w[x].y += smem_get1(meet + (wcol + 2 * x + 1) * 256);
+                }
             const bool lost = *dead != 0;
-            if (wrow < dc && (D == 128 || row < 64))
+            if (wrow < dc && row < 64)
 #pragma unroll
                 for (int x = 0; x < HC; ++x)
                     if (wcol + x < da) w1[(long long)(wcol + x) * dc + wrow] = lost ? __uint_as_float(0x7fffffffu) : x & 1 ? w[x / 2].y : w[x / 2].x;
@@ -467,9 +487,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
     if (lost && tid == 0) g_gave_up = 1;
     if constexpr (OUT) {                                         // rows behind the sequence's end; all rows of a block that gave up
         const long long zlo = lost ? lo : (first > n ? first : n), zhi = first + s.seg < s.t ? first + s.seg : s.t;
-        for (long long e = zlo * dc + tid; e < zhi * dc; e += kTcThreads) {
-            const long long i = e / dc, tok = i < n && s.reversed ? n - 1 - i : i;
-            ((__nv_bfloat16*)s.out)[(((long long)bat * s.t + tok) * s.h + head) * dc + (e - i * dc)] = from_f32<__nv_bfloat16>(i < n ? __uint_as_float(0x7fffffffu) : 0.0f);
+        for (long long e = zlo * cols + tid; e < zhi * cols; e += kTcThreads) {
+            const long long i = e / cols, tok = i < n && s.reversed ? n - 1 - i : i;
+            ((__nv_bfloat16*)s.out)[(((long long)bat * s.t + tok) * s.h + head) * dc + col0 + (e - i * cols)] = from_f32<__nv_bfloat16>(i < n ? __uint_as_float(0x7fffffffu) : 0.0f);
         }
     }
 }
@@ -508,29 +528,24 @@ int encode(CUtensorMap* map, const Rows& r, int b, int t, int h, int d) {
     return CNL_OK;
 }
 
-template <int D, bool OUT, int PARTS>
+template <int DA, bool OUT, int PARTS>
 int launch_tc(const Sweep& s, cudaStream_t st) {
     CUtensorMap a = {}, b, c;
     if (OUT) CNL_TRY(encode(&a, s.a, s.batch, s.t, s.h, s.da));
     CNL_TRY(encode(&b, s.b, s.batch, s.t, s.h, s.da));
     CNL_TRY(encode(&c, s.c, s.batch, s.t, s.h, s.dc));
-    constexpr int bytes = Map<D, OUT, PARTS>::bytes;
+    constexpr int bytes = Map<DA, OUT, PARTS>::bytes;
     static_assert(bytes <= 232448, "more shared memory than a block may have");
-    CNL_TRY(ensure_dynamic_smem(tc_kernel<D, OUT, PARTS>, bytes));
-    tc_kernel<D, OUT, PARTS><<<(unsigned)((long long)s.batch * s.h * s.segments), kTcThreads, bytes, st>>>(s, a, b, c);
+    CNL_TRY(ensure_dynamic_smem(tc_kernel<DA, OUT, PARTS>, bytes));
+    tc_kernel<DA, OUT, PARTS><<<(unsigned)((long long)s.batch * s.h * s.segments * (s.dc > kCols ? 2 : 1)), kTcThreads, bytes, st>>>(s, a, b, c);
     return after_launch("linear attention sweep");
 }
 
-template <int D>
-int run_tc(Sweep s, cudaStream_t st) {
-    if (s.end) {                                                 // the state on its own, then the outputs
-        Sweep only = s;
-        only.out = nullptr;
-        CNL_TRY(s.exact ? (launch_tc<D, false, 3>(only, st)) : (launch_tc<D, false, 2>(only, st)));
-        if (!s.out) return CNL_OK;
-        s.end = nullptr;
-    }
-    return launch_tc<D, true, 2>(s, st);
+template <int DA>
+int run_tc(const Sweep& s, cudaStream_t st) {
+    const bool exact = s.end && s.exact;
+    if (!s.out) return exact ? launch_tc<DA, false, 3>(s, st) : launch_tc<DA, false, 2>(s, st);
+    return exact ? launch_tc<DA, true, 3>(s, st) : launch_tc<DA, true, 2>(s, st);
 }
 
 bool tc_sizes(int t, int da, int dc, int dtype) { return dtype == CNL_BF16 && t >= kTok && da > 32 && dc > 32 && da % 8 == 0 && dc % 8 == 0; }
@@ -543,7 +558,7 @@ bool tc_serves(const Sweep& s, int dtype) {
     return tc_sizes(s.t, s.da, s.dc, dtype) && fits(s.a) && fits(s.b) && fits(s.c) && aligned16(s.out);
 }
 
-int run_sweep_tc(const Sweep& s, cudaStream_t st) { return s.da <= 64 && s.dc <= 64 ? run_tc<64>(s, st) : run_tc<128>(s, st); }
+int run_sweep_tc(const Sweep& s, cudaStream_t st) { return s.da <= 64 ? run_tc<64>(s, st) : run_tc<128>(s, st); }
 
 }  // namespace lin
 }  // namespace cnl
