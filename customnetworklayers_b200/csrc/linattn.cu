@@ -161,37 +161,57 @@ int run_sweep(const Sweep& s, int dtype, cudaStream_t st) {
 
 // ---- scan over the segments -------------------------------------------------------------------------------------
 // local[seg] (W of every segment from 0) becomes W at the segment's start; `last` receives W at the sequence's end.
-__global__ void __launch_bounds__(256) scan_kernel(float* __restrict__ local, const float* __restrict__ init, float* __restrict__ last,
+// Four entries a thread where the sizes allow it, eight segments asked for together.
+template <int V>
+__global__ void __launch_bounds__(128) scan_kernel(float* __restrict__ local, const float* __restrict__ init, float* __restrict__ last,
                                                    const float* __restrict__ log_decay, const int* __restrict__ lengths, int t, int h,
                                                    int size, int segments, int seg) {
-    const int parts = (size + 255) >> 8;
+    const int parts = (size + 128 * V - 1) / (128 * V);
     const long long bh = blockIdx.x / parts;
-    const int e = (int)(blockIdx.x - bh * parts) * 256 + threadIdx.x;
+    const int e = ((int)(blockIdx.x - bh * parts) * 128 + threadIdx.x) * V;
     if (e >= size) return;
     const float ld = clamp_log(log_decay[bh % h]);
     const int n = lengths ? min(max(lengths[bh / h], 0), t) : t;
     float* p = local + bh * segments * size + e;
-    float w = init ? init[bh * size + e] : 0.0f;
+    const float whole = power(ld, seg);
+    auto get = [](const float* q, float (&v)[V]) {
+        if constexpr (V == 4) {
+            const float4 f = *reinterpret_cast<const float4*>(q);
+            v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+        } else v[0] = *q;
+    };
+    auto put = [](float* q, const float (&v)[V]) {
+        if constexpr (V == 4) *reinterpret_cast<float4*>(q) = make_float4(v[0], v[1], v[2], v[3]);
+        else *q = v[0];
+    };
+    float w[V] = {};
+    if (init) get(init + bh * size + e, w);
     constexpr int kAhead = 8;
     for (int s0 = 0; s0 < segments; s0 += kAhead) {
-        float v[kAhead];
+        float v[kAhead][V];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) v[i] = s0 + i < segments ? p[(long long)(s0 + i) * size] : 0.0f;
+        for (int i = 0; i < kAhead; ++i)
+            if (s0 + i < segments) get(p + (long long)(s0 + i) * size, v[i]);
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             if (s0 + i >= segments) break;
-            p[(long long)(s0 + i) * size] = w;
+            put(p + (long long)(s0 + i) * size, w);
             const long long left = n - (long long)(s0 + i) * seg;
-            const int len = (int)(left < 0 ? 0 : left < seg ? left : seg);
-            w = fmaf(power(ld, len), w, v[i]);
+            const float keep = left >= seg ? whole : power(ld, (int)(left < 0 ? 0 : left));
+#pragma unroll
+            for (int x = 0; x < V; ++x) w[x] = fmaf(keep, w[x], v[i][x]);
         }
     }
-    if (last) last[bh * size + e] = w;
+    if (last) put(last + bh * size + e, w);
 }
 
 int run_scan(float* local, const float* init, float* last, const float* log_decay, const int* lengths, int b, int t, int h, int size,
              int segments, int seg, cudaStream_t st) {
-    scan_kernel<<<(unsigned)((long long)((size + 255) / 256) * b * h), 256, 0, st>>>(local, init, last, log_decay, lengths, t, h, size, segments, seg);
+    const bool four = size % 4 == 0 && aligned16(local) && aligned16(init) && aligned16(last);
+    const int per = four ? 512 : 128;
+    const unsigned grid = (unsigned)((long long)((size + per - 1) / per) * b * h);
+    if (four) scan_kernel<4><<<grid, 128, 0, st>>>(local, init, last, log_decay, lengths, t, h, size, segments, seg);
+    else scan_kernel<1><<<grid, 128, 0, st>>>(local, init, last, log_decay, lengths, t, h, size, segments, seg);
     return after_launch("linear attention scan");
 }
 
@@ -283,7 +303,7 @@ int segment_plan(int b, int t, int h, int dk, int dv, int dtype, int* segments, 
     CNL_TRY(sm_count(&sms));
     const int d = dk > dv ? dk : dv;
     const bool tc = tc_sizes(t, dk, dv, dtype);
-    const long long heads = ((long long)b * h > 0 ? (long long)b * h : 1) * (tc && d > 64 ? 2 : 1);       // the tcgen05 sweep takes 64 columns a block
+    const long long heads = ((long long)b * h > 0 ? (long long)b * h : 1);
     // blocks that an SM holds of the kernel that serves these sizes
     const int each = dtype == CNL_F32 ? (d > 64 ? 1 : 4) : tc ? 1 : d > 64 ? 2 : d > 32 ? 4 : 8;
     const long long places = (long long)sms * each, most = (t + 127) / 128;

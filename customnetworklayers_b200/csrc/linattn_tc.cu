@@ -1,21 +1,20 @@
 // Linear attention sweep for bf16 on the fifth-generation tensor cores (formulas: linattn.cuh).
 //
-// A block of 18 warps walks one segment of one head, and 64 columns of its outputs, in chunks of 128 tokens.  One warp brings
-// a, b, c rows by TMA (128-byte swizzle), one thread issues the products, sixteen warps do what lies between.  Per chunk,
-// accumulators in tensor memory:
+// A block of 18 warps walks one segment of one head in chunks of 128 tokens.  One warp brings a, b, c rows by TMA (128-byte
+// swizzle), one thread issues the products, sixteen warps do what lies between.  Per chunk, accumulators in tensor memory:
 //     P = a b^T                 [128 tokens x 128 tokens]   -> weighted, masked, rounded, put back in tensor memory
-//     X = a (W0 | W1)           [128 tokens x 64 + 64]      W as the sweep has it before the chunk, in two addends
-//     O = P c                   [128 tokens x 64]
-//     T = (c0 | c1)^T b         [64 + 64 x da]              what the chunk adds to W^T; c0, c1: the weighted c in two parts
-// and in registers W^T <- l^m W^T + T (fp32, both addends), out = l^{pos + off} (X0 + X1) + O.  Nothing of the recurrence
-// passes through the tensor cores: T needs only the chunk's own rows, so it is summed while the outputs are finished.
-// Reversed sweeps take the tokens of a chunk in their order in memory and turn the mask and the weights around instead.
+//     X = a W                   [128 tokens x dc]           W as the sweep has it before the chunk
+//     O = P c                   [128 tokens x dc]
+//     T = (weighted c)^T b      [dc x da]                   what the chunk adds to W^T
+// and in registers W^T <- l^m W^T + T (fp32), out = l^{pos + off} X + O.  Nothing of the recurrence passes through the tensor
+// cores: T needs only the chunk's own rows, so it is summed while the outputs are finished.  Reversed sweeps take the tokens
+// of a chunk in their order in memory and turn the mask and the weights around instead.
 //
 // Operands: a and b for P, P, and W lie with the summed dimension contiguous; c, its parts, and b for T with it strided
-// (their rows are tokens), which the descriptors say.  64 columns fill the 128 rows of T with both parts of the weighted c,
-// and twice the blocks leave fewer and longer segments: at 64 heads of 128 none is cut, which saves the pass for the states.
-// Reads of shared memory bound the products (128 x 128 x 16 reads 8 KB), so a is read once for both addends of W.
-// Roundings: as in the mma.sync kernel (P once, W once, the weighted c to 16 or, where the state is a result, 24 bits).
+// (their rows are tokens), which the descriptors say.  The weighted c is split into two or three parts (roundings as in the
+// mma.sync kernel: P once, W once, the weighted c to 16 or, where the state is a result, 24 bits).  With up to 64 columns of
+// c (DC = 64) two parts fill the 128 rows of T, so W is kept in two addends, which X meets side by side; three parts are
+// (c0 | c1 / 2) and (c1 / 2 | c2).  With 128 columns the parts add up in T.
 //
 // Every wait is bounded: a block that gives up marks the status word, fills what it owes with NaN, and returns after its
 // copies and products have ended.
@@ -69,6 +68,9 @@ __device__ __forceinline__ float smem_get1(unsigned at) {
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
     return v;
 }
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, unsigned from, int x, int h, int t, int b) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(map), "r"(x), "r"(h), "r"(t), "r"(b), "r"(from) : "memory");
+}
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -116,24 +118,24 @@ __host__ __device__ constexpr unsigned product(int n, int strided_a, int strided
     return 1u << 4 | 1u << 7 | 1u << 10 | (unsigned)strided_a << 15 | (unsigned)strided_b << 16 | (unsigned)(n >> 3) << 17 | 8u << 24;
 }
 
-constexpr int kCols = 64;                       // output columns of a block
-
-template <int DA, bool OUT, int PARTS>
+template <int DA, int DC, bool OUT, int PARTS>
 struct Map {                                    // shared memory in bytes from a 1024-byte boundary
-    static constexpr int nb = DA / 64, one = nb * kBlk;          // a's or b's rows; c's are kBlk
-    static constexpr int two_a = DA == 128 && PARTS == 3 ? 1 : 2, two = 2;         // rooms for a; for b and c
-    static constexpr int a = 0, b = a + (OUT ? two_a * one : 0), c = b + two * one, w = c + two * kBlk;
-    static constexpr int parts = w + (OUT ? one : 0), part_blocks = PARTS == 3 ? 4 : 2;
-    static constexpr int bars = parts + part_blocks * kBlk;
-    static constexpr int bytes = bars + 256 + 1024;              // and the way to the boundary
+    static constexpr int one = DA / 64 * kBlk, one_c = DC / 64 * kBlk;     // a's or b's rows; c's, or one part of them
+    // rooms: two of each as far as they go.  a is free first, then c; b is held longest
+    static constexpr int two_a = OUT && DA == 128 ? 1 : 2, two_b = 2, two_c = OUT && DA == 128 && DC == 128 ? 1 : 2;
+    static constexpr int two_r = !OUT || DC == 128 ? 0 : DA == 128 && PARTS == 3 ? 1 : 2;       // output rows on their way; none: direct stores
+    static constexpr int a = 0, b = a + (OUT ? two_a * one : 0), c = b + two_b * one, w = c + two_c * one_c;
+    static constexpr int parts = w + (OUT ? one : 0), rows = parts + PARTS * one_c;
+    static constexpr int bars = rows + two_r * kBlk;
+    static constexpr int bytes = bars + 272 + 1024;              // and the way to the boundary
 };
 
 // ---- the sweep -----------------------------------------------------------------------------------------------------
-template <int DA, bool OUT, int PARTS>
+template <int DA, int DC, bool OUT, int PARTS>
 __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                                                           const __grid_constant__ CUtensorMap map_c) {
-    using M = Map<DA, OUT, PARTS>;
-    constexpr int NB = M::nb;
+                                                           const __grid_constant__ CUtensorMap map_c, const __grid_constant__ CUtensorMap map_o) {
+    using M = Map<DA, DC, OUT, PARTS>;
+    constexpr bool kStack = DC == 64;
     extern __shared__ unsigned char raw[];
     __shared__ float whole[32], edge[64];                        // powers of the decay for P: for whole tiles, for diagonal ones
     __shared__ int dead_word;
@@ -141,22 +143,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
     const unsigned base = (smem_at(raw) + 1023u) & ~1023u, bars = base + M::bars;
     volatile int* dead = &dead_word;
     // barriers, two of each: chunk i uses number i mod 2, whose phase is then i / 2
-    enum { FULL_A, FULL_B, FULL_C, DONE_P, DONE_X, DONE_T, DONE_O, HAS_C, HAS_P, HAS_W, HAS_O, CLEARED, KINDS };
+    enum { FULL_A, FULL_B, FULL_C, DONE_P, DONE_X, DONE_T, DONE_O, HAS_C, HAS_P, HAS_W, HAS_O, HAS_R, CLEARED, SENT, KINDS };
     auto read_p = [&](int quarter) { return bars + (unsigned)(KINDS * 2 + quarter) * 8; };      // P's fp32 columns of these lanes have been read
     auto bar = [&](int kind, int i) { return bars + (unsigned)(kind * 2 + (i & 1)) * 8; };
     auto phase = [](int i) { return (unsigned)(i >> 1) & 1u; };
     auto at_a = [](int i) { return M::a + i % M::two_a * M::one; };
-    auto at_b = [](int i) { return M::b + i % M::two * M::one; };
-    auto at_c = [](int i) { return M::c + i % M::two * kBlk; };
+    auto at_b = [](int i) { return M::b + i % M::two_b * M::one; };
+    auto at_c = [](int i) { return M::c + i % M::two_c * M::one_c; };
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int halves = s.dc > kCols ? 2 : 1;
-    const int seg = blockIdx.x % s.segments, col0 = blockIdx.x / s.segments % halves * kCols, bh = blockIdx.x / s.segments / halves, head = bh % s.h, bat = bh / s.h;
+    const int seg = blockIdx.x % s.segments, bh = blockIdx.x / s.segments, head = bh % s.h, bat = bh / s.h;
     const int n = s.lengths ? min(max(s.lengths[bat], 0), s.t) : s.t;
     const long long first = (long long)seg * s.seg;
     const int lo = (int)(first < n ? first : n), hi = (int)(first + s.seg < n ? first + s.seg : n);
     const int chunks = (hi - lo + kTok - 1) / kTok;
-    const int da = s.da, dc = s.dc, cols = min(dc - col0, kCols);
+    const int da = s.da, dc = s.dc;
     const long long size = (long long)da * dc;
     // first token of chunk i; positions lo + 128 i ... of the sweep
     auto token0 = [&](int i) { return s.reversed ? n - (lo + i * kTok) - kTok : lo + i * kTok; };
@@ -166,6 +167,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
         for (int i = 0; i < 2; ++i) {
             for (int k = FULL_A; k <= DONE_O; ++k) bar_init(bar(k, i), 1);
             for (int k = HAS_C; k <= CLEARED; ++k) bar_init(bar(k, i), kWorkers);
+            bar_init(bar(SENT, i), 1);
         }
         for (int k = 0; k < 4; ++k) bar_init(read_p(k), kWorkers / 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -177,26 +179,41 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
     }
     __syncthreads();
     tc_after();
-    const unsigned tmem = tmem_word, tP = tmem, tX = tmem + 128, tO = tmem + 256, tT = tmem + 320;
+    const unsigned tmem = tmem_word, tP = tmem, tX = tmem + 128, tO = tmem + 256, tT = tmem + 256 + DC;
 
     if (warp == kWorkers) {
         // ---- rows arrive
         if (lane == 0) {
             int i = 0;
+            auto send = [&](int j) {                             // the output rows of chunk j
+                if (!bar_wait(bar(HAS_R, j), phase(j), dead)) return false;
+                if (token0(j) >= 0) {                            // (a store must not start before the tensor: those rows go without it)
+                    tma_store(&map_o, base + M::rows + (M::two_r > 1 ? j & 1 : 0) * kBlk, 0, head, token0(j), bat);
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                }
+                bar_arrive(bar(SENT, j));
+                return true;
+            };
             for (; i < chunks; ++i) {
                 const int t0 = token0(i);
-                auto take = [&](int full, int done, int room, const CUtensorMap* map, const Rows& r, int to, int x0, int blocks) {
+                auto take = [&](int full, int done, int room, const CUtensorMap* map, const Rows& r, int to, int bytes) {
                     if (i >= room && !bar_wait(bar(done, i - room), phase(i - room), dead)) return false;
                     if (i >= room && full == FULL_C && !bar_wait(bar(HAS_C, i - room), phase(i - room), dead)) return false;
-                    bar_expect(bar(full, i), blocks * kBlk);
-                    for (int x = 0; x < blocks; ++x) tma_load(base + to + x * kBlk, map, x0 + x * 64, r.sh ? head : 0, t0, r.sb ? bat : 0, bar(full, i));
+                    bar_expect(bar(full, i), bytes);
+                    for (int x = 0; x < bytes / kBlk; ++x) tma_load(base + to + x * kBlk, map, x * 64, r.sh ? head : 0, t0, r.sb ? bat : 0, bar(full, i));
                     return true;
                 };
                 // room comes free: b after T, a after X, c after O and its parts
-                if (!take(FULL_B, DONE_T, M::two, &map_b, s.b, at_b(i), 0, NB)) break;
-                if (OUT && !take(FULL_A, DONE_X, M::two_a, &map_a, s.a, at_a(i), 0, NB)) break;
-                if (!take(FULL_C, OUT ? DONE_O : DONE_T, M::two, &map_c, s.c, at_c(i), col0, 1)) break;
+                if (!take(FULL_B, DONE_T, M::two_b, &map_b, s.b, at_b(i), M::one)) break;
+                if (M::two_r && i >= M::two_r && !send(i - M::two_r)) break;
+                if (OUT && !take(FULL_A, DONE_X, M::two_a, &map_a, s.a, at_a(i), M::one)) break;
+                if (!take(FULL_C, OUT ? DONE_O : DONE_T, M::two_c, &map_c, s.c, at_c(i), M::one_c)) break;
             }
+            if (M::two_r)
+                for (int j = max(0, chunks - M::two_r); j < chunks && !*dead; ++j)
+                    if (!send(j)) break;
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
             if (*dead) {                                         // what was asked for has to land before the block leaves
                 for (int j = max(0, i - 2); j <= min(i, chunks - 1); ++j)
                     for (int k = OUT ? FULL_A : FULL_B; k <= FULL_C; ++k)
@@ -236,7 +253,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
                 tc_after();
                 if (one) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) tc_mma_t(tO, tP + k * 8, operand(C, k * 2048), product(kCols, 0, 1), k > 0);
+                    for (int k = 0; k < 8; ++k) tc_mma_t(tO, tP + k * 8, operand(C, k * 2048), product(DC, 0, 1), k > 0);
                     tc_commit(bar(DONE_O, i));
                 }
                 __syncwarp();
@@ -247,11 +264,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
             if (!bar_wait(bar(HAS_C, i), ph, dead)) break;
             tc_after();
             if (one) {
-                // the third part first
+                // small parts first
+                constexpr int kSets = kStack ? PARTS - 1 : PARTS;
 #pragma unroll
-                for (int p = PARTS - 2; p >= 0; --p)
+                for (int p = kSets - 1; p >= 0; --p)
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) tc_mma(tT, operand(Q, p * 2 * kBlk + k * 2048), operand(Bt, k * 2048), product(DA, 1, 1), p < PARTS - 2 || k > 0);
+                    for (int k = 0; k < 8; ++k) tc_mma(tT, operand(Q, p * M::one_c + k * 2048), operand(Bt, k * 2048), product(DA, 1, 1), p < kSets - 1 || k > 0);
                 tc_commit(bar(DONE_T, i));
             }
             __syncwarp();
@@ -290,12 +308,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
             }
         };
         weigh(kTok);
-        // W^T: rows 0..63 first addend, 64..127 second
-        const int wrow = col0 + (row & 63), wcol = cq * HC;
+        // W^T: a row for a column of c (kStack: rows 0..63 first addend, 64..127 second)
+        const int wrow = kStack ? row & 63 : row, wcol = cq * HC;
         float2 w[HC / 2];
         {
             const float* w0 = s.start ? s.start + ((long long)bh * s.segments + seg) * size : nullptr;
-            const bool has = w0 && wrow < dc && row < 64;
+            const bool has = w0 && wrow < dc && (!kStack || row < 64);
 #pragma unroll
             for (int x = 0; x < HC; ++x) {
                 const int i = wcol + x;
@@ -322,13 +340,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
             }
             tell(HAS_W, i);
         };
-        if constexpr (PARTS == 3) {                   // the rows that stand beside the third part
-            for (int x = tid; x < kBlk / 16; x += kAll) smem_put(base + M::parts + 3 * kBlk + x * 16, make_uint4(0, 0, 0, 0));
-            fence_async();
-        }
+        constexpr int OC = DC / 4;                               // columns of X and O that a thread holds
         const long long by = (long long)s.h * dc;
-        const int ocol = cq * 16;                                // columns of X0, X1 and O
-        __nv_bfloat16* first_out = (__nv_bfloat16*)s.out + ((long long)bat * s.t * s.h + head) * dc + col0 + ocol;
+        const int ocol = cq * OC;
+        __nv_bfloat16* first_out = (__nv_bfloat16*)s.out + ((long long)bat * s.t * s.h + head) * dc + ocol;
         const bool wide = dc % 16 == 0 && (reinterpret_cast<size_t>(s.out) & 31) == 0;       // rows of whole 32-byte sectors
         asm volatile("bar.sync 1, %0;" ::"n"(kAll) : "memory");  // the tables
         if (OUT && chunks > 0) put_w(0);
@@ -338,11 +353,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
             const int left = hi - lo - i * kTok, m = left < kTok ? left : kTok;
             if (m < kTok && !s.reversed) {                       // rows behind the end become nothing, whatever they hold
                 if (!bar_wait(bar(FULL_B, i), ph, dead) || !bar_wait(bar(FULL_C, i), ph, dead) || (OUT && !bar_wait(bar(FULL_A, i), ph, dead))) break;
-                for (int e = tid; e < M::one / 16; e += kAll)
+                for (int e = tid; e < (M::one > M::one_c ? M::one : M::one_c) / 16; e += kAll)
                     if ((e >> 3 & 127) >= m) {
-                        smem_put(base + at_b(i) + e * 16, make_uint4(0, 0, 0, 0));
-                        if (OUT) smem_put(base + at_a(i) + e * 16, make_uint4(0, 0, 0, 0));
-                        if (e < kBlk / 16) smem_put(base + at_c(i) + e * 16, make_uint4(0, 0, 0, 0));
+                        const uint4 none = make_uint4(0, 0, 0, 0);
+                        if (e < M::one / 16) smem_put(base + at_b(i) + e * 16, none);
+                        if (OUT && e < M::one / 16) smem_put(base + at_a(i) + e * 16, none);
+                        if (e < M::one_c / 16) smem_put(base + at_c(i) + e * 16, none);
                     }
                 fence_async();
                 tell(CLEARED, i);
@@ -388,8 +404,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
             if (!bar_wait(bar(FULL_C, i), ph, dead)) break;
             if (m < kTok) weigh(m);
 #pragma unroll
+            for (int x = 0; x < DC / 64; ++x)
+#pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    const int off = (tid + kAll * k) * 16;
+                    const int off = x * kBlk + (tid + kAll * k) * 16;
                     const uint4 v = smem_get(base + at_c(i) + off);
                     unsigned in[4] = {v.x, v.y, v.z, v.w}, part[PARTS][4];
                     const float2 f = make_float2(wt[k], wt[k]);
@@ -402,12 +420,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
                             if (p + 1 < PARTS) {
                                 const float2 z = unpack2(part[p][e], __nv_bfloat16());
                                 y = __fadd2_rn(y, make_float2(-z.x, -z.y));
+                                if (kStack && PARTS == 3 && p == 1) part[p][e] = pack2<__nv_bfloat16>(0.5f * z.x, 0.5f * z.y);       // it is there twice
                             }
                         }
                     }
 #pragma unroll
                     for (int p = 0; p < PARTS; ++p)
-                        smem_put(base + M::parts + p * kBlk + off, make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]));
+                        smem_put(base + M::parts + p * M::one_c + off, make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]));
                 }
             fence_async();
             tell(HAS_C, i);
@@ -415,28 +434,42 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
                 // out = l^{pos + off} X + O
                 if (!bar_wait(bar(DONE_X, i), ph, dead) || !bar_wait(bar(DONE_O, i), ph, dead)) break;
                 tc_after();
-                const bool live = pos < m;
-                __nv_bfloat16* out = first_out + (token0(i) + row) * by;
-                {
+                const bool live = pos < m, turned = token0(i) < 0;           // a TMA store must not start before the tensor
+                if (M::two_r && i >= M::two_r && !bar_wait(bar(SENT, i - M::two_r), phase(i - M::two_r), dead)) break;
+#pragma unroll
+                for (int y = 0; y < OC / 16; ++y) {
                     unsigned r0[16], r1[16], r2[16];
-                    tc_load(tX + lanes + ocol, r0);
-                    tc_load(tX + lanes + kCols + ocol, r1);
-                    tc_load(tO + lanes + ocol, r2);
+                    tc_load(tX + lanes + ocol + y * 16, r0);
+                    if constexpr (kStack) tc_load(tX + lanes + 64 + ocol, r1);
+                    tc_load(tO + lanes + ocol + y * 16, r2);
                     tc_wait_load();
-                    tell(HAS_O, i);
+                    if (y == OC / 16 - 1) tell(HAS_O, i);
                     float2 v[8];
 #pragma unroll
-                    for (int x = 0; x < 8; ++x)
-                        v[x] = __ffma2_rn(make_float2(far, far), __fadd2_rn(make_float2(__uint_as_float(r0[2 * x]), __uint_as_float(r0[2 * x + 1])), make_float2(__uint_as_float(r1[2 * x]), __uint_as_float(r1[2 * x + 1]))),
-                                          make_float2(__uint_as_float(r2[2 * x]), __uint_as_float(r2[2 * x + 1])));
-                    const uint4 lo8 = four(v), hi8 = four(v + 4);
-                    if (live && wide) {
-                        if (ocol < cols)
-                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out), "r"(lo8.x), "r"(lo8.y), "r"(lo8.z), "r"(lo8.w), "r"(hi8.x), "r"(hi8.y), "r"(hi8.z), "r"(hi8.w) : "memory");
-                    } else if (live) {
-                        if (ocol < cols) *reinterpret_cast<uint4*>(out) = lo8;
-                        if (ocol + 8 < cols) *reinterpret_cast<uint4*>(out + 8) = hi8;
+                    for (int x = 0; x < 8; ++x) {
+                        float2 z = make_float2(__uint_as_float(r0[2 * x]), __uint_as_float(r0[2 * x + 1]));
+                        if constexpr (kStack) z = __fadd2_rn(z, make_float2(__uint_as_float(r1[2 * x]), __uint_as_float(r1[2 * x + 1])));
+                        v[x] = __ffma2_rn(make_float2(far, far), z, make_float2(__uint_as_float(r2[2 * x]), __uint_as_float(r2[2 * x + 1])));
                     }
+                    const uint4 lo8 = four(v), hi8 = four(v + 4);
+                    if (M::two_r && !turned) {                   // rows leave by TMA (those behind the end as the zeros they are)
+                        const unsigned to = base + M::rows + (M::two_r > 1 ? i & 1 : 0) * kBlk + row * 128;
+                        smem_put(to + (((cq * 2) ^ (row & 7)) << 4), live ? lo8 : make_uint4(0, 0, 0, 0));
+                        smem_put(to + (((cq * 2 + 1) ^ (row & 7)) << 4), live ? hi8 : make_uint4(0, 0, 0, 0));
+                    } else if (live) {
+                        __nv_bfloat16* to = first_out + (token0(i) + row) * by + y * 16;
+                        if (wide) {
+                            if (ocol + y * 16 < dc)
+                                asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(lo8.x), "r"(lo8.y), "r"(lo8.z), "r"(lo8.w), "r"(hi8.x), "r"(hi8.y), "r"(hi8.z), "r"(hi8.w) : "memory");
+                        } else {
+                            if (ocol + y * 16 < dc) *reinterpret_cast<uint4*>(to) = lo8;
+                            if (ocol + y * 16 + 8 < dc) *reinterpret_cast<uint4*>(to + 8) = hi8;
+                        }
+                    }
+                }
+                if (M::two_r) {
+                    fence_async();
+                    tell(HAS_R, i);
                 }
             }
             // W^T <- l^m W^T + T
@@ -457,23 +490,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
         }
         if (s.end) {
             float* w1 = s.end + ((long long)bh * s.segments + seg) * size;
-            asm volatile("bar.sync 1, %0;" ::"n"(kAll) : "memory");
-            const unsigned meet = base + M::parts + (row & 63) * 4;        // the two addends meet in the parts' room
-            if (row >= 64)
+            if constexpr (kStack) {
+                asm volatile("bar.sync 1, %0;" ::"n"(kAll) : "memory");
+                const unsigned meet = base + M::parts + (row & 63) * 4;        // the two addends meet in the parts' room
+                if (row >= 64)
 #pragma unroll
-                for (int x = 0; x < HC / 2; ++x) {
-                    smem_put(meet + (wcol + 2 * x) * 256, w[x].x);
-                    smem_put(meet + (wcol + 2 * x + 1) * 256, w[x].y);
-                }
-            asm volatile("bar.sync 1, %0;" ::"n"(kAll) : "memory");
-            if (row < 64)
+                    for (int x = 0; x < HC / 2; ++x) {
+                        smem_put(meet + (wcol + 2 * x) * 256, w[x].x);
+                        smem_put(meet + (wcol + 2 * x + 1) * 256, w[x].y);
+                    }
+                asm volatile("bar.sync 1, %0;" ::"n"(kAll) : "memory");
+                if (row < 64)
 #pragma unroll
-                for (int x = 0; x < HC / 2; ++x) {
-                    w[x].x += smem_get1(meet + (wcol + 2 * x) * 256);
-                    w[x].y += smem_get1(meet + (wcol + 2 * x + 1) * 256);
-                }
+                    for (int x = 0; x < HC / 2; ++x) {
+                        w[x].x += smem_get1(meet + (wcol + 2 * x) * 256);
+                        w[x].y += smem_get1(meet + (wcol + 2 * x + 1) * 256);
+                    }
+            }
             const bool lost = *dead != 0;
-            if (wrow < dc && row < 64)
+            if (wrow < dc && (!kStack || row < 64))
 #pragma unroll
                 for (int x = 0; x < HC; ++x)
                     if (wcol + x < da) w1[(long long)(wcol + x) * dc + wrow] = lost ? __uint_as_float(0x7fffffffu) : x & 1 ? w[x / 2].y : w[x / 2].x;
@@ -487,9 +522,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
     if (lost && tid == 0) g_gave_up = 1;
     if constexpr (OUT) {                                         // rows behind the sequence's end; all rows of a block that gave up
         const long long zlo = lost ? lo : (first > n ? first : n), zhi = first + s.seg < s.t ? first + s.seg : s.t;
-        for (long long e = zlo * cols + tid; e < zhi * cols; e += kTcThreads) {
-            const long long i = e / cols, tok = i < n && s.reversed ? n - 1 - i : i;
-            ((__nv_bfloat16*)s.out)[(((long long)bat * s.t + tok) * s.h + head) * dc + col0 + (e - i * cols)] = from_f32<__nv_bfloat16>(i < n ? __uint_as_float(0x7fffffffu) : 0.0f);
+        for (long long e = zlo * dc + tid; e < zhi * dc; e += kTcThreads) {
+            const long long i = e / dc, tok = i < n && s.reversed ? n - 1 - i : i;
+            ((__nv_bfloat16*)s.out)[(((long long)bat * s.t + tok) * s.h + head) * dc + (e - i * dc)] = from_f32<__nv_bfloat16>(i < n ? __uint_as_float(0x7fffffffu) : 0.0f);
         }
     }
 }
@@ -528,24 +563,36 @@ int encode(CUtensorMap* map, const Rows& r, int b, int t, int h, int d) {
     return CNL_OK;
 }
 
-template <int DA, bool OUT, int PARTS>
+template <int DA, int DC, bool OUT, int PARTS>
 int launch_tc(const Sweep& s, cudaStream_t st) {
-    CUtensorMap a = {}, b, c;
-    if (OUT) CNL_TRY(encode(&a, s.a, s.batch, s.t, s.h, s.da));
+    CUtensorMap a = {}, b, c, o = {};
+    if (OUT) {
+        CNL_TRY(encode(&a, s.a, s.batch, s.t, s.h, s.da));
+        CNL_TRY(encode(&o, Rows{s.out, (long long)s.t * s.h * s.dc, (long long)s.h * s.dc, s.dc}, s.batch, s.t, s.h, s.dc));
+    }
     CNL_TRY(encode(&b, s.b, s.batch, s.t, s.h, s.da));
     CNL_TRY(encode(&c, s.c, s.batch, s.t, s.h, s.dc));
-    constexpr int bytes = Map<DA, OUT, PARTS>::bytes;
+    constexpr int bytes = Map<DA, DC, OUT, PARTS>::bytes;
     static_assert(bytes <= 232448, "more shared memory than a block may have");
-    CNL_TRY(ensure_dynamic_smem(tc_kernel<DA, OUT, PARTS>, bytes));
-    tc_kernel<DA, OUT, PARTS><<<(unsigned)((long long)s.batch * s.h * s.segments * (s.dc > kCols ? 2 : 1)), kTcThreads, bytes, st>>>(s, a, b, c);
+    CNL_TRY(ensure_dynamic_smem(tc_kernel<DA, DC, OUT, PARTS>, bytes));
+    tc_kernel<DA, DC, OUT, PARTS><<<(unsigned)((long long)s.batch * s.h * s.segments), kTcThreads, bytes, st>>>(s, a, b, c, o);
     return after_launch("linear attention sweep");
 }
 
-template <int DA>
-int run_tc(const Sweep& s, cudaStream_t st) {
+template <int DA, int DC>
+int run_tc(Sweep s, cudaStream_t st) {
     const bool exact = s.end && s.exact;
-    if (!s.out) return exact ? launch_tc<DA, false, 3>(s, st) : launch_tc<DA, false, 2>(s, st);
-    return exact ? launch_tc<DA, true, 3>(s, st) : launch_tc<DA, true, 2>(s, st);
+    if constexpr (DC == 64) {
+        if (s.out) return exact ? launch_tc<DA, DC, true, 3>(s, st) : launch_tc<DA, DC, true, 2>(s, st);
+    }
+    if (s.out && exact) {                                        // no room for three parts beside the outputs: the state on its own
+        Sweep only = s;
+        only.out = nullptr;
+        CNL_TRY((launch_tc<DA, DC, false, 3>(only, st)));
+        s.end = nullptr;
+    }
+    if (s.out) return launch_tc<DA, DC, true, 2>(s, st);
+    return exact ? launch_tc<DA, DC, false, 3>(s, st) : launch_tc<DA, DC, false, 2>(s, st);
 }
 
 bool tc_sizes(int t, int da, int dc, int dtype) { return dtype == CNL_BF16 && t >= kTok && da > 32 && dc > 32 && da % 8 == 0 && dc % 8 == 0; }
@@ -558,7 +605,10 @@ bool tc_serves(const Sweep& s, int dtype) {
     return tc_sizes(s.t, s.da, s.dc, dtype) && fits(s.a) && fits(s.b) && fits(s.c) && aligned16(s.out);
 }
 
-int run_sweep_tc(const Sweep& s, cudaStream_t st) { return s.da <= 64 ? run_tc<64>(s, st) : run_tc<128>(s, st); }
+int run_sweep_tc(const Sweep& s, cudaStream_t st) {
+    if (s.da <= 64) return s.dc <= 64 ? run_tc<64, 64>(s, st) : run_tc<64, 128>(s, st);
+    return s.dc <= 64 ? run_tc<128, 64>(s, st) : run_tc<128, 128>(s, st);
+}
 
 }  // namespace lin
 }  // namespace cnl
