@@ -55,6 +55,9 @@ __device__ __forceinline__ bool bar_wait(unsigned bar, unsigned parity, volatile
 __device__ __forceinline__ void tma_load(unsigned to, const CUtensorMap* map, int x, int h, int t, int b, unsigned bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to), "l"(map), "r"(x), "r"(h), "r"(t), "r"(b), "r"(bar) : "memory");
 }
+__device__ __forceinline__ void tma_ahead(const CUtensorMap* map, int x, int h, int t, int b) {      // into L2
+    asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(map), "r"(x), "r"(h), "r"(t), "r"(b) : "memory");
+}
 // 16 bytes of shared memory by address: a generic pointer, which alignment by hand leaves, would cost the slower path
 __device__ __forceinline__ uint4 smem_get(unsigned at) {
     uint4 v;
@@ -123,10 +126,12 @@ struct Map {                                    // shared memory in bytes from a
     static constexpr int one = DA / 64 * kBlk, one_c = DC / 64 * kBlk;     // a's or b's rows; c's, or one part of them
     // rooms: two of each as far as they go.  a is free first, then c; b is held longest
     static constexpr int two_a = OUT && DA == 128 ? 1 : 2, two_b = 2, two_c = OUT && DA == 128 && DC == 128 ? 1 : 2;
-    static constexpr int two_r = !OUT || DC == 128 ? 0 : DA == 128 && PARTS == 3 ? 1 : 2;       // output rows on their way; none: direct stores
+    // output rows on their way: rooms of their own, or (128 columns) c's, which O and the parts were the last to read
+    static constexpr bool through_c = DC == 128;
+    static constexpr int two_r = !OUT ? 0 : through_c ? two_c : DA == 128 && PARTS == 3 ? 1 : 2;
     static constexpr int a = 0, b = a + (OUT ? two_a * one : 0), c = b + two_b * one, w = c + two_c * one_c;
     static constexpr int parts = w + (OUT ? one : 0), rows = parts + PARTS * one_c;
-    static constexpr int bars = rows + two_r * kBlk;
+    static constexpr int bars = rows + (through_c ? 0 : two_r * kBlk);
     static constexpr int bytes = bars + 272 + 1024;              // and the way to the boundary
 };
 
@@ -150,6 +155,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
     auto at_a = [](int i) { return M::a + i % M::two_a * M::one; };
     auto at_b = [](int i) { return M::b + i % M::two_b * M::one; };
     auto at_c = [](int i) { return M::c + i % M::two_c * M::one_c; };
+    auto at_r = [](int i) { return M::through_c ? M::c + i % M::two_c * M::one_c : M::rows + i % (M::two_r > 1 ? 2 : 1) * kBlk; };
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int seg = blockIdx.x % s.segments, bh = blockIdx.x / s.segments, head = bh % s.h, bat = bh / s.h;
@@ -188,7 +194,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
             auto send = [&](int j) {                             // the output rows of chunk j
                 if (!bar_wait(bar(HAS_R, j), phase(j), dead)) return false;
                 if (token0(j) >= 0) {                            // (a store must not start before the tensor: those rows go without it)
-                    tma_store(&map_o, base + M::rows + (M::two_r > 1 ? j & 1 : 0) * kBlk, 0, head, token0(j), bat);
+                    for (int x = 0; x < DC / 64; ++x)
+                        if (x * 64 < dc) tma_store(&map_o, base + at_r(j) + x * kBlk, x * 64, head, token0(j), bat);
                     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                 }
@@ -204,10 +211,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
                     for (int x = 0; x < bytes / kBlk; ++x) tma_load(base + to + x * kBlk, map, x * 64, r.sh ? head : 0, t0, r.sb ? bat : 0, bar(full, i));
                     return true;
                 };
-                // room comes free: b after T, a after X, c after O and its parts
+                // room comes free: b after T, a after X, c after O and its parts (and the output rows that pass through it)
                 if (!take(FULL_B, DONE_T, M::two_b, &map_b, s.b, at_b(i), M::one)) break;
-                if (M::two_r && i >= M::two_r && !send(i - M::two_r)) break;
+                if (M::through_c && M::two_c == 1 && i > 0)      // its room comes free late: at least from L2 then
+                    for (int x = 0; x < DC / 64; ++x) tma_ahead(&map_c, x * 64, s.c.sh ? head : 0, t0, s.c.sb ? bat : 0);
+                if (OUT && !M::through_c && i >= M::two_r && !send(i - M::two_r)) break;
                 if (OUT && !take(FULL_A, DONE_X, M::two_a, &map_a, s.a, at_a(i), M::one)) break;
+                if (OUT && M::through_c && i >= M::two_r && !send(i - M::two_r)) break;
                 if (!take(FULL_C, OUT ? DONE_O : DONE_T, M::two_c, &map_c, s.c, at_c(i), M::one_c)) break;
             }
             if (M::two_r)
@@ -343,9 +353,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
         constexpr int OC = DC / 4;                               // columns of X and O that a thread holds
         const long long by = (long long)s.h * dc;
         const int ocol = cq * OC;
-        __nv_bfloat16* first_out = (__nv_bfloat16*)s.out + ((long long)bat * s.t * s.h + head) * dc + ocol;
-        const bool wide = dc % 16 == 0 && (reinterpret_cast<size_t>(s.out) & 31) == 0;       // rows of whole 32-byte sectors
         asm volatile("bar.sync 1, %0;" ::"n"(kAll) : "memory");  // the tables
+        __nv_bfloat16* first_out = (__nv_bfloat16*)s.out + ((long long)bat * s.t * s.h + head) * dc + ocol;
         if (OUT && chunks > 0) put_w(0);
 
         for (int i = 0; i < chunks; ++i) {
@@ -435,7 +444,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
                 if (!bar_wait(bar(DONE_X, i), ph, dead) || !bar_wait(bar(DONE_O, i), ph, dead)) break;
                 tc_after();
                 const bool live = pos < m, turned = token0(i) < 0;           // a TMA store must not start before the tensor
-                if (M::two_r && i >= M::two_r && !bar_wait(bar(SENT, i - M::two_r), phase(i - M::two_r), dead)) break;
+                if (M::through_c ? !bar_wait(bar(HAS_C, i), ph, dead)        // every warp has read c
+                                 : i >= M::two_r && !bar_wait(bar(SENT, i - M::two_r), phase(i - M::two_r), dead)) break;
 #pragma unroll
                 for (int y = 0; y < OC / 16; ++y) {
                     unsigned r0[16], r1[16], r2[16];
@@ -452,25 +462,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
                         v[x] = __ffma2_rn(make_float2(far, far), z, make_float2(__uint_as_float(r2[2 * x]), __uint_as_float(r2[2 * x + 1])));
                     }
                     const uint4 lo8 = four(v), hi8 = four(v + 4);
-                    if (M::two_r && !turned) {                   // rows leave by TMA (those behind the end as the zeros they are)
-                        const unsigned to = base + M::rows + (M::two_r > 1 ? i & 1 : 0) * kBlk + row * 128;
-                        smem_put(to + (((cq * 2) ^ (row & 7)) << 4), live ? lo8 : make_uint4(0, 0, 0, 0));
-                        smem_put(to + (((cq * 2 + 1) ^ (row & 7)) << 4), live ? hi8 : make_uint4(0, 0, 0, 0));
+                    const int piece = (ocol + y * 16) / 8;       // rows leave by TMA (those behind the end as the zeros they are)
+                    if (!turned) {
+                        const unsigned to = base + at_r(i) + (piece >> 3) * kBlk + row * 128;
+                        smem_put(to + (((piece & 7) ^ (row & 7)) << 4), live ? lo8 : make_uint4(0, 0, 0, 0));
+                        smem_put(to + (((piece + 1 & 7) ^ (row & 7)) << 4), live ? hi8 : make_uint4(0, 0, 0, 0));
                     } else if (live) {
                         __nv_bfloat16* to = first_out + (token0(i) + row) * by + y * 16;
-                        if (wide) {
-                            if (ocol + y * 16 < dc)
-                                asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(lo8.x), "r"(lo8.y), "r"(lo8.z), "r"(lo8.w), "r"(hi8.x), "r"(hi8.y), "r"(hi8.z), "r"(hi8.w) : "memory");
-                        } else {
-                            if (ocol + y * 16 < dc) *reinterpret_cast<uint4*>(to) = lo8;
-                            if (ocol + y * 16 + 8 < dc) *reinterpret_cast<uint4*>(to + 8) = hi8;
-                        }
+                        if (ocol + y * 16 < dc) *reinterpret_cast<uint4*>(to) = lo8;
+                        if (ocol + y * 16 + 8 < dc) *reinterpret_cast<uint4*>(to + 8) = hi8;
                     }
                 }
-                if (M::two_r) {
-                    fence_async();
-                    tell(HAS_R, i);
-                }
+                fence_async();
+                tell(HAS_R, i);
             }
             // W^T <- l^m W^T + T
             if (!bar_wait(bar(DONE_T, i), ph, dead)) break;
