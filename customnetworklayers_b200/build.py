@@ -12,7 +12,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libcnl_b200.so")
 SOURCES = ["common.cu", "tv_fista.cu", "tv_fused.cu", "tv_flow.cu", "peer_allreduce.cu", "tv_noalloc.cu", "median.cu", "quadfit.cu", "tgv.cu", "tgv_vec.cu", "wmedian.cu",
-           "ckpt8.cu", "blocknorm.cu", "blocknorm_vec.cu", "linattn.cu", "linattn_mma.cu", "linattn_tc.cu"]
+           "ckpt8.cu", "blocknorm.cu", "blocknorm_vec.cu", "linattn.cu", "linattn_f32.cu", "linattn_mma.cu",
+           "linattn_tc.cu"]
 HEADERS = ["common.h", "tv_math.cuh", "tv_fused.cuh", "tv_tile.cuh", "tgv_vec.cuh", "dtypes.cuh", "ckpt8.cuh", "blocknorm.cuh", "linattn.cuh",
            os.path.join("..", "..", "include", "cnl_b200.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

@@ -1,161 +1,14 @@
-// Linear attention with a decay for each head: drivers, the kernel in fp32 arithmetic, the scan over segments and the
-// single-token step (formulas: linattn.cuh).
+// Linear attention with a decay for each head: drivers, the scan over segments and the single-token step (formulas:
+// linattn.cuh; sweeps: linattn_f32.cu, linattn_mma.cu, linattn_tc.cu).
 #include "linattn.cuh"
 
 namespace cnl {
 namespace lin {
 
 constexpr int kMaxD = 128;
-constexpr int kC = 32;                       // positions of a chunk
-constexpr int kThreads = 256;
-
-// ---- sweep in fp32 arithmetic -----------------------------------------------------------------------------------
-// A block walks one segment of one head chunk by chunk.  Operands, the C x C product and W lie in shared memory in fp32;
-// every product is plain multiply-adds on 4 x 4 register tiles.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) sweep_kernel(const Sweep s) {
-    extern __shared__ float4 smem4[];
-    const int da = s.da, dc = s.dc, pa = (da + 3) / 4 * 4, pc = (dc + 3) / 4 * 4;
-    const int ra = pa + 4, rc = pc + 4;                          // row strides: 16-byte rows on different banks
-    float* A = reinterpret_cast<float*>(smem4);
-    float* B = A + kC * ra;
-    float* Cc = B + kC * ra;
-    float* W = Cc + kC * rc;
-    float* P = W + pa * rc;
-    const int tid = threadIdx.x;
-    const int seg = blockIdx.x % s.segments, bh = blockIdx.x / s.segments, head = bh % s.h, bat = bh / s.h;
-    const float ld = clamp_log(s.log_decay[head]);
-    const int n = s.lengths ? min(max(s.lengths[bat], 0), s.t) : s.t;
-    const long long first = (long long)seg * s.seg;
-    const int lo = (int)(first < n ? first : n), hi = (int)(first + s.seg < n ? first + s.seg : n);
-    const long long size = (long long)da * dc;
-
-    const float* w0 = s.start ? s.start + ((long long)bh * s.segments + seg) * size : nullptr;
-    for (int e = tid; e < pa * pc; e += kThreads) {
-        const int i = e / pc, j = e - i * pc;
-        W[i * rc + j] = w0 && i < da && j < dc ? (s.transposed ? w0[(long long)j * da + i] : w0[(long long)i * dc + j]) : 0.0f;
-    }
-    for (int c0 = lo; c0 < hi; c0 += kC) {
-        const int m = min(kC, hi - c0);
-        __syncthreads();
-        auto fetch = [&](const Rows& r, float* dst, int d, int stride) {
-            const int p = stride - 4;
-            const T* src = (const T*)r.p + bat * r.sb + head * r.sh;
-            for (int e = tid; e < kC * p; e += kThreads) {
-                const int j = e / p, x = e - j * p;
-                const long long tok = s.reversed ? n - 1 - (c0 + j) : c0 + j;
-                dst[j * stride + x] = j < m && x < d ? to_f32(src[tok * r.st + x]) : 0.0f;
-            }
-        };
-        if (s.out) fetch(s.a, A, da, ra);
-        fetch(s.b, B, da, ra);
-        fetch(s.c, Cc, dc, rc);
-        __syncthreads();
-        if (s.out) {
-            for (int e = tid; e < kC * kC; e += kThreads) {
-                const int i = e / kC, j = e % kC;
-                float v = 0.0f;
-                if (j <= i && i < m) {
-                    for (int x = 0; x < pa; x += 4) {
-                        const float4 p = *reinterpret_cast<const float4*>(A + i * ra + x), q = *reinterpret_cast<const float4*>(B + j * ra + x);
-                        v = fmaf(p.x, q.x, v); v = fmaf(p.y, q.y, v); v = fmaf(p.z, q.z, v); v = fmaf(p.w, q.w, v);
-                    }
-                    v *= power(ld, i - j) * s.in_scale;
-                }
-                P[i * (kC + 1) + j] = v;
-            }
-            __syncthreads();
-            const int cols = pc / 4;
-            for (int e = tid; e < kC / 4 * cols; e += kThreads) {
-                const int i0 = e / cols * 4, x = e % cols * 4;
-                float in[4][4] = {}, far[4][4] = {};
-                for (int j = 0; j < min(m, i0 + 4); ++j) {
-                    const float4 q = *reinterpret_cast<const float4*>(Cc + j * rc + x);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float p = P[(i0 + r) * (kC + 1) + j];
-                        in[r][0] = fmaf(p, q.x, in[r][0]); in[r][1] = fmaf(p, q.y, in[r][1]);
-                        in[r][2] = fmaf(p, q.z, in[r][2]); in[r][3] = fmaf(p, q.w, in[r][3]);
-                    }
-                }
-                for (int y = 0; y < pa; ++y) {
-                    const float4 q = *reinterpret_cast<const float4*>(W + y * rc + x);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float p = A[(i0 + r) * ra + y];
-                        far[r][0] = fmaf(p, q.x, far[r][0]); far[r][1] = fmaf(p, q.y, far[r][1]);
-                        far[r][2] = fmaf(p, q.z, far[r][2]); far[r][3] = fmaf(p, q.w, far[r][3]);
-                    }
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (i0 + r >= m) break;
-                    const long long tok = s.reversed ? n - 1 - (c0 + i0 + r) : c0 + i0 + r;
-                    T* out = (T*)s.out + (((long long)bat * s.t + tok) * s.h + head) * dc;
-                    const float f = power(ld, i0 + r + s.off);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (x + k < dc) out[x + k] = from_f32<T>(s.out_scale * fmaf(f, far[r][k], in[r][k]));
-                }
-            }
-            __syncthreads();
-        }
-        for (int e = tid; e < m * pa; e += kThreads) {
-            const int j = e / pa, x = e - j * pa;
-            B[j * ra + x] *= power(ld, m - s.off - j) * s.in_scale;
-        }
-        __syncthreads();
-        const float keep = power(ld, m);
-        const int cols = pc / 4;
-        for (int e = tid; e < pa / 4 * cols; e += kThreads) {
-            const int y = e / cols * 4, x = e % cols * 4;
-            float acc[4][4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float4 q = *reinterpret_cast<const float4*>(W + (y + r) * rc + x);
-                acc[r][0] = keep * q.x; acc[r][1] = keep * q.y; acc[r][2] = keep * q.z; acc[r][3] = keep * q.w;
-            }
-            for (int j = 0; j < m; ++j) {
-                const float4 p = *reinterpret_cast<const float4*>(B + j * ra + y), q = *reinterpret_cast<const float4*>(Cc + j * rc + x);
-                const float pv[4] = {p.x, p.y, p.z, p.w};
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    acc[r][0] = fmaf(pv[r], q.x, acc[r][0]); acc[r][1] = fmaf(pv[r], q.y, acc[r][1]);
-                    acc[r][2] = fmaf(pv[r], q.z, acc[r][2]); acc[r][3] = fmaf(pv[r], q.w, acc[r][3]);
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) *reinterpret_cast<float4*>(W + (y + r) * rc + x) = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
-        }
-    }
-    __syncthreads();
-    if (s.end) {
-        float* w1 = s.end + ((long long)bh * s.segments + seg) * size;
-        for (int e = tid; e < da * dc; e += kThreads) {
-            const int i = e / dc, j = e - i * dc;
-            w1[e] = W[i * rc + j];
-        }
-    }
-    if (s.out) {                                                 // rows behind the sequence's end
-        const long long zlo = first > n ? first : n, zhi = first + s.seg < s.t ? first + s.seg : s.t;
-        for (long long e = zlo * dc + tid; e < zhi * dc; e += kThreads) {
-            const long long tok = e / dc;
-            ((T*)s.out)[(((long long)bat * s.t + tok) * s.h + head) * dc + (e - tok * dc)] = from_f32<T>(0.0f);
-        }
-    }
-}
-
-template <typename T>
-int launch_sweep(const Sweep& s, cudaStream_t st) {
-    const int pa = (s.da + 3) / 4 * 4, pc = (s.dc + 3) / 4 * 4;
-    const int bytes = (2 * kC * (pa + 4) + kC * (pc + 4) + pa * (pc + 4) + kC * (kC + 1)) * 4;
-    CNL_TRY(ensure_dynamic_smem(sweep_kernel<T>, bytes));
-    sweep_kernel<T><<<(unsigned)((long long)s.batch * s.h * s.segments), kThreads, bytes, st>>>(s);
-    return after_launch("linear attention sweep");
-}
 
 int run_sweep(const Sweep& s, int dtype, cudaStream_t st) {
-    if (dtype == CNL_F32) return launch_sweep<float>(s, st);
+    if (dtype == CNL_F32) return run_sweep_f32(s, st);
     return tc_serves(s, dtype) ? run_sweep_tc(s, st) : run_sweep_mma(s, dtype, st);
 }
 
@@ -305,7 +158,7 @@ int segment_plan(int b, int t, int h, int dk, int dv, int dtype, int* segments, 
     const bool tc = tc_sizes(t, dk, dv, dtype);
     const long long heads = ((long long)b * h > 0 ? (long long)b * h : 1);
     // blocks that an SM holds of the kernel that serves these sizes
-    const int each = dtype == CNL_F32 ? (d > 64 ? 1 : 4) : tc ? 1 : d > 64 ? 2 : d > 32 ? 4 : 8;
+    const int each = dtype == CNL_F32 ? (d > 64 ? 1 : d > 32 ? 2 : 4) : tc ? 1 : d > 64 ? 2 : d > 32 ? 4 : 8;
     const long long places = (long long)sms * each, most = (t + 127) / 128;
     long long best = 0;
     *segments = 1;

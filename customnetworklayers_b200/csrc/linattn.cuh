@@ -1,4 +1,4 @@
-// One sweep of linear attention with a decay for each head: shared by the fp32 kernel, the tensor-core kernel and the drivers.
+// One sweep of linear attention with a decay for each head: shared by the kernels and the drivers.
 //
 // Sweep over positions i = 0 .. n-1 of one head (l = exp(log_decay)):
 //     out_i = out_scale ( in_scale sum_{j <= i} l^{i-j} (a_i . b_j) c_j  +  l^{i + off} a_i^T W_0 )
@@ -42,6 +42,7 @@ __device__ __forceinline__ float clamp_log(float a) { return a < -1e30f ? -1e30f
 __device__ __forceinline__ float power(float a, int n) { return expf(a * (float)n); }
 
 int run_sweep(const Sweep& s, int dtype, cudaStream_t st);          // dispatches to the kernel that serves the type and sizes
+int run_sweep_f32(const Sweep& s, cudaStream_t st);
 int run_sweep_mma(const Sweep& s, int dtype, cudaStream_t st);      // fp16, bf16: mma.sync
 bool tc_sizes(int t, int da, int dc, int dtype);                    // sizes that the tcgen05 sweep serves
 bool tc_serves(const Sweep& s, int dtype);                          // ... and rows that TMA can take

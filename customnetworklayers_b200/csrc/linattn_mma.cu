@@ -6,7 +6,8 @@
 // chunk: P = a b^T (ten 16 x 16 blocks at or under the diagonal, shared out over the warps), out = l^{i+off} (a W) + P c,
 // W = l^m W + (weighted c)^T b.  The next chunk's rows arrive by cp.async meanwhile.
 //
-// Roundings to the type: P's weights and W where they meet the outputs, once each, as the outputs themselves.  The weighted
+// Roundings to the type: W where it meets the outputs, once, as the outputs themselves; P's weights go in two parts (a tenth
+// of the products: short sequences, which have nothing else, would lose 1.5 times what the outputs' own rounding costs).  The weighted
 // c of the state is split into parts of the type (one part would be off by 1.6e-3): fp16 into two, 22 bits, the second times
 // 2^11 and summed apart, so that it does not fall under fp16's range; bf16 into two (16 bits, 7e-7 rms) where W only feeds
 // rounded outputs, and into all three where a caller gets the state (EXACT).  A chunk is summed apart and added to W by one
@@ -44,7 +45,7 @@ template <int DA, int DC, bool OUT>
 struct Layout {                              // shared memory, in elements of the type
     static constexpr int ra = DA + kPad, rc = DC + kPad, rp = kChunk + kPad;
     static constexpr int a = 0, b = OUT ? kChunk * ra : 0, c = b + kChunk * ra, stage = c + kChunk * rc;
-    static constexpr int p = 2 * stage, o = p + (OUT ? kChunk * rp : 0);
+    static constexpr int p = 2 * stage, p2 = kChunk * rp, o = p + (OUT ? 2 * p2 : 0);      // P's two parts
     static constexpr bool own_o = OUT && DC > DA;              // otherwise outputs pass through the rows of a just read
     static constexpr int end = o + (own_o ? kChunk * rc : 0);
     static constexpr int bytes = (end * 2 + 15) / 16 * 16 + (3 * kChunk + 24) * 4;      // and the three tables of powers
@@ -182,7 +183,13 @@ __global__ void __launch_bounds__(2 * DC, DC == 128 ? 2 : DC == 64 ? 4 : 8) mma_
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
-                        *reinterpret_cast<unsigned*>(to + h * 8 * L::rp + x * 8) = pack2<T>(acc[x][2 * h] * z[8 * h - 8 * x], acc[x][2 * h + 1] * z[8 * h - 8 * x - 1]);
+                    {
+                        const float2 v = make_float2(acc[x][2 * h] * z[8 * h - 8 * x], acc[x][2 * h + 1] * z[8 * h - 8 * x - 1]);
+                        const unsigned top = pack2<T>(v.x, v.y);
+                        const float2 f = unpack2(top, T());
+                        *reinterpret_cast<unsigned*>(to + h * 8 * L::rp + x * 8) = top;
+                        *reinterpret_cast<unsigned*>(to + L::p2 + h * 8 * L::rp + x * 8) = pack2<T>(v.x - f.x, v.y - f.y);
+                    }
             }
             __syncthreads();
             float down = 1.0f, up = s.out_scale;
@@ -241,6 +248,9 @@ __global__ void __launch_bounds__(2 * DC, DC == 128 ? 2 : DC == 64 ? 4 : 8) mma_
                         if (k > half * 2 + i) continue;
                         unsigned a[4];
                         ldsm(a, P + (half * 32 + i * 16 + (lane & 15)) * L::rp + k * 16 + (lane >> 4) * 8);
+                        mma(o[i][0], a, b[0], b[1], T());
+                        mma(o[i][1], a, b[2], b[3], T());
+                        ldsm(a, P + L::p2 + (half * 32 + i * 16 + (lane & 15)) * L::rp + k * 16 + (lane >> 4) * 8);
                         mma(o[i][0], a, b[0], b[1], T());
                         mma(o[i][1], a, b[2], b[3], T());
                     }
