@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(BLOCK, 512 / BLOCK) backward_vec(const Args a)
     int asked = 0;
     unsigned into = 0, from = 0;
     float4 st_next = {};
-    unsigned sc_next = 0;
+    unsigned sc_x = 0, sc_u = 0, sc_z = 0;                                 // not joined before use: that would wait for them
     auto ask = [&]() {
         if (in && asked < mine) {
             if (has_y) slots.ask(into, 0, (const T*)a.dy + next);
@@ -318,7 +318,9 @@ __global__ void __launch_bounds__(BLOCK, 512 / BLOCK) backward_vec(const Args a)
             st_next = __ldg(a.stats + r);
             if (a.fmt) {
                 const unsigned char* sc = a.scales + r * blocks + (t >> 2);
-                sc_next = (has_h ? __ldg(sc) : 0u) | (has_u ? __ldg(sc + nb) : 0u) << 8 | (a.gate_full ? __ldg(sc + 2 * nb) : 0u) << 16;
+                if (has_h) sc_x = __ldg(sc);
+                if (has_u) sc_u = __ldg(sc + nb);
+                if (a.gate_full) sc_z = __ldg(sc + 2 * nb);
             }
         }
     };
@@ -360,7 +362,7 @@ __global__ void __launch_bounds__(BLOCK, 512 / BLOCK) backward_vec(const Args a)
     for (int it = 0; it < count; ++it) {
         const bool on = in && it < mine;
         const float4 st = st_next;
-        const unsigned sc = sc_next;
+        const int e_x = (int)sc_x - 127, e_u = (int)sc_u - 127, e_z = (int)sc_z - 127;
         float2 g[4], dh[4], y[4], u[4], z[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) g[k] = dh[k] = y[k] = u[k] = z[k] = f2(0.0f);      // a slot without a row adds nothing
@@ -368,9 +370,9 @@ __global__ void __launch_bounds__(BLOCK, 512 / BLOCK) backward_vec(const Args a)
         if (on) {
             if (has_h) slots.take(from, 1, dh);
             if (a.fmt) {
-                if (has_h) slots.take_codes(from, 2, (int)(sc & 255u) - 127, a.fmt, y);
-                if (has_u) slots.take_codes(from, 3, (int)(sc >> 8 & 255u) - 127, a.fmt, u);
-                if (a.gate_full) slots.take_codes(from, 4, (int)(sc >> 16 & 255u) - 127, a.fmt, z);
+                if (has_h) slots.take_codes(from, 2, e_x, a.fmt, y);
+                if (has_u) slots.take_codes(from, 3, e_u, a.fmt, u);
+                if (a.gate_full) slots.take_codes(from, 4, e_z, a.fmt, z);
             } else {
                 if (has_h) slots.take(from, 2, y);
                 if (has_u) slots.take(from, 3, u);
