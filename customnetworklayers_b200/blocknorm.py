@@ -93,13 +93,16 @@ def forward(x, u, gate, scale, weight, bias, next_weight, next_bias, kind="rms",
     return y, h, stats, codes, scales
 
 
+def _contiguous(*tensors):
+    return [None if t is None else t.contiguous() for t in tensors]
+
+
 class BlockNormFunction(Function):
     """forward(x, u, gate, scale, weight, bias, next_weight, next_bias, kind, eps, gate_kind, fmt) -> y, h or (y, h)."""
 
     @staticmethod
     def forward(ctx, x, u, gate, scale, weight, bias, next_weight, next_bias, kind, eps, gate_kind, fmt):
-        x, u, gate, scale, weight, bias, next_weight, next_bias = (
-            None if t is None else t.contiguous() for t in (x, u, gate, scale, weight, bias, next_weight, next_bias))
+        x, u, gate, scale, weight, bias, next_weight, next_bias = _contiguous(x, u, gate, scale, weight, bias, next_weight, next_bias)
         y, h, stats, codes, scales = forward(x, u, gate, scale, weight, bias, next_weight, next_bias, kind, eps, gate_kind, fmt, True)
         mode, groups = _gate_mode(x, gate)
         packed = fmt is not None
@@ -155,7 +158,7 @@ def pre_norm(x, weight, bias=None, *, kind: str = "rms", eps: float = 1e-6, chec
     if wants_grad(x, weight, bias):
         return BlockNormFunction.apply(x, None, None, None, None, None, weight, bias, kind, eps, "sigmoid", checkpoint)
     format_code(checkpoint)
-    return forward(x.contiguous(), None, None, None, None, None, weight, bias, kind, eps)[1]
+    return forward(*_contiguous(x, None, None, None, None, None, weight, bias), kind, eps)[1]
 
 
 def residual_norm(x, u, weight, bias=None, *, gate=None, gate_kind: str = "sigmoid", scale=None, next_weight=None, next_bias=None,
@@ -164,8 +167,7 @@ def residual_norm(x, u, weight, bias=None, *, gate=None, gate_kind: str = "sigmo
     if wants_grad(x, u, weight, bias, gate, scale, next_weight, next_bias):
         return BlockNormFunction.apply(x, u, gate, scale, weight, bias, next_weight, next_bias, kind, eps, gate_kind, checkpoint)
     format_code(checkpoint)
-    y, h = forward(x.contiguous(), u.contiguous(), None if gate is None else gate.contiguous(), scale, weight, bias, next_weight,
-                   next_bias, kind, eps, gate_kind)[:2]
+    y, h = forward(*_contiguous(x, u, gate, scale, weight, bias, next_weight, next_bias), kind, eps, gate_kind)[:2]
     return y if h is None else (y, h)
 
 

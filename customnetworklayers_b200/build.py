@@ -7,6 +7,8 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -17,7 +19,7 @@ SOURCES = ["common.cu", "tv_fista.cu", "tv_fused.cu", "tv_flow.cu", "peer_allred
 HEADERS = ["common.h", "tv_math.cuh", "tv_fused.cuh", "tv_tile.cuh", "tgv_vec.cuh", "dtypes.cuh", "ckpt8.cuh", "blocknorm.cuh", "linattn.cuh",
            os.path.join("..", "..", "include", "cnl_b200.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-              "-Xcompiler", "-fPIC", "-shared", "--cudart", "shared"]
+              "-Xcompiler", "-fPIC", "--cudart", "shared"]
 
 
 def _nvcc() -> str:
@@ -39,12 +41,18 @@ def build(force: bool = False, verbose: bool = False) -> str:
     """Compiles every .cu of the package into libcnl_b200.so; returns the library path."""
     if not force and not needs_build():
         return LIB_PATH
-    cmd = [_nvcc()] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else [])
-    cmd += [os.path.join(CSRC, s) for s in SOURCES] + ["-o", LIB_PATH]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if verbose or res.returncode != 0:
+    flags = NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else [])
+    with tempfile.TemporaryDirectory() as tmp:                    # every source on its own, as many at a time as there are cores
+        objects = [os.path.join(tmp, s + ".o") for s in SOURCES]
+        cmds = [[_nvcc()] + flags + ["-c", os.path.join(CSRC, s), "-o", o] for s, o in zip(SOURCES, objects)]
+        with ThreadPoolExecutor(max(1, os.cpu_count() or 1)) as pool:
+            results = list(pool.map(lambda c: subprocess.run(c, capture_output=True, text=True), cmds))
+        if all(r.returncode == 0 for r in results):
+            results.append(subprocess.run([_nvcc()] + NVCC_FLAGS + ["-shared"] + objects + ["-o", LIB_PATH], capture_output=True, text=True))
+    failed = [r for r in results if r.returncode != 0]
+    for res in results if verbose else failed:
         sys.stderr.write(res.stdout + res.stderr)
-    if res.returncode != 0:
+    if failed:
         raise RuntimeError("nvcc failed building libcnl_b200.so")
     return LIB_PATH
 

@@ -40,8 +40,6 @@ def _check(q, k, v, log_decay, state, lengths, dims: int):
         if t.stride(-1) != 1 and t.shape[-1] > 1:
             raise RuntimeError(f"the last dimension of {name} must be contiguous")
     check_tensor(log_decay, "log_decay", torch.float32, q.device, (h,))
-    if log_decay.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("log_decay is a constant of the layer: there is no gradient for it")
     if state is not None:
         check_tensor(state, "state", torch.float32, q.device, (q.shape[0], h, dk, dv))
     if lengths is not None:
@@ -124,9 +122,12 @@ def linear_attention(q, k, v, log_decay, *, state=None, lengths=None, scale: Opt
     """q, k [B, T, H, Dk], v [B, T, H, Dv] -> (out [B, T, H, Dv], end state [B, H, Dk, Dv] fp32).
 
     log_decay [H] fp32, at most 0, is a constant; state (optional) is what came before; lengths [B] int32 (optional): tokens
-    at or behind a sequence's length are ignored and give zeros.  scale defaults to Dk ** -0.5."""
-    if wants_grad(q, k, v, state, log_decay):
-        _check(q, k, v, log_decay, None, lengths, 4) if log_decay.requires_grad else None
+    at or behind a sequence's length are not read and give zeros (values are held to 0..T).  scale defaults to Dk ** -0.5.
+    A token that is not finite makes all later outputs of its head not finite, and may make those of up to 127 earlier ones
+    (a chunk meets as one product); sequences of the batch do not touch one another."""
+    if log_decay.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("log_decay is a constant of the layer: there is no gradient for it")
+    if wants_grad(q, k, v, state):
         return LinearAttentionFunction.apply(q, k, v, log_decay, state, lengths, scale)
     return forward(_rows(q), _rows(k), _rows(v), log_decay, None if state is None else state.contiguous(), lengths, scale)[:2]
 

@@ -312,6 +312,46 @@ def test_same_bits_every_call_and_on_another_stream():
 
 
 @pytest.mark.gpu
+def test_elements_past_32_bits():
+    d, rows = 8192, 2 ** 18 + 3                           # 2^31 elements and three rows
+    x = torch.zeros(rows, d, dtype=torch.bfloat16, device="cuda")
+    tail = torch.randn(5, d, device="cuda").bfloat16()
+    x[-5:] = tail
+    w = torch.linspace(0.5, 1.5, d, device="cuda").bfloat16()
+    with torch.no_grad():
+        assert torch.equal(blocknorm.pre_norm(x, w)[-5:], blocknorm.pre_norm(tail, w))
+        x = x.view(-1, 4096)
+        assert torch.equal(blocknorm.pre_norm(x, w[:4096].clone())[-10:], blocknorm.pre_norm(tail.view(-1, 4096), w[:4096].clone()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [None, "int8"])
+def test_forward_and_backward_in_a_graph(fmt):
+    t, up = make((300, 72), torch.bfloat16, seed=12)
+    dev = {k: v.cuda().requires_grad_(True) for k, v in t.items()}
+    up = {k: v.cuda() for k, v in up.items()}
+
+    def once():
+        y, h = blocknorm.residual_norm(dev["x"], dev["u"], dev["weight"], dev["bias"], gate=dev["gate"], scale=dev["scale"],
+                                       next_weight=dev["next_weight"], next_bias=dev["next_bias"], checkpoint=fmt)
+        g = torch.autograd.grad((y, h), list(dev.values()), (up["dy"], up["dh"]))
+        return [y.detach(), h.detach(), *g]               # no eager graph of these leaves lives on while a capture runs
+
+    want = [o.clone() for o in once()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = once()
+    keep = up["dh"].clone()
+    up["dh"].zero_()
+    graph.replay()
+    assert not torch.equal(got[2], want[2])
+    up["dh"].copy_(keep)
+    graph.replay()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_refusals_on_the_device():
     x = torch.randn(4, 16, device="cuda")
     w = torch.ones(16, device="cuda")

@@ -109,7 +109,7 @@ def test_zeros_limits_and_elements_that_are_not_finite(fmt, dtype):
 def test_empty_and_large():
     empty = ckpt8.store(torch.empty(0, 5, device="cuda"))
     assert ckpt8.restore(empty).shape == (0, 5)
-    n = 32 * 40_000_000 + 7                             # byte offsets past 2^31
+    n = 2 ** 31 + 39                                    # elements and code bytes past 2^31
     x = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
     x[-3:] = torch.tensor([3.0, -127.0, 0.5])
     x[2 ** 30] = 5.0

@@ -121,6 +121,26 @@ def test_segments(t, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dk,dv", [(64, 64), (40, 56), (128, 128), (64, 128), (128, 64), (72, 40), (48, 104)])
+@pytest.mark.parametrize("t", [128, 129, 255, 256, 257, 640, 1001])
+def test_chunks_of_wide_heads(t, dk, dv):
+    """Sizes of the kernel with 128-token chunks: whole and cut chunks, one and several segments, both directions."""
+    check(1, t, 3, dk, dv, torch.bfloat16, seed=t + dk, state=t % 2 == 0)
+    check(2, t, 2, dk, dv, torch.bfloat16, lengths=[t - 1, max(t - 130, 0)], seed=t + dv)
+    assert _lib.load().cnl_linattn_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", DT)
+def test_so_many_heads_that_no_sequence_is_cut(d, dtype):
+    codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    assert _lib.load().cnl_linattn_segments(10, 300, 74, d, d, codes[dtype]) == 1
+    decay = -torch.exp2(-torch.linspace(0.0, 9.0, 74))
+    check(10, 300, 74, d, d, dtype, decay=decay, seed=d, lengths=[300, 299, 0, 1, 128, 129, 256, 257, 127, 300])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("lengths", [[0, 1, 600], [600, 599, 257], [0, 0, 0], [256, 255, 128]])
 def test_ragged_batches(lengths, dtype):
