@@ -71,7 +71,7 @@ int run_scan(float* local, const float* init, float* last, const float* log_deca
 // ---- one token --------------------------------------------------------------------------------------------------
 // S <- l S + k v^T in place, o = scale q^T S.  One block a head; reads and writes the state once: HBM bound, 8 dk dv bytes.
 template <typename T, int V>
-__global__ void __launch_bounds__(256) step_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
+__global__ void __launch_bounds__(256, 4) step_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
                                                    const float* __restrict__ log_decay, float* __restrict__ state, T* __restrict__ out,
                                                    int h, int dk, int dv, int cols, float scale, long long qb, long long qh, long long kb,
                                                    long long kh, long long vb, long long vh) {
@@ -95,21 +95,32 @@ __global__ void __launch_bounds__(256) step_kernel(const T* __restrict__ q, cons
     __syncthreads();
     float* s = state + bh * dk * dv + x;
     if (live) {
-#pragma unroll 8
-        for (int y = ty; y < dk; y += rows) {
-            float w[V];
-            if constexpr (V == 4) {
-                const float4 f = *reinterpret_cast<const float4*>(s + (long long)y * dv);
-                w[0] = f.x; w[1] = f.y; w[2] = f.z; w[3] = f.w;
-            } else w[0] = s[(long long)y * dv];
-            const float kk = sk[y], qq = sq[y];
+        constexpr int kAhead = 8;                                // rows of the state asked for together
+        for (int y0 = ty; y0 < dk; y0 += kAhead * rows) {
+            float w[kAhead][V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                w[i] = fmaf(l, w[i], kk * vv[i]);
-                acc[i] = fmaf(qq, w[i], acc[i]);
+            for (int k = 0; k < kAhead; ++k) {
+                const int y = y0 + k * rows;
+                if (y < dk) {
+                    if constexpr (V == 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(s + (long long)y * dv);
+                        w[k][0] = f.x; w[k][1] = f.y; w[k][2] = f.z; w[k][3] = f.w;
+                    } else w[k][0] = s[(long long)y * dv];
+                }
             }
-            if constexpr (V == 4) *reinterpret_cast<float4*>(s + (long long)y * dv) = make_float4(w[0], w[1], w[2], w[3]);
-            else s[(long long)y * dv] = w[0];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int y = y0 + k * rows;
+                if (y >= dk) break;
+                const float kk = sk[y], qq = sq[y];
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    w[k][i] = fmaf(l, w[k][i], kk * vv[i]);
+                    acc[i] = fmaf(qq, w[k][i], acc[i]);
+                }
+                if constexpr (V == 4) *reinterpret_cast<float4*>(s + (long long)y * dv) = make_float4(w[k][0], w[k][1], w[k][2], w[k][3]);
+                else s[(long long)y * dv] = w[k][0];
+            }
         }
     }
 #pragma unroll
