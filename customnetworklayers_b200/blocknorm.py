@@ -55,7 +55,10 @@ def _check(x, u, gate, scale, weight, bias, next_weight, next_bias):
         check_tensor(u, "u", x.dtype, device, x.shape)
     if gate is not None:
         check_tensor(gate, "gate", x.dtype, device)
-    wdtype = (weight if weight is not None else next_weight).dtype
+    first = weight if u is not None else next_weight
+    if first is None:
+        raise RuntimeError("a norm needs its weight")
+    wdtype = first.dtype
     if wdtype not in (x.dtype, torch.float32):
         raise RuntimeError(f"parameters must be {x.dtype} or float32, not {wdtype}")
     for t, name in ((scale, "scale"), (weight, "weight"), (bias, "bias"), (next_weight, "next_weight"), (next_bias, "next_bias")):

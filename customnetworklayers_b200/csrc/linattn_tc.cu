@@ -20,6 +20,8 @@
 // copies and products have ended.
 #include <cuda.h>
 
+#include <atomic>
+
 #include "linattn.cuh"
 
 namespace cnl {
@@ -735,13 +737,14 @@ using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*
                             CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 int encoder(Encode* out) {
-    static Encode fn = nullptr;
+    static std::atomic<Encode> known{nullptr};
+    Encode fn = known.load();
     if (!fn) {
         void* p = nullptr;
         cudaDriverEntryPointQueryResult found;
         CNL_TRY(check_cuda(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found), "cudaGetDriverEntryPoint"));
         if (!p || found != cudaDriverEntryPointSuccess) return fail(CNL_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
-        fn = reinterpret_cast<Encode>(p);
+        known.store(fn = reinterpret_cast<Encode>(p));
     }
     *out = fn;
     return CNL_OK;

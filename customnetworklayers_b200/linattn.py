@@ -13,6 +13,7 @@ from typing import Optional
 import torch
 from torch import nn
 from torch.autograd import Function
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._tensor import DTYPES, check_tensor, first_order, launch, on_device, ptr, wants_grad
@@ -146,6 +147,8 @@ def step(q, k, v, log_decay, state, *, scale: Optional[float] = None):
     launch("linear attention step", _lib.load().cnl_linattn_step, q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(),
            _strides(q, k, v), log_decay.data_ptr(), state.data_ptr(), out.data_ptr(), b, h, dk, dv,
            dk ** -0.5 if scale is None else float(scale), DTYPES[q.dtype])
+    if not state.is_inference():
+        increment_version(state)                 # a graph that has kept this state refuses to use it, as after any in-place call
     return out
 
 

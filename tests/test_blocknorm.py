@@ -359,6 +359,7 @@ def test_refusals_on_the_device():
                  lambda: blocknorm.residual_norm(x, x, w[:8].clone()), lambda: blocknorm.residual_norm(x, x, w.half()),
                  lambda: blocknorm.residual_norm(x, x, w, next_bias=w), lambda: blocknorm.residual_norm(x, x, w, gate=x[:2]),
                  lambda: blocknorm.pre_norm(torch.randn(2, 8200, device="cuda"), torch.ones(8200, device="cuda")),
-                 lambda: blocknorm.pre_norm(x.double(), w.double())):
+                 lambda: blocknorm.pre_norm(x, None), lambda: blocknorm.residual_norm(x, x, None),
+                 lambda: blocknorm.residual_norm(x, x, None, next_weight=w), lambda: blocknorm.pre_norm(x.double(), w.double())):
         with pytest.raises(RuntimeError):
             call()

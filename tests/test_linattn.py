@@ -413,3 +413,62 @@ def test_refusals_on_the_device():
                  lambda: linattn.step(x[:, 0].clone().requires_grad_(True), x[:, 0], x[:, 0], decay, torch.zeros(2, 2, 8, 8, device="cuda"))):
         with pytest.raises(RuntimeError):
             call()
+
+
+@pytest.mark.gpu
+def test_a_step_shows_in_the_state_it_writes():
+    # a graph that has kept the state must not read what a later step has made of it
+    b, t, h, d = 2, 5, 2, 16
+    q, k, v = (torch.randn(b, t, h, d, device="cuda") for _ in range(3))
+    decay = torch.full((h,), -0.1, device="cuda")
+    state = torch.randn(b, h, d, d, device="cuda")
+    q.requires_grad_(True)
+    o, _ = linattn.linear_attention(q, k, v, decay, state=state)
+    with torch.no_grad():
+        linattn.step(q[:, 0], k[:, 0], v[:, 0], decay, state)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        o.sum().backward()
+    with torch.inference_mode():
+        own = state.clone()
+        linattn.step(k[:, 0], k[:, 0], v[:, 0], decay, own)
+        linattn.step(k[:, 0], k[:, 0], v[:, 0], decay, state.detach())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_two_streams_at_once_and_two_graphs(dtype):
+    b, t, h, d = 1, 900, 6, 64
+    decay = -torch.exp2(-torch.linspace(1, 6, h)).cuda()
+    sets = [[torch.randn(b, t, h, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(s + i)).to(dtype) for i in range(4)]
+            for s in (0, 10)]
+
+    def both(q, k, v, g):
+        o, e, s = linattn.forward(q, k, v, decay)
+        return (o, e, *linattn.backward(g, None, q, k, v, decay, None, None, s))
+
+    alone = [both(*x) for x in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    together = []
+    for _ in range(4):
+        for stream, x in zip(streams, sets):
+            with torch.cuda.stream(stream):
+                together.append(both(*x))
+    torch.cuda.synchronize()
+    for i, got in enumerate(together):
+        assert all(torch.equal(a, c) for a, c in zip(got, alone[i % 2]))
+    graphs, outs = [], []
+    for x in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(both(*x))
+    for order in ((0, 1), (1, 0)):
+        for stream, i in zip(streams, order):
+            with torch.cuda.stream(stream):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            assert all(torch.equal(a, c) for a, c in zip(outs[i], alone[i]))
+            for a in outs[i]:
+                a.zero_()
+        torch.cuda.synchronize()
