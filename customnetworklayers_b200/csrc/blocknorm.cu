@@ -182,6 +182,9 @@ __device__ __forceinline__ void center(float (&v)[K], const Args& a, int t, floa
 }
 
 // ---- forward ----------------------------------------------------------------------------------------------------
+// Here without vectors: one element a lane and load, so that loads and conversions, not memory, are the bound.  Forward /
+// backward: 21996 x 150 fp32 33 / 65 us, 61440 x 501 bf16 218 / 530 us (1.4 and 0.9 TB/s); with vectors, 3840 x 8192 fp32, 172 / 687 us
+// (one block of 1024 threads an SM, whose row sums meet at a barrier, is all that the registers of such a row allow).
 template <typename T, bool VEC, bool WIDE, int BLOCK>
 __global__ void __launch_bounds__(BLOCK, BLOCK <= 256 ? 3 : 1) forward_kernel(const Args a) {
     __shared__ float sm[2 * 32 * 2];

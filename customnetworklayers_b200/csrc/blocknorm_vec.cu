@@ -5,6 +5,10 @@
 // keeps 8 channels in pairs (packed fp32 arithmetic takes two a slot), the parameters of its channels in registers, folded
 // (s w and s b, since s, w, b only appear so), and rows arrive by cp.async in shared-memory slots that belong to one thread
 // each: it waits for its own copies, needs no barrier, and STAGES - 1 rows are under way while one is worked on.
+// 61440 x 512 bf16 with a full gate: rms forward 60 us (5.2 TB/s, 0.8 of a copy), layer norm with biases 84 us (two blocks an SM
+// instead of three; three with spills 90); backward 160 and 167 us (3.0 TB/s); with 8-bit checkpoints 117 and 187 us.  Wide or
+// narrow rows run alike (32: 64 and 153, 4096: 74 and 196 us for as many elements).  Instructions issue on half of the cycles at 16
+// warps an SM; mean and squares in one way through the row instead of two left all of these times as they are.
 #include "blocknorm.cuh"
 
 namespace cnl {

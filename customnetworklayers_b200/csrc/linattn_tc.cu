@@ -16,6 +16,11 @@
 // c (DC = 64) two parts fill the 128 rows of T, so W is kept in two addends, which X meets side by side; three parts are
 // (c0 | c1 / 2) and (c1 / 2 | c2).  With 128 columns the parts add up in T.
 //
+// Measured, bf16 (one sweep with its outputs; the sums of all launches of a call are in the drivers' comment): 1 x 122880 tokens
+// x 8 heads of 64 122 us (rows 252 MB in and out: 2.1 TB/s), 8 x 7680 x 8 x 128 117 us.  Tensor
+// pipes are active on 24 to 32 % of cycles, instructions issue on 36 to 42 %: what bounds a chunk is the chain weights -> P ->
+// outputs with 16 warps to hide it, and the operands' way through shared memory; a second block would not fit either memory.
+//
 // Every wait is bounded: a block that gives up marks the status word, fills what it owes with NaN, and returns after its
 // copies and products have ended.
 #include <cuda.h>
@@ -352,12 +357,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
         {
             const float* w0 = s.start ? s.start + ((long long)bh * s.segments + seg) * size : nullptr;
             const bool has = w0 && wrow < dc && (!kStack || row < 64);
+            // (a transposed state by vectors, as its rows lie apart: 8 x 7680 x 8 x 128, 1 float at a time 131 us, 4 at a time 119 us)
+            if (s.transposed && ((unsigned long long)w0 & 15) == 0) {
 #pragma unroll
-            for (int x = 0; x < HC; ++x) {
-                const int i = wcol + x;
-                const float v = has && i < da ? (s.transposed ? w0[(long long)wrow * da + i] : w0[(long long)i * dc + wrow]) : 0.0f;
-                if (x & 1) w[x / 2].y = v;
-                else w[x / 2].x = v;
+                for (int x = 0; x < HC; x += 4) {
+                    const float4 f = has && wcol + x < da ? *reinterpret_cast<const float4*>(w0 + (long long)wrow * da + wcol + x) : make_float4(0, 0, 0, 0);
+                    w[x / 2] = make_float2(f.x, f.y);
+                    w[x / 2 + 1] = make_float2(f.z, f.w);
+                }
+            } else {
+#pragma unroll
+                for (int x = 0; x < HC; ++x) {
+                    const int i = wcol + x;
+                    const float v = has && i < da ? (s.transposed ? w0[(long long)wrow * da + i] : w0[(long long)i * dc + wrow]) : 0.0f;
+                    if (x & 1) w[x / 2].y = v;
+                    else w[x / 2].x = v;
+                }
             }
         }
         auto four = [](const float2* v) {                        // eight numbers as a 16-byte piece
@@ -531,6 +546,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
 
 // A thread's share of W^T as a sweep begins and ends: a row of it (a column of c) and HC of its columns.  kStack: rows 64..127 are
 // a second addend, which starts at 0 and meets the first in `room` (256 da bytes of shared memory, free by then).
+// (no sweep that makes a state begins from a transposed one)
 template <int HC, bool kStack>
 __device__ __forceinline__ void take_start(const Sweep& s, int row, int wcol, float2 (&w)[HC / 2]) {
     const int wrow = kStack ? row & 63 : row;
@@ -539,7 +555,7 @@ __device__ __forceinline__ void take_start(const Sweep& s, int row, int wcol, fl
 #pragma unroll
     for (int x = 0; x < HC; ++x) {
         const int i = wcol + x;
-        const float v = has && i < s.da ? (s.transposed ? w0[(long long)wrow * s.da + i] : w0[(long long)i * s.dc + wrow]) : 0.0f;
+        const float v = has && i < s.da ? w0[(long long)i * s.dc + wrow] : 0.0f;
         if (x & 1) w[x / 2].y = v;
         else w[x / 2].x = v;
     }
@@ -809,6 +825,9 @@ int run_tc(Sweep s, cudaStream_t st) {
     return exact ? launch_state<DA, DC, 3>(s, st) : launch_state<DA, DC, 2>(s, st);
 }
 
+// Measured against the mma.sync sweep (forward / backward, us): 64 x 128 tokens x 8 heads of 128 65 / 95 against 64 / 169, of 64
+// 33 / 75 against 29 / 73; 1 x 128 of 64 11 / 26 against 12 / 34; 16 x 1024 of 64 31 / 73 against 65 / 146; 8 x 7680 of 128
+// 190 / 403 against 474 / 1146.  Heads of 32 would fill half of its tiles; shorter sequences less than one chunk.
 bool tc_sizes(int t, int da, int dc, int dtype) { return dtype == CNL_BF16 && t >= kTok && da > 32 && dc > 32 && da % 8 == 0 && dc % 8 == 0; }
 
 bool tc_serves(const Sweep& s, int dtype) {
