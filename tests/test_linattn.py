@@ -141,6 +141,30 @@ def test_so_many_heads_that_no_sequence_is_cut(d, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("state", [True, False])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (64, 128), (128, 64), (128, 128), (40, 72)])
+def test_segments_of_many_chunks(dk, dv, state):
+    # so many heads that a segment is five or six chunks long, the last of them cut; three sequences, each in many copies
+    t, h, dtype = 1300, 2, torch.bfloat16
+    x, _, do, ds = make(3, t, h, dk, dv, dtype, seed=dk + dv, state=state)
+    decay, n, sc = torch.tensor([-2.0 ** -9, -0.02]), torch.tensor([1300, 1111, 770], dtype=torch.int32), dk ** -0.5
+    copy = torch.arange(37) % 3
+    dev = {k: None if v is None else v[copy].cuda().requires_grad_(True) for k, v in x.items()}
+    o, end = linattn.linear_attention(dev["q"], dev["k"], dev["v"], decay.cuda(), state=dev["state"], lengths=n[copy].cuda())
+    leaves = [k for k in x if x[k] is not None]
+    got = (o, end, *torch.autograd.grad((o, end), [dev[k] for k in leaves], (do[copy].cuda(), ds[copy].cuda())))
+    ref = {k: None if v is None else v.double().requires_grad_(True) for k, v in x.items()}
+    ro, rend = attention(ref["q"], ref["k"], ref["v"], decay.double(), ref["state"], n, sc)
+    exact = (ro, rend, *torch.autograd.grad((ro, rend), [ref[k] for k in leaves], (do.double(), ds.double())))
+    mags = bounds(x, decay, do, ds, n, sc, dtype)
+    for name, g, r, m in zip(["out", "end state"] + leaves, got, exact, mags):
+        assert torch.equal(g, g[:3][copy])                            # copies, wherever they ran
+        in_fp32 = name in ("end state", "state")                      # never rounded to 16 bits
+        bound = m / (2 * HALF[dtype] + 512 * 2.0 ** -24) * 512 * 2.0 ** -24 + 1e-30 if in_fp32 else HALF[dtype] * r.abs() + m + TINY[dtype]
+        assert_within(g[:3], r, bound, name)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("lengths", [[0, 1, 600], [600, 599, 257], [0, 0, 0], [256, 255, 128]])
 def test_ragged_batches(lengths, dtype):
