@@ -38,18 +38,15 @@ int ensure_dynamic_smem(const void* kernel, int bytes) {
 }
 
 int sm_count(int* out) {
-    static std::mutex mu;
-    static std::map<int, int> known;                             // device -> multiprocessors
+    static std::atomic<int> known[64];                           // by device; 0: not asked yet
     int dev = 0;
     CNL_TRY(check_cuda(cudaGetDevice(&dev), "cudaGetDevice"));
-    std::lock_guard<std::mutex> lock(mu);
-    auto it = known.find(dev);
-    if (it == known.end()) {
-        int n = 0;
+    int n = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+    if (n == 0) {
         CNL_TRY(check_cuda(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute"));
-        it = known.emplace(dev, n).first;
+        if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
     }
-    *out = it->second;
+    *out = n;
     return CNL_OK;
 }
 
