@@ -11,11 +11,13 @@
 // c of the state is split into parts of the type (one part would be off by 1.6e-3): fp16 into two, 22 bits, the second times
 // 2^11 and summed apart, so that it does not fall under fp16's range; bf16 into two (16 bits, 7e-7 rms) where W only feeds
 // rounded outputs, and into all three where a caller gets the state (EXACT).  A chunk is summed apart and added to W by one
-// rounded multiply-add, because the tensor cores truncate their sums.  fp16's range: W is brought to at most 2^8 by a power
-// of two for its product (the sum over a head can leave the range that the inputs are in), P carries the whole scale of its
-// outputs.
+// rounded multiply-add, because the tensor cores truncate their sums.  fp16's range: W is brought to at most 2^15 by a power
+// of two for its product (the sum over a head can leave the range that the inputs are in, and a column that is small beside
+// its neighbours keeps 2^-40 of their largest).  P, a product of two rows that may each be near either end, stays fp32 in
+// shared memory and meets c as two parts in tf32, which has fp32's range and holds fp16's values of c as they are.
 //
-// fp16, forward / backward: 8 x 7680 tokens x 8 heads of 128 474 / 1146 us, of 64 179 / 435 us, 4 x 7680 x 8 of 32 56 / 128 us; bound
+// fp16, forward / backward: 8 x 7680 tokens x 8 heads of 128 534 / 1317 us, of 64 204 / 512 us, 4 x 7680 x 8 of 32 62 / 142 us (with P
+// as two parts in fp16, which loses weights above 65504, 478 / 1148, 179 / 437 and 56 / 130 us); bound
 // by the legacy tensor path and the fragments' way through shared memory.  The tcgen05 sweep takes 190 / 403 and 118 / 245 us for
 // the same in bf16; fp16 stays here, where the state's second part can be summed apart.
 #include <type_traits>
@@ -45,11 +47,22 @@ __device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsig
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Eight rows summed: tf32, whose 11 significant bits are fp16's
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const unsigned (&a)[4], float2 b) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(__float_as_uint(b.x)), "r"(__float_as_uint(b.y)));
+}
+__device__ __forceinline__ unsigned to_tf32(float v) {
+    unsigned r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
+    return r;
+}
+
 template <int DA, int DC, bool OUT>
 struct Layout {                              // shared memory, in elements of the type
     static constexpr int ra = DA + kPad, rc = DC + kPad, rp = kChunk + kPad;
     static constexpr int a = 0, b = OUT ? kChunk * ra : 0, c = b + kChunk * ra, stage = c + kChunk * rc;
-    static constexpr int p = 2 * stage, p2 = kChunk * rp, o = p + (OUT ? 2 * p2 : 0);      // P's two parts
+    static constexpr int p = 2 * stage, p2 = kChunk * rp, o = p + (OUT ? 2 * p2 : 0);      // P's two parts, or P in fp32
     static constexpr bool own_o = OUT && DC > DA;              // otherwise outputs pass through the rows of a just read
     static constexpr int end = o + (own_o ? kChunk * rc : 0);
     static constexpr int bytes = (end * 2 + 15) / 16 * 16 + (3 * kChunk + 24) * 4;      // and the three tables of powers
@@ -182,17 +195,22 @@ __global__ void __launch_bounds__(2 * DC, DC == 128 ? 2 : DC == 64 ? 4 : 8) mma_
                     mma(acc[1], a, b[2], b[3], T());
                 }
                 const float* z = pz + (bi - bj) * 16 + g - q2;               // position i after position j: 8 h - 8 x - e more
-                T* to = P + (bi * 16 + g) * L::rp + bj * 16 + q2;
+                const int at = (bi * 16 + g) * L::rp + bj * 16 + q2;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
                     {
                         const float2 v = make_float2(acc[x][2 * h] * z[8 * h - 8 * x], acc[x][2 * h + 1] * z[8 * h - 8 * x - 1]);
-                        const unsigned top = pack2<T>(v.x, v.y);
-                        const float2 f = unpack2(top, T());
-                        *reinterpret_cast<unsigned*>(to + h * 8 * L::rp + x * 8) = top;
-                        *reinterpret_cast<unsigned*>(to + L::p2 + h * 8 * L::rp + x * 8) = pack2<T>(v.x - f.x, v.y - f.y);
+                        const int to = at + h * 8 * L::rp + x * 8;
+                        if constexpr (kHalf) {
+                            *reinterpret_cast<float2*>(reinterpret_cast<float*>(P) + to) = v;
+                        } else {
+                            const unsigned top = pack2<T>(v.x, v.y);
+                            const float2 f = unpack2(top, T());
+                            *reinterpret_cast<unsigned*>(P + to) = top;
+                            *reinterpret_cast<unsigned*>(P + L::p2 + to) = pack2<T>(v.x - f.x, v.y - f.y);
+                        }
                     }
             }
             __syncthreads();
@@ -206,8 +224,8 @@ __global__ void __launch_bounds__(2 * DC, DC == 128 ? 2 : DC == 64 ? 4 : 8) mma_
 #pragma unroll
                 for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
                 const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 100);
-                down = __uint_as_float((unsigned)(127 + 7 - ex) << 23);
-                up *= __uint_as_float((unsigned)(127 - 7 + ex) << 23);
+                down = __uint_as_float((unsigned)(127 + 14 - ex) << 23);
+                up *= __uint_as_float((unsigned)(127 - 14 + ex) << 23);
             }
             auto round = [&](float2 v) {
                 if constexpr (kHalf) v = __fmul2_rn(v, make_float2(down, down));
@@ -251,6 +269,27 @@ __global__ void __launch_bounds__(2 * DC, DC == 128 ? 2 : DC == 64 ? 4 : 8) mma_
                     for (int i = 0; i < 2; ++i) {
                         if (k > half * 2 + i) continue;
                         unsigned a[4];
+                        if constexpr (kHalf) {
+                            // columns 2 t and 2 t + 1 of 8 stand where the product sums over t and t + 4: c's pairs are there already
+                            const float* from = reinterpret_cast<const float*>(P) + (half * 32 + i * 16 + g) * L::rp + k * 16 + q2;
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const float2 p0 = *reinterpret_cast<const float2*>(from + e * 8), p1 = *reinterpret_cast<const float2*>(from + e * 8 + 8 * L::rp);
+                                const float v[4] = {p0.x, p1.x, p0.y, p1.y};
+                                unsigned small[4];
+#pragma unroll
+                                for (int x = 0; x < 4; ++x) {
+                                    a[x] = to_tf32(v[x]);
+                                    small[x] = to_tf32(v[x] - __uint_as_float(a[x]));
+                                }
+                                const float2 b0 = unpack2(b[e], T()), b1 = unpack2(b[2 + e], T());
+                                mma_tf32(o[i][0], small, b0);
+                                mma_tf32(o[i][1], small, b1);
+                                mma_tf32(o[i][0], a, b0);
+                                mma_tf32(o[i][1], a, b1);
+                            }
+                            continue;
+                        }
                         ldsm(a, P + (half * 32 + i * 16 + (lane & 15)) * L::rp + k * 16 + (lane >> 4) * 8);
                         mma(o[i][0], a, b[0], b[1], T());
                         mma(o[i][1], a, b[2], b[3], T());

@@ -496,3 +496,56 @@ def test_two_streams_at_once_and_two_graphs(dtype):
             for a in outs[i]:
                 a.zero_()
         torch.cuda.synchronize()
+
+
+# ---- products beyond fp16's range --------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("large", ["qk", "vdo"])
+@pytest.mark.parametrize("dk,dv", [(32, 32), (24, 120), (64, 64), (128, 64), (128, 128)])
+def test_products_beyond_the_range_of_fp16(dk, dv, large, dtype):
+    """scale q.k or v.do above 65504 with results in range: a prompt's weights, and gradients under a loss scale."""
+    t, decay = 200, torch.tensor([-0.1, -2.0 ** -9])
+    g = torch.Generator().manual_seed(dk + dv)
+    r = lambda d, size: (torch.randn(1, t, 2, d, generator=g, dtype=torch.float64) * size).to(dtype)  # noqa: E731
+    top = (2.0 ** 18 / (dk if large == "qk" else dv)) ** 0.5
+    size = [top, top, 2.0 ** -8, 2.0 ** -8] if large == "qk" else [2.0 ** -8, 2.0 ** -8, top, top]
+    q, k, v, do = (r(d, s) for d, s in zip((dk, dk, dv, dv), size))
+    if large == "qk":
+        q, k = q.abs(), k.abs()
+    else:
+        v, do = v.abs(), do.abs()
+    x = {"q": q, "k": k, "v": v, "state": torch.zeros(1, 2, dk, dv)}
+    ds = torch.zeros(1, 2, dk, dv)
+    f = {n: z.double().requires_grad_(True) for n, z in x.items()}
+    assert (torch.einsum("bihd,bjhd->bhij", *((q, k) if large == "qk" else (v, do))).double()).max() > 2 * 65504
+    ro, _ = attention(f["q"], f["k"], f["v"], decay.double(), f["state"], None, 1.0)
+    want = (ro, *torch.autograd.grad(ro, [f["q"], f["k"], f["v"]], do.double()))
+    assert all(0 < w.abs().max() < 65504 for w in want)
+    dev = {n: z.cuda().requires_grad_(True) for n, z in x.items()}
+    o, _ = linattn.linear_attention(dev["q"], dev["k"], dev["v"], decay.cuda(), state=dev["state"], scale=1.0)
+    got = (o, *torch.autograd.grad(o, [dev["q"], dev["k"], dev["v"]], do.cuda()))
+    mags = bounds(x, decay, do, ds, None, 1.0, dtype)
+    for name, a, w, m in zip(("out", "gradient of q", "gradient of k", "gradient of v"), got, want, [mags[0], *mags[2:5]]):
+        assert_within(a, w, HALF[dtype] * w.abs() + m + TINY[dtype], name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dk,dv", [(32, 32), (64, 64), (128, 128)])
+def test_small_fp16_gradients_that_meet_large_rows(dk, dv):
+    """Weights scale v.do of 2^-21 and below, of which fp16's own steps would keep three bits, times rows of 2^9: gradients
+    that fp16 holds in full.  No allowance for small weights."""
+    t, sc, decay = 200, 2.0 ** -10, torch.tensor([-0.1, -2.0 ** -9])
+    g = torch.Generator().manual_seed(dk)
+    r = lambda d, size: (torch.randn(1, t, 2, d, generator=g, dtype=torch.float64) * size).half()  # noqa: E731
+    x = {"q": r(dk, 2.0 ** 9), "k": r(dk, 2.0 ** 9), "v": r(dv, 2.0 ** -4), "state": torch.zeros(1, 2, dk, dv)}
+    do, ds = r(dv, 2.0 ** -10), torch.zeros(1, 2, dk, dv)
+    f = {n: z.double().requires_grad_(True) for n, z in x.items()}
+    ro, _ = attention(f["q"], f["k"], f["v"], decay.double(), f["state"], None, sc)
+    want = torch.autograd.grad(ro, [f["q"], f["k"], f["v"]], do.double())
+    dev = {n: z.cuda().requires_grad_(True) for n, z in x.items()}
+    o, _ = linattn.linear_attention(dev["q"], dev["k"], dev["v"], decay.cuda(), state=dev["state"], scale=sc)
+    got = torch.autograd.grad(o, [dev["q"], dev["k"], dev["v"]], do.cuda())
+    mags = bounds(x, decay, do, ds, None, sc, torch.float16)
+    for name, a, w, m in zip(("gradient of q", "gradient of k", "gradient of v"), got, want, mags[2:5]):
+        assert_within(a, w, HALF[torch.float16] * w.abs() + m + TINY[torch.float16], name)
