@@ -6,8 +6,8 @@
 // chunk: P = a b^T (ten 16 x 16 blocks at or under the diagonal, shared out over the warps), out = l^{i+off} (a W) + P c,
 // W = l^m W + (weighted c)^T b.  The next chunk's rows arrive by cp.async meanwhile.
 //
-// Roundings to the type: W where it meets the outputs, once, as the outputs themselves; P's weights go in two parts (a tenth
-// of the products: short sequences, which have nothing else, would lose 1.5 times what the outputs' own rounding costs).  The weighted
+// Roundings to the type: P and, where it meets the outputs, W go in two parts each, so that a result carries its own rounding
+// and little else (each rounded once, a result would be off by 1.4 times what its own rounding costs).  The weighted
 // c of the state is split into parts of the type (one part would be off by 1.6e-3): fp16 into two, 22 bits, the second times
 // 2^11 and summed apart, so that it does not fall under fp16's range; bf16 into two (16 bits, 7e-7 rms) where W only feeds
 // rounded outputs, and into all three where a caller gets the state (EXACT).  A chunk is summed apart and added to W by one
@@ -16,9 +16,9 @@
 // its neighbours keeps 2^-40 of their largest).  P, a product of two rows that may each be near either end, stays fp32 in
 // shared memory and meets c as two parts in tf32, which has fp32's range and holds fp16's values of c as they are.
 //
-// fp16, forward / backward: 8 x 7680 tokens x 8 heads of 128 534 / 1317 us, of 64 204 / 512 us, 4 x 7680 x 8 of 32 62 / 142 us (with P
-// as two parts in fp16, which loses weights above 65504, 478 / 1148, 179 / 437 and 56 / 130 us); bound
-// by the legacy tensor path and the fragments' way through shared memory.  The tcgen05 sweep takes 190 / 403 and 118 / 245 us for
+// fp16, forward / backward: 8 x 7680 tokens x 8 heads of 128 609 / 1541 us, of 64 222 / 566 us, 4 x 7680 x 8 of 32 65 / 148 us (with P
+// as two parts in fp16, which loses weights above 65504, and W as one, 478 / 1148, 179 / 437 and 56 / 130 us); bound
+// by the legacy tensor path and the fragments' way through shared memory.  The tcgen05 sweep takes 208 / 497 and 140 / 308 us for
 // the same in bf16; fp16 stays here, where the state's second part can be summed apart.
 #include <type_traits>
 
@@ -227,9 +227,12 @@ __global__ void __launch_bounds__(2 * DC, DC == 128 ? 2 : DC == 64 ? 4 : 8) mma_
                 down = __uint_as_float((unsigned)(127 + 14 - ex) << 23);
                 up *= __uint_as_float((unsigned)(127 - 14 + ex) << 23);
             }
-            auto round = [&](float2 v) {
+            auto round = [&](float2 v, unsigned& small) {            // W in two parts
                 if constexpr (kHalf) v = __fmul2_rn(v, make_float2(down, down));
-                return pack2<T>(v.x, v.y);
+                const unsigned top = pack2<T>(v.x, v.y);
+                const float2 f = unpack2(top, T());
+                small = pack2<T>(v.x - f.x, v.y - f.y);
+                return top;
             };
             // outputs pass through shared memory, so that a warp stores whole 32-byte pieces of its rows
             T* O = L::own_o ? sm + L::o : A;
@@ -244,11 +247,14 @@ __global__ void __launch_bounds__(2 * DC, DC == 128 ? 2 : DC == 64 ? 4 : 8) mma_
                     for (int e = 0; e < 4; ++e) o[i][0][e] = o[i][1][e] = 0.0f;
 #pragma unroll
                 for (int k = 0; k < KT; ++k) {
-                    const unsigned b00 = round(w[2 * k][0]), b01 = round(w[2 * k + 1][0]), b10 = round(w[2 * k][1]), b11 = round(w[2 * k + 1][1]);
+                    unsigned s00, s01, s10, s11;
+                    const unsigned b00 = round(w[2 * k][0], s00), b01 = round(w[2 * k + 1][0], s01), b10 = round(w[2 * k][1], s10), b11 = round(w[2 * k + 1][1], s11);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         unsigned a[4];
                         ldsm(a, A + (half * 32 + i * 16 + (lane & 15)) * L::ra + k * 16 + (lane >> 4) * 8);
+                        mma(o[i][0], a, s00, s01, T());
+                        mma(o[i][1], a, s10, s11, T());
                         mma(o[i][0], a, b00, b01, T());
                         mma(o[i][1], a, b10, b11, T());
                     }

@@ -11,10 +11,13 @@
 // of a chunk in their order in memory and turn the mask and the weights around instead.
 //
 // Operands: a and b for P, P, and W lie with the summed dimension contiguous; c, its parts, and b for T with it strided
-// (their rows are tokens), which the descriptors say.  The weighted c is split into two or three parts (roundings as in the
-// mma.sync kernel: P once, W once, the weighted c to 16 or, where the state is a result, 24 bits).  With up to 64 columns of
+// (their rows are tokens), which the descriptors say.  Roundings as in the mma.sync kernel, so that a result carries its own
+// rounding and little else: P and W are two bf16 parts each (16 bits; P's lie side by side in P's columns of tensor memory, W's
+// smaller one waits in the parts' room until X has read it), the weighted c two or, where the state is a result, three.  With up to 64 columns of
 // c (DC = 64) two parts fill the 128 rows of T, so W is kept in two addends, which X meets side by side; three parts are
-// (c0 | c1 / 2) and (c1 / 2 | c2).  With 128 columns the parts add up in T.
+// (c0 | c1 / 2) and (c1 / 2 | c2).  With 128 columns the parts add up in T.  P and W rounded once would take 10 to 13 % less time
+// (1 x 122880 x 8 x 64 forward 194 instead of 216 us, 8 x 7680 x 8 x 128 backward 451 instead of 497 us) at 1.4 times the error: 2.35e-3 rms of
+// the outputs against 1.66e-3, which the outputs' own rounding is.
 //
 // Measured, bf16 (one sweep with its outputs; the sums of all launches of a call are in the drivers' comment): 1 x 122880 tokens
 // x 8 heads of 64 122 us (rows 252 MB in and out: 2.1 TB/s), 8 x 7680 x 8 x 128 117 us.  Tensor
@@ -272,7 +275,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
     } else if (warp == kWorkers + 1) {
         // ---- products.  The warp runs as one, so that what the products are given is uniform; one lane issues them
         const bool one = elected();
-        const unsigned W = rows_word(base + M::w), Q = columns_word(base + M::parts);
+        const unsigned W = rows_word(base + M::w), Wlow = rows_word(base + M::parts), Q = columns_word(base + M::parts);
         for (int i = 0; i < chunks; ++i) {
             const unsigned ph = phase(i);
             const bool cut = hi - lo - i * kTok < kTok && !s.reversed;       // rows behind the end are cleared first
@@ -293,6 +296,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
             if (one) {
 #pragma unroll
                 for (int k = 0; k < DA / 16; ++k) tc_mma(tX, operand(A, (k / 4) * kBlk + (k % 4) * 32), operand(W, (k / 4) * kBlk + (k % 4) * 32), product(128, 0, 0), k > 0);
+#pragma unroll
+                for (int k = 0; k < DA / 16; ++k) tc_mma(tX, operand(A, (k / 4) * kBlk + (k % 4) * 32), operand(Wlow, (k / 4) * kBlk + (k % 4) * 32), product(DC, 0, 0), true);
                 tc_commit(bar(DONE_X, i));
             }
             __syncwarp();
@@ -300,7 +305,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
             tc_after();
             if (one) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) tc_mma_t(tO, tP + k * 8, operand(C, k * 2048), product(DC, 0, 1), k > 0);
+                for (int k = 0; k < 16; ++k) tc_mma_t(tO, tP + (k ^ 8) * 8, operand(C, (k & 7) * 2048), product(DC, 0, 1), k > 0);      // small parts first
                 tc_commit(bar(DONE_O, i));
             }
             __syncwarp();
@@ -378,6 +383,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
         auto four = [](const float2* v) {                        // eight numbers as a 16-byte piece
             return make_uint4(pack2<__nv_bfloat16>(v[0].x, v[0].y), pack2<__nv_bfloat16>(v[1].x, v[1].y), pack2<__nv_bfloat16>(v[2].x, v[2].y), pack2<__nv_bfloat16>(v[3].x, v[3].y));
         };
+        auto rest = [&](const float2* v, uint4 top) {            // what those leave of them
+            const unsigned t[4] = {top.x, top.y, top.z, top.w};
+            float2 r[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = unpack2(t[e], __nv_bfloat16());
+                r[e] = __fadd2_rn(v[e], make_float2(-f.x, -f.y));
+            }
+            return four(r);
+        };
         auto tell = [&](int kind, int i) {
             tc_before();
             __syncwarp();
@@ -387,7 +402,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
             const unsigned to = base + M::w + (DA == 128 ? (cq >> 1) * kBlk : 0) + row * 128;
             const int piece = DA == 128 ? (cq & 1) * 4 : cq * 2;
 #pragma unroll
-            for (int x = 0; x < HC / 8; ++x) smem_put(to + (((piece + x) ^ (row & 7)) << 4), four(w + 4 * x));
+            for (int x = 0; x < HC / 8; ++x) {
+                const unsigned at = to + (((piece + x) ^ (row & 7)) << 4);
+                const uint4 top = four(w + 4 * x);
+                smem_put(at, top);
+                if (!kStack || row < 64) smem_put(at + (M::parts - M::w), rest(w + 4 * x, top));
+            }
             fence_async();
             tell(HAS_W, i);
         };
@@ -416,10 +436,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
             // P: weights and mask; back into tensor memory, two columns in one, once the four warps of these lanes have read it
             if (!bar_wait(bar(DONE_P, i), ph, dead)) break;
             tc_after();
-            unsigned r[32], to[16];
+            unsigned r[32], to[16], low[16];
+            auto parts = [&](int x, float2 y) {
+                to[x] = pack2<__nv_bfloat16>(y.x, y.y);
+                const float2 f = unpack2(to[x], __nv_bfloat16());
+                y = __fadd2_rn(y, make_float2(-f.x, -f.y));
+                low[x] = pack2<__nv_bfloat16>(y.x, y.y);
+            };
             if (s.reversed ? cq < q : cq > q) {              // above the diagonal
 #pragma unroll
-                for (int x = 0; x < 16; ++x) to[x] = 0;
+                for (int x = 0; x < 16; ++x) to[x] = low[x] = 0;
             } else {
                 tc_load(tP + lanes + cq * 32, r);
                 tc_wait_load();
@@ -429,14 +455,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
                     for (int x = 0; x < 16; ++x) {
                         const float2 f = s.reversed ? make_float2(e[2 * x], e[2 * x + 1]) : make_float2(e[-2 * x], e[-2 * x - 1]);
                         const float2 y = __fmul2_rn(__fmul2_rn(make_float2(__uint_as_float(r[2 * x]), __uint_as_float(r[2 * x + 1])), make_float2(both, both)), f);
-                        to[x] = pack2<__nv_bfloat16>(y.x, y.y);
+                        parts(x, y);
                     }
                 } else {
 #pragma unroll
                     for (int x = 0; x < 16; ++x) {
                         const float2 f = *reinterpret_cast<const float2*>(whole + 2 * x);
                         const float2 y = __fmul2_rn(__fmul2_rn(make_float2(__uint_as_float(r[2 * x]), __uint_as_float(r[2 * x + 1])), make_float2(u, u)), f);
-                        to[x] = pack2<__nv_bfloat16>(y.x, y.y);
+                        parts(x, y);
                     }
                 }
             }
@@ -446,10 +472,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
             if (!bar_wait(read_p(q), (unsigned)i & 1u, dead)) break;
             tc_after();
             tc_store(tP + lanes + cq * 16, to);
+            tc_store(tP + lanes + 64 + cq * 16, low);
             tc_wait_store();
             tell(HAS_P, i);
             // the weighted c in parts
-            if (!bar_wait(bar(FULL_C, i), ph, dead)) break;
+            if (!bar_wait(bar(FULL_C, i), ph, dead) || !bar_wait(bar(DONE_X, i), ph, dead)) break;      // (X reads W's smaller part in their room)
             if (m < kTok) weigh(m);
 #pragma unroll
             for (int x = 0; x < DC / 64; ++x)
@@ -465,7 +492,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
             fence_async();
             tell(HAS_C, i);
             // out = l^{pos + off} X + O
-            if (!bar_wait(bar(DONE_X, i), ph, dead) || !bar_wait(bar(DONE_O, i), ph, dead)) break;
+            if (!bar_wait(bar(DONE_O, i), ph, dead)) break;
             tc_after();
             const bool live = pos < m, turned = token0(i) < 0;           // a TMA store must not start before the tensor
             if (M::through_c ? !bar_wait(bar(HAS_C, i), ph, dead)        // every warp has read c

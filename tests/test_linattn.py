@@ -549,3 +549,27 @@ def test_small_fp16_gradients_that_meet_large_rows(dk, dv):
     mags = bounds(x, decay, do, ds, None, sc, torch.float16)
     for name, a, w, m in zip(("gradient of q", "gradient of k", "gradient of v"), got, want, mags[2:5]):
         assert_within(a, w, HALF[torch.float16] * w.abs() + m + TINY[torch.float16], name)
+
+
+# ---- what 16-bit results are rounded by --------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dk,dv", [(32, 32), (40, 72), (64, 64), (64, 128), (128, 64), (128, 128)])
+@pytest.mark.parametrize("t", [127, 128, 700])
+def test_16_bit_results_carry_their_own_rounding_alone(t, dk, dv, dtype):
+    """Beside the rounding of the result: a chunk's weights, and the state where it meets a chunk, are held in two parts
+    (bf16: 2^-16 of a value each; fp16 2^-22), the values summed into the state likewise, whose smaller part may be rounded
+    once more: three such roundings of a term at most; then 32-bit sums."""
+    sc = dk ** -0.5
+    x, decay, do, ds = make(1, t, 3, dk, dv, dtype, seed=t + dk + dv)
+    f = {n: z.double().requires_grad_(True) for n, z in x.items()}
+    ro, rend = attention(f["q"], f["k"], f["v"], decay.double(), f["state"], None, sc)
+    want = (ro, *torch.autograd.grad((ro, rend), list(f.values())[:3], (do.double(), ds.double())))
+    dev = {n: z.cuda().requires_grad_(True) for n, z in x.items()}
+    o, end = linattn.linear_attention(dev["q"], dev["k"], dev["v"], decay.cuda(), state=dev["state"])
+    got = (o, *torch.autograd.grad((o, end), list(dev.values())[:3], (do.cuda(), ds.cuda())))
+    mags = bounds(x, decay, do, ds, None, sc, dtype)
+    part = HALF[dtype] ** 2
+    for name, a, w, m in zip(("out", "gradient of q", "gradient of k", "gradient of v"), got, want, [mags[0], *mags[2:5]]):
+        mag = m / (2 * HALF[dtype] + 512 * 2.0 ** -24)
+        assert_within(a, w, HALF[dtype] * w.abs() + (3 * part + 512 * 2.0 ** -24) * mag + TINY[dtype], name)
