@@ -6,7 +6,7 @@
 // 8 (fp32) neighbouring lanes and its maximum costs two or three shuffles; a thread's vectors are all loaded before the first
 // is used.  Addresses that are not 16-byte aligned take the same code with one element a lane.
 // 126 M elements: fp32 store and restore 100 us (6.3 TB/s, 0.96 of a copy), GELU and SiLU either way 170 to 175 us (1.0 of one);
-// 16 bits store 74 (int8) and 82 us (e4m3), restore 66, SiLU 104 and 98, GELU 111 and 125 us (0.76 to 0.98: conversions and the
+// 16 bits store 74 (int8) and 82 us (e4m3), restore 66, SiLU 104 and 98, GELU 113 and 125 us (0.76 to 0.98: conversions and the
 // error function issue beside the copies).
 #include "ckpt8.cuh"
 
@@ -21,7 +21,12 @@ constexpr int kThreads = 256;
 template <int ACT> constexpr int kUnrollOf = ACT ? 2 : 4;
 
 __device__ __forceinline__ float2 pair(float v) { return make_float2(v, v); }
-__device__ __forceinline__ float relu(float x) { return x > 0.0f ? x : (x == x ? 0.0f : x); }      // keeps NaN
+__device__ __forceinline__ float relu(float x) { return max_nan(x, 0.0f); }
+__device__ __forceinline__ float below_inf(float x) {                    // +inf as the largest number; NaN and -inf stay
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(3.402823466e38f));
+    return r;
+}
 
 // Phi(x) = exp(-x^2/2) t P(t) for x <= 0, t = 1 / (1 + 0.3 |x|), and 1 - that for x > 0.  P was fitted here to the scaled
 // complementary error function by least squares with weights moved towards an even relative error over |x| <= 14:
@@ -61,7 +66,8 @@ __device__ __forceinline__ float2 logistic(float2 x) {
 template <int ACT, typename T>
 __device__ __forceinline__ float2 act(float2 x) {
     if constexpr (ACT == CNL_ACT_GELU) {                                                 // x Phi(x) = max(x, 0) - |x| Phi(-|x|)
-        const float2 m = make_float2(fabsf(x.x), fabsf(x.y)), q = cdf_tail<T>(x, m);
+        // (a finite factor, so that the tail of +inf, which is 0, leaves +inf as it is; -inf times its Phi, 0, is NaN)
+        const float2 m = make_float2(fabsf(below_inf(x.x)), fabsf(below_inf(x.y))), q = cdf_tail<T>(x, m);
         return __ffma2_rn(make_float2(-m.x, -m.y), q, make_float2(relu(x.x), relu(x.y)));
     } else {
         return __fmul2_rn(x, logistic(x));

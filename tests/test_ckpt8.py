@@ -232,3 +232,22 @@ def test_quadfit_with_features_in_8_bits():
     assert_within(nchw(got[1]), want[1], 2.0 ** -24 * 64 * want[1].abs().max().double())
     with pytest.raises(RuntimeError, match="int8"):
         QuadFittingFromFlow("cuda", checkpoint="int5")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("kind", ["gelu", "silu"])
+@pytest.mark.parametrize("n", [8, 5])
+def test_activation_at_the_ends_of_the_line(n, kind, dtype):
+    """x Phi(x) and x sigmoid(x) at infinities, NaN and the type's largest values, aligned and not."""
+    top = torch.finfo(dtype).max
+    x = torch.tensor([float("inf"), float("-inf"), float("nan"), top, -top, 0.0, -0.0, 1.0][:n], dtype=dtype)
+    ref = act(x.double(), kind)
+    assert ref[0] == float("inf") and ref[3] == top and ref[4] == 0
+    for at in (0, 1):
+        dev = torch.zeros(n + 1, dtype=dtype, device="cuda")[at:at + n].copy_(x)
+        with torch.no_grad():
+            y = ckpt8.activation(dev, kind)
+        y2 = ckpt8.activation(dev.clone().requires_grad_(True), kind, "e4m3").detach()
+        for got in (y, y2):
+            assert_within(got, ref, 2.0 ** -18 * torch.ones(n, dtype=torch.float64) + HALF[dtype] * ref.abs().nan_to_num(0, 0, 0), "y")
