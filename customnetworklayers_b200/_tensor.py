@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -54,8 +55,14 @@ def launch(what: str, fn, device, *args) -> None:
         _lib.check(rc, what)
 
 
+def has_tangent(*tensors) -> bool:
+    """Whether a forward-mode derivative enters with one of the tensors."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether a derivative is asked for: a gradient, or a forward-mode one, which the autograd functions refuse."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or has_tangent(*tensors)
 
 
 def first_order(backward):

@@ -16,7 +16,7 @@ from torch.autograd import Function
 from torch.autograd.graph import increment_version
 
 from . import _lib
-from ._tensor import DTYPES, check_tensor, first_order, launch, on_device, ptr, wants_grad
+from ._tensor import DTYPES, check_tensor, first_order, has_tangent, launch, on_device, ptr, wants_grad
 
 MAX_HEAD = 128
 _ARRAYS = {n: ctypes.c_longlong * n for n in (6, 9, 12)}
@@ -128,14 +128,14 @@ def linear_attention(q, k, v, log_decay, *, state=None, lengths=None, scale: Opt
     (a chunk meets as one product); sequences of the batch do not touch one another."""
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("log_decay is a constant of the layer: there is no gradient for it")
-    if wants_grad(q, k, v, state):
+    if wants_grad(q, k, v, state) or has_tangent(log_decay):
         return LinearAttentionFunction.apply(q, k, v, log_decay, state, lengths, scale)
     return forward(_rows(q), _rows(k), _rows(v), log_decay, None if state is None else state.contiguous(), lengths, scale)[:2]
 
 
 def step(q, k, v, log_decay, state, *, scale: Optional[float] = None):
     """One token: q, k [B, H, Dk], v [B, H, Dv] -> out [B, H, Dv]; state [B, H, Dk, Dv] is updated in place.  No gradient."""
-    if wants_grad(q, k, v, state):
+    if wants_grad(q, k, v, state) or has_tangent(log_decay):
         raise RuntimeError("step keeps no gradient: call it under torch.no_grad()")
     q, k, v = _rows(q), _rows(k), _rows(v)
     if state is None:

@@ -165,3 +165,49 @@ def test_training_step_in_a_graph():
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert rel(a, b) <= 2.0 ** -16                    # the library's products may split their sums differently
+
+
+# ---- forward-mode derivatives ------------------------------------------------------------------------------------
+def _forward_mode_calls(device):
+    import torch.autograd.forward_ad as fwd
+    from customnetworklayers_b200 import blocknorm, ckpt8, linattn
+    r = lambda *s: torch.randn(*s, device=device)  # noqa: E731
+    dual = lambda *s: fwd.make_dual(r(*s), r(*s))  # noqa: E731
+    x, q, decay, w = r(4, 16), r(1, 5, 2, 8), -torch.ones(2, device=device), torch.ones(16, device=device)
+    state = torch.zeros(1, 2, 8, 8, device=device)
+    return [lambda: ckpt8.activation(dual(4, 16)), lambda: blocknorm.pre_norm(dual(4, 16), w), lambda: blocknorm.pre_norm(x, dual(16)),
+            lambda: blocknorm.residual_norm(x, dual(4, 16), w), lambda: blocknorm.residual_norm(x, x, w, gate=dual(4, 16)),
+            lambda: blocknorm.residual_norm(x, x, w, scale=dual(16)), lambda: blocknorm.residual_norm(x, x, w, next_weight=dual(16)),
+            lambda: linattn.linear_attention(dual(1, 5, 2, 8), q, q, decay), lambda: linattn.linear_attention(q, q, dual(1, 5, 2, 8), decay),
+            lambda: linattn.linear_attention(q, q, q, dual(2)), lambda: linattn.linear_attention(q, q, q, decay, state=dual(1, 2, 8, 8)),
+            lambda: linattn.step(dual(1, 2, 8), q[:, 0], q[:, 0], decay, state), lambda: linattn.step(q[:, 0], q[:, 0], q[:, 0], dual(2), state),
+            lambda: linattn.step(q[:, 0], q[:, 0], q[:, 0], decay, dual(1, 2, 8, 8))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(grad):
+    # as the optimisation layers refuse it; a result without its tangent would pass for a derivative of zero
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level(), torch.set_grad_enabled(grad):
+        for i, call in enumerate(_forward_mode_calls("cuda")):
+            with pytest.raises(RuntimeError):             # NotImplementedError is one
+                call()
+                pytest.fail(f"call {i} came back")
+
+
+def test_inputs_with_a_tangent_want_a_derivative():
+    import torch.autograd.forward_ad as fwd
+    from customnetworklayers_b200 import linattn
+    from customnetworklayers_b200._tensor import wants_grad
+    x = torch.ones(1, 2, 8)
+    assert not wants_grad(x, None)
+    with fwd.dual_level():
+        assert not wants_grad(x, None)
+        d = fwd.make_dual(x, x)
+        assert wants_grad(None, x, d)
+        with torch.no_grad():
+            assert wants_grad(d)
+        with pytest.raises(RuntimeError, match="no gradient"):
+            linattn.step(d, x, x, torch.zeros(2), torch.zeros(1, 2, 8, 8))
+    assert not wants_grad(d)
