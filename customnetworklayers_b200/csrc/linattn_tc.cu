@@ -874,7 +874,8 @@ int run_sweep_tc(const Sweep& s, cudaStream_t st) {
 }  // namespace cnl
 
 extern "C" int cnl_linattn_status(void) {
+    // the copy alone would wait for the default stream and not for those that are independent of it
     int v = 0;
-    if (cudaMemcpyFromSymbol(&v, cnl::lin::g_gave_up, sizeof(int)) != cudaSuccess) { cudaGetLastError(); return -1; }
+    if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyFromSymbol(&v, cnl::lin::g_gave_up, sizeof(int)) != cudaSuccess) { cudaGetLastError(); return -1; }
     return v;
 }

@@ -333,8 +333,9 @@ int cnl_blocknorm_backward(const void* x, const void* u, const void* gate, const
  * updated in place.
  */
 int cnl_linattn_segments(int b, int t, int h, int dk, int dv, int dtype);
-/* 1 if a block of the current device's sweeps has ever given up waiting for its own copies or products (its outputs are NaN
- * then), 0 if none, negative on error.  Waits for the device. */
+/* 1 if a block of the current device's sweeps has given up waiting for its own copies or products since the library was loaded
+ * (its outputs are NaN then; the mark stays), 0 if none, negative on error.  Waits for all work of the device on every stream;
+ * not for use while a stream is being captured. */
 int cnl_linattn_status(void);
 int cnl_linattn_forward(const void* q, const void* k, const void* v, const long long* strides_host, const float* log_decay,
                         const int* lengths, const float* state, void* out, float* state_out, float* starts, int b, int t, int h,

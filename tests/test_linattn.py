@@ -573,3 +573,19 @@ def test_16_bit_results_carry_their_own_rounding_alone(t, dk, dv, dtype):
     for name, a, w, m in zip(("out", "gradient of q", "gradient of k", "gradient of v"), got, want, [mags[0], *mags[2:5]]):
         mag = m / (2 * HALF[dtype] + 512 * 2.0 ** -24)
         assert_within(a, w, HALF[dtype] * w.abs() + (3 * part + 512 * 2.0 ** -24) * mag + TINY[dtype], name)
+
+
+@pytest.mark.gpu
+def test_the_status_waits_for_every_stream():
+    # torch's streams do not wait for the default stream, nor it for them
+    x, decay, _, _ = make(2, 7680, 8, 64, 64, torch.bfloat16, seed=14, state=False)
+    q, k, v, decay = x["q"].cuda(), x["k"].cuda(), x["v"].cuda(), -torch.exp2(-torch.linspace(1, 8, 8)).cuda()
+    linattn.linear_attention(q, k, v, decay)
+    side, done = torch.cuda.Stream(), torch.cuda.Event()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(200):
+            linattn.linear_attention(q, k, v, decay)
+        done.record()
+    assert _lib.load().cnl_linattn_status() == 0
+    assert done.query()
