@@ -589,3 +589,29 @@ def test_the_status_waits_for_every_stream():
         done.record()
     assert _lib.load().cnl_linattn_status() == 0
     assert done.query()
+
+
+# ---- rows behind the end in the kernels that load them -----------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dk,dv", [(64, 64), (64, 128), (128, 64), (128, 128), (40, 72)])
+@pytest.mark.parametrize("t,lengths", [(200, [130, 0]), (300, [130, 257]), (300, [0, 299]), (1300, [1111, 129]), (1300, [0, 513]), (128, [127, 1])])
+def test_wide_rows_behind_the_end_may_hold_anything(t, lengths, dk, dv):
+    """As test_rows_behind_the_end_are_not_read, at the sizes whose kernels bring whole chunks: whatever stands behind a length
+    gives the same bits as zeros there.  Cut chunks, one and several segments, both directions."""
+    x, decay, do, ds = make(2, t, 2, dk, dv, torch.bfloat16, seed=t + dk + dv)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    res = []
+    for bad in (0.0, float("nan"), float("inf")):
+        d = {k: v.clone().cuda() for k, v in x.items()}
+        g = do.clone().cuda()
+        for z in (d["q"], d["k"], d["v"], g):
+            for i, m in enumerate(lengths):
+                z[i, m:] = bad
+        for v in d.values():
+            v.requires_grad_(True)
+        o, end = linattn.linear_attention(d["q"], d["k"], d["v"], decay.cuda(), state=d["state"], lengths=n)
+        res.append([o, end, *torch.autograd.grad((o, end), list(d.values()), (g, ds.cuda()))])
+    for other in res[1:]:
+        for a, b in zip(res[0], other):
+            assert torch.isfinite(a).all() and torch.equal(a, b)
+    assert _lib.load().cnl_linattn_status() == 0
