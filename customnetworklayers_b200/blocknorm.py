@@ -27,7 +27,7 @@ MAX_CHANNELS = 8192
 
 
 def _gate_mode(x, gate):
-    """(mode, groups): 0 no gate, 1 of x's shape, 2 shared by the rows of each of `groups` groups."""
+    """(mode, groups): 0 no gate (or none to read), 1 of x's shape, 2 shared by the rows of each of `groups` groups."""
     if gate is None:
         return 0, 1
     if gate.dim() > x.dim() or gate.dim() < 1 or gate.shape[-1] != x.shape[-1]:
@@ -42,7 +42,7 @@ def _gate_mode(x, gate):
     if any(n != 1 for n in lead[i:]):
         raise RuntimeError(f"gate {list(gate.shape)} must have x's shape {list(x.shape)}, or size 1 in all dimensions between "
                            "some leading ones and the last")
-    return 2, groups
+    return (2, groups) if groups else (0, 1)     # the gates of no images: there is no row either
 
 
 def _check(x, u, gate, scale, weight, bias, next_weight, next_bias):

@@ -363,3 +363,25 @@ def test_refusals_on_the_device():
                  lambda: blocknorm.residual_norm(x, x, None, next_weight=w), lambda: blocknorm.pre_norm(x.double(), w.double())):
         with pytest.raises(RuntimeError):
             call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [None, "int8"])
+@pytest.mark.parametrize("shape,gate", [((0, 5, 16), (0, 1, 16)), ((0, 5, 16), (1, 1, 16)), ((3, 0, 16), (3, 1, 16)), ((0, 4, 6, 16), (0, 1, 1, 16)),
+                                        ((0, 4, 6, 16), (0, 4, 1, 16)), ((3, 0, 16), (16,))])
+def test_no_rows_with_a_gate_for_each_image(shape, gate, fmt):
+    t, up = make(shape, torch.float32, gate=gate)
+    outs, grads = run(t, up, checkpoint=fmt)
+    assert outs["y"].shape == outs["h"].shape == shape and grads["x"].shape == grads["u"].shape == shape
+    assert grads["gate"].shape == gate and torch.count_nonzero(grads["gate"]) == 0
+    for k in ("weight", "bias", "scale", "next_weight", "next_bias"):
+        assert torch.count_nonzero(grads[k]) == 0 and grads[k].shape == (16,)
+
+
+def test_gates_of_no_images():
+    mode = lambda x, g: blocknorm._gate_mode(torch.zeros(*x), torch.zeros(*g))  # noqa: E731
+    assert mode((0, 5, 8), (0, 1, 8)) == (0, 1) and mode((0, 5, 8), (0, 5, 8)) == (1, 1) and mode((0, 5, 8), (1, 1, 8)) == (2, 1)
+    assert mode((3, 0, 8), (3, 1, 8)) == (2, 3)
+    for x, g in (((0, 5, 8), (2, 1, 8)), ((2, 5, 8), (0, 1, 8)), ((0, 5, 8), (0, 2, 8))):
+        with pytest.raises(RuntimeError):
+            mode(x, g)
