@@ -169,7 +169,7 @@ class LinearAttention(nn.Module):
 
     def forward(self, x, state=None, lengths=None):
         n, c = x.shape[0], x.shape[-1]
-        q, k, v = self.qkv(x).view(n, -1, 3, self.heads, c // self.heads).unbind(2)
+        q, k, v = self.qkv(x).view(n, x.shape[1:-1].numel(), 3, self.heads, c // self.heads).unbind(2)
         o, state = linear_attention(q, k, v, self.log_decay.float(), state=state, lengths=lengths)
         return self.out(o.reshape(x.shape)), state
 
@@ -178,5 +178,5 @@ class LinearAttention(nn.Module):
         return torch.zeros(n, self.heads, d, d, dtype=torch.float32, device=self.log_decay.device)
 
     def step(self, x, state):
-        q, k, v = self.qkv(x).view(x.shape[0], 3, self.heads, -1).unbind(1)
+        q, k, v = self.qkv(x).view(x.shape[0], 3, self.heads, x.shape[-1] // self.heads).unbind(1)
         return self.out(step(q, k, v, self.log_decay.float(), state).reshape(x.shape))

@@ -211,3 +211,17 @@ def test_inputs_with_a_tangent_want_a_derivative():
         with pytest.raises(RuntimeError, match="no gradient"):
             linattn.step(d, x, x, torch.zeros(2), torch.zeros(1, 2, 8, 8))
     assert not wants_grad(d)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(0, 6, 32), (0, 3, 4, 32), (2, 0, 32), (0, 0, 5, 32)])
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_empty_batches_and_images(shape, checkpoint):
+    m = PixelMixer(32, 2, depth=2, checkpoint=checkpoint).cuda()
+    x = torch.zeros(*shape, device="cuda", requires_grad=True)
+    y, states = m(x, m.new_states(shape[0]))
+    assert y.shape == shape and all(s.shape == (shape[0], 2, 16, 16) for s in states)
+    y.sum().backward()
+    assert x.grad.shape == shape and all(torch.count_nonzero(p.grad) == 0 for p in m.parameters())
+    states = m.new_states(0)
+    assert m.step(torch.zeros(0, 32, device="cuda"), states).shape == (0, 32)
