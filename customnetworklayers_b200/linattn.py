@@ -156,7 +156,7 @@ class LinearAttention(nn.Module):
     """Token mixer over [N, T, C] or [N, H, W, C] (pixels in raster order): projections, linear attention, projection.
 
     forward(x, state=None, lengths=None) -> (out, state); step(x [N, C], state) -> out.  Memories of the heads run from
-    2^first to 2^last tokens."""
+    2^first to 2^last tokens; the decays stay fp32 whatever type the module is brought to."""
 
     def __init__(self, channels: int, heads: int, first: float = 2.0, last: float = 11.0):
         super().__init__()
@@ -165,7 +165,14 @@ class LinearAttention(nn.Module):
         self.heads = heads
         self.qkv = nn.Linear(channels, 3 * channels, bias=False)
         self.out = nn.Linear(channels, channels, bias=False)
-        self.register_buffer("log_decay", -torch.exp2(-torch.linspace(first, last, heads)))
+        self.register_buffer("log_decay", -torch.exp2(-torch.linspace(first, last, heads, dtype=torch.float32)))
+
+    def _apply(self, fn, recurse=True):
+        decay = self.log_decay
+        super()._apply(fn, recurse)
+        if self.log_decay.dtype != torch.float32:        # the weights' type is not the memories': bf16 would change their lengths
+            self.log_decay = decay.to(self.log_decay.device)
+        return self
 
     def forward(self, x, state=None, lengths=None):
         n, c = x.shape[0], x.shape[-1]

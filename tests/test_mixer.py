@@ -225,3 +225,39 @@ def test_empty_batches_and_images(shape, checkpoint):
     assert x.grad.shape == shape and all(torch.count_nonzero(p.grad) == 0 for p in m.parameters())
     states = m.new_states(0)
     assert m.step(torch.zeros(0, 32, device="cuda"), states).shape == (0, 32)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float64])
+def test_memories_keep_their_length_in_every_type(dtype):
+    m = PixelMixer(64, 8, depth=2)
+    want = -torch.exp2(-torch.linspace(2.0, 11.0, 8))
+    state = m.state_dict()
+    for net in (m.to(dtype), copy.deepcopy(m), m.float(), m.to(dtype).to("cpu")):
+        for a in net.attention:
+            assert a.log_decay.dtype == torch.float32 and torch.equal(a.log_decay, want)
+    m.half().load_state_dict({k: v.clone() for k, v in state.items()})
+    assert all(torch.equal(a.log_decay, want) for a in m.attention) and m.gate[0].weight.dtype == torch.float16
+    try:
+        torch.set_default_dtype(dtype)
+        assert torch.equal(PixelMixer(64, 8, depth=1).attention[0].log_decay, want)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    with torch.device("meta"):
+        empty = PixelMixer(64, 8, depth=1)
+    assert empty.to(dtype).to_empty(device="cpu").attention[0].log_decay.dtype == torch.float32
+
+
+@pytest.mark.gpu
+def test_a_bf16_mixer_is_the_fp32_one_with_rounded_weights():
+    """Against 64 bits with the decays of the fp32 model: projections, norms and attention round 2^-8 some 20 times; a decay of
+    2^-9 too much or too little for each token would add 2^-9 times the memory's length over what it holds."""
+    torch.manual_seed(6)
+    m = PixelMixer(64, 8, depth=1).cuda()
+    want = [a.log_decay.clone() for a in m.attention]
+    m = m.to(torch.bfloat16)
+    x = torch.randn(1, 2000, 64, device="cuda").bfloat16()
+    with torch.no_grad():
+        y, ends = m(x)
+    m2, _, y2, ends2 = reference(m, x)
+    assert all(torch.equal(a.log_decay.float(), w) for a, w in zip(m2.attention, want))
+    assert rel(y, y2) <= 2.0 ** -5 and all(rel(a, b) <= 2.0 ** -5 for a, b in zip(ends, ends2))
