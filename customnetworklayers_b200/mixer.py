@@ -6,7 +6,8 @@
 
 Runs [N, H, W, C] images (pixels in raster order) or [N, T, C] sequences at once, or one token at a time with the state of
 every block kept by the caller.  `checkpoint` ("int8", "e4m3") keeps what the norms and the MLP's activation save for the
-backward pass in 8 bits.  The projections are plain library products."""
+backward pass in 8 bits.  The projections are plain library products; under torch.autocast they, the attention and the
+activation run in 16 bits, the norms and the stream in the type of x."""
 from __future__ import annotations
 
 from typing import Optional
@@ -39,8 +40,9 @@ class PixelMixer(nn.Module):
     def _blocks(self, x, mix):
         h = self.pre(x)
         for i, gate in enumerate(self.gate):
-            x, h = self.after_attention[i](x, mix(i, h), gate(h))
-            out = self.after_mlp[i](x, self.down[i](self.act(self.up[i](h))))
+            # (under autocast the projections leave 16 bits, the stream stays as it is)
+            x, h = self.after_attention[i](x, mix(i, h).to(x.dtype), gate(h).to(x.dtype))
+            out = self.after_mlp[i](x, self.down[i](self.act(self.up[i](h))).to(x.dtype))
             x, h = out if i + 1 < len(self.gate) else (out, None)
         return x
 

@@ -261,3 +261,28 @@ def test_a_bf16_mixer_is_the_fp32_one_with_rounded_weights():
     m2, _, y2, ends2 = reference(m, x)
     assert all(torch.equal(a.log_decay.float(), w) for a, w in zip(m2.attention, want))
     assert rel(y, y2) <= 2.0 ** -5 and all(rel(a, b) <= 2.0 ** -5 for a, b in zip(ends, ends2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_mixed_precision(dtype, checkpoint):
+    """fp32 parameters and stream under autocast: the projections, the attention and the activation run in 16 bits."""
+    torch.manual_seed(7)
+    m = PixelMixer(32, 2, depth=2, checkpoint=checkpoint).cuda()
+    x = torch.randn(2, 150, 32, device="cuda", requires_grad=True)
+    params = list(m.parameters())
+    y, ends = m(x)
+    up = torch.randn_like(y)
+    want = torch.autograd.grad(y, [x, *params], up)
+    with torch.autocast("cuda", dtype=dtype):
+        y2, ends2 = m(x)
+        with torch.no_grad():
+            one = m.step(x[:, 0], m.new_states(2))
+            first, _ = m(x[:, :1])
+    got = torch.autograd.grad(y2, [x, *params], up)
+    assert y2.dtype == torch.float32 and all(e.dtype == torch.float32 for e in ends2) and one.dtype == torch.float32
+    # half a step of the type (2^-8 at most) in each of some twenty projections, attentions and activations in a row
+    assert 0 < rel(y2, y) <= 2.0 ** -4 and rel(one, first[:, 0]) <= 2.0 ** -4
+    for a, b in zip(got, want):
+        assert a.dtype == torch.float32 and rel(a, b) <= 2.0 ** -3
