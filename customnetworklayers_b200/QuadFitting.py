@@ -7,6 +7,7 @@ from torch import nn
 from torch.autograd import Function
 
 from . import QuadFit_cuda_ext, ckpt8
+from ._tensor import wants_grad
 
 
 class QuadFittingFromFlowFunction(Function):
@@ -58,7 +59,7 @@ class QuadFittingFromFlow(nn.Module):
         self.checkpoint = checkpoint
 
     def _fit(self, feat0, feat1, flow):
-        if self.checkpoint is None:
+        if self.checkpoint is None or not wants_grad(feat0, feat1, flow):      # nothing to put away
             return QuadFittingFromFlowFunction.apply(feat0, feat1, flow)
         return QuadFittingFromFlow8Function.apply(feat0, feat1, flow, self.checkpoint)
 

@@ -251,3 +251,25 @@ def test_activation_at_the_ends_of_the_line(n, kind, dtype):
         y2 = ckpt8.activation(dev.clone().requires_grad_(True), kind, "e4m3").detach()
         for got in (y, y2):
             assert_within(got, ref, 2.0 ** -18 * torch.ones(n, dtype=torch.float64) + HALF[dtype] * ref.abs().nan_to_num(0, 0, 0), "y")
+
+
+@pytest.mark.gpu
+def test_quadfit_puts_nothing_away_where_no_gradient_is_wanted():
+    from customnetworklayers_b200.QuadFitting import QuadFittingFromFlow
+    g = torch.Generator(device="cuda").manual_seed(5)
+    f0, f1 = (torch.randn(1, 12, 20, 4, generator=g, device="cuda") for _ in range(2))
+    flow = torch.rand(1, 12, 20, 2, generator=g, device="cuda")
+    fit = QuadFittingFromFlow("cuda", checkpoint="int8")
+    lib = _lib.load()
+
+    def launches(*maps):
+        before = lib.cnl_launch_count()
+        sol = fit(*maps)
+        return lib.cnl_launch_count() - before, sol
+
+    plain, want = launches(f0, f1, flow)
+    with torch.no_grad():
+        n, sol = launches(f0.clone().requires_grad_(True), f1, flow)
+    assert n == plain == 1 and torch.equal(sol, want)
+    n, sol = launches(f0, f1.clone().requires_grad_(True), flow)
+    assert n == plain + 2 and torch.equal(sol, want)               # one map's gradient needs both maps
