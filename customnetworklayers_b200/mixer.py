@@ -17,6 +17,7 @@ from torch import nn
 
 from .blocknorm import PreNorm, ResidualNorm
 from .ckpt8 import Activation8
+from .dist import allreduce_scalar_grads
 from .linattn import LinearAttention
 
 
@@ -64,3 +65,9 @@ class PixelMixer(nn.Module):
     def step(self, x, states):
         """x [N, C]: one token; states (from new_states or forward) are updated in place."""
         return self._blocks(x, lambda i, h: self.attention[i].step(h, states[i]))
+
+    def allreduce_parameter_grads(self) -> None:
+        """Data-parallel step: sum the parameter gradients, the projections' among them, over all ranks."""
+        for p in self.parameters():
+            if p.grad is not None:
+                allreduce_scalar_grads(p.grad)

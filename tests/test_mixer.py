@@ -286,3 +286,48 @@ def test_mixed_precision(dtype, checkpoint):
     assert 0 < rel(y2, y) <= 2.0 ** -4 and rel(one, first[:, 0]) <= 2.0 ** -4
     for a, b in zip(got, want):
         assert a.dtype == torch.float32 and rel(a, b) <= 2.0 ** -3
+
+
+# ---- several ranks -----------------------------------------------------------------------------------------------
+def _sum_gradients(rank, world, port, q):
+    import os
+    import torch.distributed as dist
+    from customnetworklayers_b200.blocknorm import ResidualNorm
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    torch.set_num_threads(1)
+    torch.manual_seed(0)
+    nets = [PixelMixer(16, 2, depth=1), ResidualNorm(16, bias=True)]
+    g = torch.Generator().manual_seed(rank)
+    own = []
+    for net in nets:
+        for i, p in enumerate(net.parameters()):
+            if i != 1:                                   # a parameter without a gradient stays so
+                p.grad = torch.randn(p.shape, generator=g)
+            own.append(None if p.grad is None else p.grad.clone())
+        net.allreduce_parameter_grads()
+    got = [p.grad for net in nets for p in net.parameters()]
+    q.put((rank, [None if t is None else t.numpy() for t in own], [None if t is None else t.numpy() for t in got]))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def test_two_ranks_sum_the_gradients_of_all_parameters():
+    import socket
+    import torch.multiprocessing as mp
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_sum_gradients, args=(r, 2, port, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    (_, own0, got0), (_, own1, got1) = sorted((q.get(timeout=120) for _ in procs), key=lambda r: r[0])
+    for p in procs:
+        p.join(timeout=60)
+        assert p.exitcode == 0
+    assert len(own0) > 10 and sum(t is None for t in got0) == 2
+    for a, b, x, y in zip(own0, own1, got0, got1):
+        if a is not None:
+            assert (a + b == x).all() and (x == y).all()
