@@ -273,3 +273,32 @@ def test_quadfit_puts_nothing_away_where_no_gradient_is_wanted():
     assert n == plain == 1 and torch.equal(sol, want)
     n, sol = launches(f0, f1.clone().requires_grad_(True), flow)
     assert n == plain + 2 and torch.equal(sol, want)               # one map's gradient needs both maps
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_what_an_activation_keeps_for_its_backward_pass(fmt):
+    n = 1 << 22
+    x = torch.randn(n, device="cuda", requires_grad=True)
+    y = ckpt8.activation(x * 1.0, "gelu", fmt)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    y.detach_()                                            # lets go of the graph and of what it keeps
+    kept = before - torch.cuda.memory_allocated()
+    assert n * (1 + 1 / 32) <= kept <= n * (1 + 1 / 32) + 512
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["gelu", "silu"])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_the_two_passes_without_autograd(fmt, kind):
+    g = torch.Generator(device="cuda").manual_seed(9)
+    x, dy = (torch.randn(3, 77, 9, generator=g, device="cuda").half() for _ in range(2))
+    y, stored = ckpt8.forward(x, kind, fmt)
+    dx = ckpt8.backward(stored, dy, kind)
+    leaf = x.clone().requires_grad_(True)
+    want = ckpt8.activation(leaf, kind, fmt)
+    assert torch.equal(y, want) and torch.equal(dx, torch.autograd.grad(want, leaf, dy)[0])
+    assert torch.equal(stored.codes, ckpt8.store(x, fmt).codes) and stored.shape == x.shape
+    with pytest.raises(RuntimeError, match="shape"):
+        ckpt8.backward(stored, dy[:1].clone(), kind)
