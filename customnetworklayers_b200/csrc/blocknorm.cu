@@ -487,7 +487,6 @@ inline int plan(long long rows, int d, long long groups, bool vec, int blocks_wa
         while (p->tpr < need) p->tpr <<= 1;
     }
     p->block = p->tpr <= 256 ? 256 / p->tpr * p->tpr : p->tpr;
-    if (p->tpr > 32 && p->tpr <= 256) p->block = 256 / p->tpr * p->tpr;
     p->rpb = p->block / p->tpr;
     p->groups = groups;
     const long long per = rows / groups, most = (per + p->rpb - 1) / p->rpb;

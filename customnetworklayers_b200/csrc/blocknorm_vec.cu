@@ -6,8 +6,10 @@
 // (s w and s b, since s, w, b only appear so), and rows arrive by cp.async in shared-memory slots that belong to one thread
 // each: it waits for its own copies, needs no barrier, and STAGES - 1 rows are under way while one is worked on.
 // 61440 x 512 bf16 with a full gate: rms forward 60 us (5.2 TB/s, 0.8 of a copy), layer norm with biases 84 us (two blocks an SM
-// instead of three; three with spills 90); backward 160 and 167 us (3.0 TB/s); with 8-bit checkpoints 117 and 187 us.  Wide or
-// narrow rows run alike (32: 64 and 153, 4096: 74 and 196 us for as many elements).  Instructions issue on half of the cycles at 16
+// instead of three; three with spills 90); backward 110 us without biases (4.6 TB/s), with them 160 and 167 us (3.0 TB/s); with
+// 8-bit checkpoints and biases 117 and 187 us.  Wide or narrow rows run alike (with biases, 32: 64 and 153, 4096: 74 and 196 us for as many elements).
+// fp32 with a full gate, rms: 152 and 261 us (4.1 and 3.9 TB/s; two rows under way instead of three), 30720 x 1024 150 and 265 us.  A norm
+// alone: bf16 34 and 71 us, fp32 66 and 112 us.  Instructions issue on half of the cycles at 16
 // warps an SM; mean and squares in one way through the row instead of two left all of these times as they are.
 #include "blocknorm.cuh"
 
@@ -272,7 +274,8 @@ __global__ void __launch_bounds__(BLOCK, BLOCK == 512 ? 1 : BIAS ? 2 : 3) forwar
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------
-// BIAS: some bias has a gradient, or the scale's needs one, so the sums of t a and of dh are kept too.
+// BIAS: a bias takes part or its gradient is asked for, so the sums of t a and of dh are kept too (without: 110 us where the
+// rms norm of 61440 x 512 bf16 takes 160).
 template <typename T, bool WIDE, bool LAYER, bool BIAS, int BLOCK>
 __global__ void __launch_bounds__(BLOCK, 512 / BLOCK) backward_vec(const Args a) {
     using S = Slots<T, 5, BLOCK>;

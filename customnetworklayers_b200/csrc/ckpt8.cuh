@@ -19,7 +19,7 @@ namespace ckpt8 {
 
 constexpr int kBlock = 32;
 
-// s of a block from the bits of max |x|; sets `odd` when an element is not finite (its bits are the maximum then).
+// s of a block from the bits of its largest finite |x|.
 template <int FMT>
 __device__ __forceinline__ int exponent_of(unsigned top) {
     const int e = (int)(top >> 23) - 127;                        // -127 for subnormals: held to -126 below either way

@@ -19,10 +19,10 @@
 // (1 x 122880 x 8 x 64 forward 194 instead of 216 us, 8 x 7680 x 8 x 128 backward 451 instead of 497 us) at 1.4 times the error: 2.35e-3 rms of
 // the outputs against 1.66e-3, which the outputs' own rounding is.
 //
-// Measured, bf16 (one sweep with its outputs; the sums of all launches of a call are in the drivers' comment): 1 x 122880 tokens
-// x 8 heads of 64 122 us (rows 252 MB in and out: 2.1 TB/s), 8 x 7680 x 8 x 128 117 us.  Tensor
-// pipes are active on 24 to 32 % of cycles, instructions issue on 36 to 42 %: what bounds a chunk is the chain weights -> P ->
-// outputs with 16 warps to hide it, and the operands' way through shared memory; a second block would not fit either memory.
+// Measured, bf16 (one sweep with its outputs; beside it a call's states take 61 and 64 us, a scan 12 to 20): 1 x 122880 tokens x 8
+// heads of 64 148 us, 8 x 7680 x 8 x 128 134 us (rows of 503 MB in and out: 3.4 and 3.8 TB/s).  Tensor pipes are active on 28 to
+// 39 % of cycles, instructions issue on 35 to 43 %: what bounds a chunk is the chain weights -> P -> outputs with 16 warps to hide
+// it, and the operands' way through shared memory; a second block would not fit either memory.
 //
 // Every wait is bounded: a block that gives up marks the status word, fills what it owes with NaN, and returns after its
 // copies and products have ended.
@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const Sweep s, const 
         {
             const float* w0 = s.start ? s.start + ((long long)bh * s.segments + seg) * size : nullptr;
             const bool has = w0 && wrow < dc && (!kStack || row < 64);
-            // (a transposed state by vectors, as its rows lie apart: 8 x 7680 x 8 x 128, 1 float at a time 131 us, 4 at a time 119 us)
+            // (a transposed state by vectors, as its rows lie apart: 8 x 7680 x 8 x 128, 4 floats at a time 12 us less than 1 at a time)
             if (s.transposed && ((unsigned long long)w0 & 15) == 0) {
 #pragma unroll
                 for (int x = 0; x < HC; x += 4) {
@@ -852,9 +852,9 @@ int run_tc(Sweep s, cudaStream_t st) {
     return exact ? launch_state<DA, DC, 3>(s, st) : launch_state<DA, DC, 2>(s, st);
 }
 
-// Measured against the mma.sync sweep (forward / backward, us): 64 x 128 tokens x 8 heads of 128 65 / 95 against 64 / 169, of 64
-// 33 / 75 against 29 / 73; 1 x 128 of 64 11 / 26 against 12 / 34; 16 x 1024 of 64 31 / 73 against 65 / 146; 8 x 7680 of 128
-// 190 / 403 against 474 / 1146.  Heads of 32 would fill half of its tiles; shorter sequences less than one chunk.
+// Measured against the mma.sync sweep (forward / backward, us): 64 x 128 tokens x 8 heads of 128 69 / 159 against 76 / 259, of 64
+// 34 / 89 against 29 / 77; 1 x 128 of 64 12 / 29 against 14 / 36; 16 x 1024 of 64 33 / 85 against 67 / 144; 8 x 7680 of 128
+// 204 / 458 against 544 / 1304.  Heads of 32 would fill half of its tiles; shorter sequences less than one chunk.
 bool tc_sizes(int t, int da, int dc, int dtype) { return dtype == CNL_BF16 && t >= kTok && da > 32 && dc > 32 && da % 8 == 0 && dc % 8 == 0; }
 
 bool tc_serves(const Sweep& s, int dtype) {
